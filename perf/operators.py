@@ -146,10 +146,12 @@ def _moe_inputs(case: dict, seed: int) -> list[tuple[torch.Tensor, torch.Tensor]
 
 
 def _pack(case: dict, layer: dict) -> torch.Tensor:
-    """The resident slots [E, bytes]: gate, up and down codes, then their scales in that order."""
+    """The resident slots [E, bytes]: gate, up and down codes, then their scales in that order, filled up
+    to a multiple of 16 bytes."""
     E = case["E"]
     parts = [layer[n][0] for n in ("gate", "up", "down")] + [layer[n][1] for n in ("gate", "up", "down")]
-    return torch.cat([p.reshape(E, -1).view(torch.uint8) for p in parts], 1)
+    slots = torch.cat([p.reshape(E, -1).view(torch.uint8) for p in parts], 1)
+    return torch.nn.functional.pad(slots, (0, -slots.shape[1] % 16))
 
 
 def _mode(case: dict) -> str:
