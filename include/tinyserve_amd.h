@@ -45,7 +45,7 @@ typedef enum tsa_route_mode {
 
 typedef enum tsa_act { TSA_ACT_SILU = 0, TSA_ACT_SWIGLU_OAI = 1 } tsa_act;
 
-typedef enum tsa_expert_format { TSA_EXPERT_MXFP4 = 1, TSA_EXPERT_GGUF = 2 } tsa_expert_format;
+typedef enum tsa_expert_format { TSA_EXPERT_MXFP4 = 1, TSA_EXPERT_GGUF = 2, TSA_EXPERT_FP8 = 3 } tsa_expert_format;
 
 /* Where one expert's tensors sit inside a packed slot (byte offsets from the slot start).
  *  MXFP4 (GPT-OSS): gate_up blocks [2I, H/32, 16] u8 at gate_off (rows interleaved:
@@ -56,6 +56,12 @@ typedef enum tsa_expert_format { TSA_EXPERT_MXFP4 = 1, TSA_EXPERT_GGUF = 2 } tsa
  *    tsa_mxfp4_tile produces (the fast decode path); 0: the checkpoint order above.
  *  GGUF: gate [I x H] of gate_type at gate_off, up [I x H] of up_type at up_off,
  *    down [H x I] of down_type at down_off (GGUF has no biases; set them to -1).
+ *  FP8: gate [I, H], up [I, H] and down [H, I] as e4m3 codes at gate_off, up_off and down_off
+ *    (multiples of 16, as slot_bytes is); float32 scales, one per block of 128 x 128, at
+ *    gate_scales_off (gate's [ceil(I/128), ceil(H/128)], then up's) and at down_scales_off
+ *    ([ceil(H/128), ceil(I/128)]), both multiples of 4. No biases (-1). Pool, x and workspaces
+ *    16-byte aligned. Activations are quantised as tsa_fp8_quantize does, x before gate and up and
+ *    h = act(gate, up) (float32) before down.
  *  act: TSA_ACT_SWIGLU_OAI = (up+1)*g*sigmoid(alpha*g), g = min(gate, limit),
  *    up = clamp(up, -limit, limit); TSA_ACT_SILU = silu(gate)*up.
  *  prefill_mfma (tiled MXFP4 prefill GEMMs): TSA_PREFILL_FP6 (0, the default) multiplies the
@@ -131,6 +137,32 @@ int tsa_mxfp4_tile(const void* blocks, const void* scales, int64_t N, int64_t K,
 int tsa_mxfp4_matvec(const void* blocks, const void* scales, const void* bias, int bias_dtype,
                      const void* x, int x_dtype, int64_t T,
                      void* y, int y_dtype, int64_t N, int64_t K, void* stream);
+
+/* ---- FP8 with a float32 scale per block of 128 (no reference counterpart: the reference stores
+ * FP8 experts, but widens them before it computes). e4m3 is the OCP format (largest number 448, no
+ * infinities). A weight matrix w [N, K] has scales [ceil(N/128), ceil(K/128)]; a token's values
+ * have one scale per 128 columns. ---- */
+
+/* Quantise x [T, K] (any K): per token and group of 128 columns (the last one may be shorter)
+ *   scale = max(max|x| / 448, 2^-126),  code = e4m3(x / scale)
+ * with both quotients rounded to float32 and codes to the nearest, ties to even. codes [T, K],
+ * scales [T, ceil(K/128)]. A group that holds a NaN or an infinity has that as its scale. */
+int tsa_fp8_quantize(const void* x, int x_dtype, int64_t T, int64_t K, void* codes, float* scales, void* stream);
+
+/* y[t, n] = sum_b scales[t, b] w_scales[n/128, b] (sum over block b's k of codes[t, k] w[n, k])
+ * (+ bias[n], may be NULL): float32 sums, one rounding to y_dtype. K a multiple of 16 of at most
+ * 2^20; codes and w 16-byte aligned. */
+int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T, int64_t K, const void* w, const float* w_scales,
+                   int64_t N, const void* bias, int bias_dtype, void* y, int y_dtype, void* stream);
+
+/* Workspace bytes of tsa_fp8_linear (16-byte aligned, no initialisation). */
+int tsa_fp8_linear_workspace_size(int64_t T, int64_t K, int64_t* bytes);
+
+/* tsa_fp8_quantize of x [T, K] followed by tsa_fp8_matmul; few tokens are quantised inside the
+ * product's launch. x and w 16-byte aligned. */
+int tsa_fp8_linear(const void* x, int x_dtype, int64_t T, int64_t K, const void* w, const float* w_scales, int64_t N,
+                   const void* bias, int bias_dtype, void* y, int y_dtype, void* workspace, int64_t workspace_bytes,
+                   void* stream);
 
 /* Router top-k over logits [T, E] (logits_dtype F32/BF16/F16): idx [T, k] int32 and
  * weights [T, k] f32, descending, ties to the lower expert id.

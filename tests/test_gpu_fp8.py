@@ -1,0 +1,379 @@
+"""FP8 quantisation, products and MoE layers against their definition in 64 bits (fp8_ref)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import fp8_ref as ref
+from tinyserve_amd import ops, synth
+from tinyserve_amd.expert_forward import fp8_expert_layout
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def acts(seed, *shape, dtype=BF):
+    g = gen(seed)
+    x = torch.randn(shape, device=DEV, generator=g)
+    x *= torch.where(torch.rand(shape[-1], device=DEV, generator=g) < 1 / 64, 8.0, 1.0)
+    return x.to(dtype)
+
+
+def weights(seed, N, K):
+    """A matrix of N(0, 0.03) with its blocks' largest value at 448, as checkpoints have them."""
+    w = torch.zeros((ref.blocks(N) * 128, ref.blocks(K) * 128), device=DEV)
+    w[:N, :K] = 0.03 * torch.randn((N, K), device=DEV, generator=gen(seed))
+    b = w.view(ref.blocks(N), 128, ref.blocks(K), 128)
+    s = b.abs().amax((1, 3)) / 448
+    return (b / s[:, None, :, None]).view_as(w)[:N, :K].to(torch.float8_e4m3fn).contiguous(), s
+
+
+def same(a, b):
+    """Equal numbers, NaN where NaN."""
+    a, b = a.double(), b.double()
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+# ----------------------------------------------------------------------------- quantisation
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("T,K", [(1, 16), (1, 2880), (3, 128), (24, 2880), (7, 200), (5, 1), (2, 131), (257, 2048)])
+def test_quantize(T, K, dtype):
+    x = acts(T + K, T, K, dtype=dtype)
+    c, s = ops.fp8_quantize(x)
+    q64, s64 = ref.quantize(x.double())
+    assert c.shape == (T, K) and s.shape == (T, ref.blocks(K)) and c.dtype == torch.float8_e4m3fn
+    assert torch.equal(s.double(), s64) and torch.equal(c.double(), q64)
+
+
+def test_quantize_ties():
+    """Quotients that are borders between codes, to the even one: maximum 448 makes the scale 1."""
+    v = torch.arange(-447, 448, device=DEV).float() / 16
+    x = torch.cat([v, torch.zeros(-len(v) % 127, device=DEV)]).view(-1, 127)
+    x = torch.cat([torch.full((len(x), 1), 448.0, device=DEV), x], 1)
+    for dtype in (F32, HF, BF):
+        y = x.to(dtype)
+        c, s = ops.fp8_quantize(y)
+        assert torch.equal(s, torch.ones_like(s)) and torch.equal(c.double(), ref.e4m3(y.double()))
+
+
+def test_quantize_small_and_large():
+    """Zeros, numbers near the smallest float32 and large ones, groups beside each other (the steps of
+    row 2's linspace overflow: it holds infinities and NaN)."""
+    x = torch.zeros((6, 384), device=DEV)
+    x[1, 128:256] = torch.linspace(-1e-38, 1e-38, 128, device=DEV)
+    x[2, :128] = torch.linspace(-3e38, 3e38, 128, device=DEV)
+    x[3, 256:] = 1e-42
+    x[4, ::3] = 2.0**-120
+    x[5] = torch.linspace(1e-30, 1e30, 384, device=DEV)
+    for v in (x, x.to(BF)):
+        c, s = ops.fp8_quantize(v)
+        q64, s64 = ref.quantize(v.double())
+        assert same(s, s64) and same(c, q64)
+
+
+def test_quantize_largest():
+    """Numbers up to the largest float32."""
+    x = torch.linspace(0.5, 1.0, 256, device=DEV).view(2, 128) * torch.finfo(F32).max
+    for v in (x, -x, (x / 2).to(BF)):
+        c, s = ops.fp8_quantize(v)
+        q64, s64 = ref.quantize(v.double())
+        assert same(s, s64) and same(c, q64)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_quantize_not_finite(dtype):
+    """A NaN or an infinity takes its own group of its own token, and the product's row, no other."""
+    x = acts(3, 4, 256, dtype=dtype)
+    x[1, 5], x[2, 200] = float("nan"), float("inf")
+    c, s = ops.fp8_quantize(x)
+    d = c.float() * ref.spread(s, 256)
+    want = torch.zeros((4, 256), dtype=torch.bool, device=DEV)
+    want[1, :128] = want[2, 128:] = True
+    assert torch.equal(torch.isnan(d), want)
+    w, ws = weights(1, 48, 256)
+    for y in (ops.fp8_matmul(c, s, w, ws), ops.fp8_linear(x, w, ws)):
+        assert torch.isnan(y[1:3]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[3]).all()
+
+
+def test_quantize_views():
+    """Rows of a wider tensor, a start off the 16-byte boundary, leading dimensions, no token."""
+    x = acts(5, 6, 400)
+    for v in (x[:, 3:259], x.view(2, 3, 400)[..., :144], x.view(-1)[1 : 1 + 5 * 160].view(5, 160)):
+        c, s = ops.fp8_quantize(v)
+        c2, s2 = ops.fp8_quantize(v.reshape(-1, v.shape[-1]).clone())
+        assert torch.equal(c.view(torch.uint8), c2.view(torch.uint8)) and torch.equal(s, s2)
+    c, s = ops.fp8_quantize(x[:0])
+    assert c.shape == (0, 400) and s.shape == (0, 4)
+
+
+# ----------------------------------------------------------------------------- products
+SHAPES = [(1, 16, 16), (1, 2880, 2880), (3, 129, 144), (16, 96, 2048), (17, 200, 272), (5, 1, 128), (24, 257, 4096),
+          (33, 512, 16), (64, 300, 640), (77, 640, 2880), (129, 255, 1040), (200, 1000, 512), (513, 384, 384)]
+
+
+@pytest.mark.parametrize("T,N,K", SHAPES)
+@pytest.mark.parametrize("dtype,bias", [(BF, None), (F32, BF), (HF, F32)])
+def test_matmul(T, N, K, dtype, bias):
+    x, (w, ws) = acts(T + K, T, K), weights(N + K, N, K)
+    b = None if bias is None else torch.randn(N, device=DEV, generator=gen(9)).to(bias)
+    c, s = ops.fp8_quantize(x)
+    y = ops.fp8_matmul(c, s, w, ws, b, out_dtype=dtype)
+    want, err = ref.matmul(*ref.quantize(x.double()), w, ws, wide=dtype == F32)
+    if b is not None:
+        want, err = want + b.double(), err + b.double().abs() * 2.0**-23 + want.abs() * 2.0**-23
+    ref.check(y, want, err)
+
+
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 40, 300])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_linear(T, dtype):
+    """One call from values is the quantisation and the product in two, for any number of tokens."""
+    N, K = 272, 1424
+    x, (w, ws) = acts(T, T, K, dtype=dtype), weights(2, N, K)
+    b = torch.randn(N, device=DEV, generator=gen(1)).to(dtype)
+    y = ops.fp8_linear(x, w, ws, b)
+    want, err = ref.matmul(*ref.quantize(x.double()), w, ws, wide=dtype == F32)
+    ref.check(y, want + b.double(), err + (b.double().abs() + want.abs()) * 2.0**-23)
+
+
+def test_linear_scales_differ():
+    """Scales of neighbouring blocks and tokens that differ by powers of ten: each meets its own block."""
+    T, N, K = 40, 400, 656
+    x = acts(1, T, K) * (10.0 ** torch.randint(-6, 7, (T, ref.blocks(K)), device=DEV, generator=gen(2))).repeat_interleave(128, 1)[:, :K].to(BF)
+    w, ws = weights(3, N, K)
+    ws = ws * 10.0 ** torch.randint(-6, 7, ws.shape, device=DEV, generator=gen(4))
+    for T2 in (1, 16, T):
+        y = ops.fp8_linear(x[:T2], w, ws, out_dtype=F32)
+        ref.check(y, *ref.matmul(*ref.quantize(x[:T2].double()), w, ws, wide=True))
+
+
+def test_linear_one_nan_weight():
+    """A NaN code in a weight row makes that output NaN for every token and leaves the others."""
+    x, (w, ws) = acts(1, 20, 256), weights(2, 160, 256)
+    w.view(torch.uint8)[70, 100] = 0x7F
+    for T in (1, 20):
+        y = ops.fp8_linear(x[:T], w, ws)
+        assert torch.isnan(y[:, 70]).all() and int(torch.isnan(y).sum()) == T
+
+
+def test_linear_tokens_apart():
+    """A token's result does not depend on the tokens beside it in kernels of one kind."""
+    x, (w, ws) = acts(1, 16, 512), weights(2, 208, 512)
+    y = ops.fp8_linear(x, w, ws)
+    assert all(torch.equal(ops.fp8_linear(x[t : t + 1], w, ws), y[t : t + 1]) for t in range(16))
+
+
+def test_linear_views():
+    x, (w, ws) = acts(1, 20, 800), weights(2, 96, 400)
+    want = ops.fp8_linear(x[:, 3:403].clone(), w, ws)
+    assert torch.equal(ops.fp8_linear(x[:, 3:403], w, ws), want)
+    assert torch.equal(ops.fp8_linear(x[:, 3:403].unflatten(0, (4, 5)), w, ws), want)
+    off = torch.empty(w.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(96, 400)
+    off.copy_(w.view(torch.uint8))
+    wide = torch.zeros((4, 8), device=DEV)
+    wide[:1, ::2] = ws
+    assert torch.equal(ops.fp8_linear(x[:, 3:403], off, wide[:1, ::2]), want)
+    assert ops.fp8_linear(x[:0, :400], w, ws).shape == (0, 96)
+
+
+def test_linear_past_two_gib():
+    """Offsets past 31 bits: a weight of more than 2 GiB, and more than 2 GiB of results."""
+    N, K = 140000, 16384
+    w = torch.randint(0, 0x60, (N, K), dtype=torch.uint8, device=DEV, generator=gen(1))
+    ws = torch.rand((ref.blocks(N), 128), device=DEV, generator=gen(2)) * 1e-3
+    rows = torch.tensor([0, 1, 131071, 131072, 139998, 139999], device=DEV)
+    for T in (1, 40):
+        x = acts(3, T, K)
+        y = ops.fp8_linear(x, w, ws, out_dtype=F32)
+        W = (w[rows].view(torch.float8_e4m3fn).double() * ref.spread(ws.double()[rows // 128], K))
+        q, s = ref.quantize(x.double())
+        q = q * ref.spread(s, K)
+        ref.check(y[:, rows], q @ W.t(), (q.abs() @ W.abs().t()) * ref.unit(K))
+    del w
+    T, N, K = 9000, 131072, 16
+    x, (w, ws) = acts(4, T, K), weights(5, N, K)
+    y = ops.fp8_linear(x, w, ws)
+    want, err = ref.matmul(*ref.quantize(x[-300:].double()), w[-512:], ws[-4:])
+    ref.check(y[-300:, -512:], want, err)
+
+
+# ----------------------------------------------------------------------------- MoE layers
+def experts(seed, E, H, I):
+    out = []
+    for e in range(E):
+        d = {}
+        for i, (n, r, c) in enumerate((("gate_proj", I, H), ("up_proj", I, H), ("down_proj", H, I))):
+            d[n], d[n + "_scale_inv"] = weights(seed + 10 * e + i, r, c)
+        out.append(d)
+    return out
+
+
+def pool_of(ex, H, I, slots=None):
+    lay = synth.fp8_layout(H, I)
+    slots = list(range(len(ex))) if slots is None else slots
+    pool = torch.zeros((max(slots) + 1, lay.total_bytes), dtype=torch.uint8, device=DEV)
+    for e, sl in zip(ex, slots):
+        for n, t in e.items():
+            o = lay.offsets[n]
+            pool[sl, o : o + lay.sizes[n]] = t.reshape(-1).view(torch.uint8)
+    return fp8_expert_layout(lay), pool
+
+
+def routes(seed, T, E, k):
+    lg = torch.randn((T, E), device=DEV, generator=gen(seed))
+    idx, w = ops.route_topk(lg, k)
+    return lg, idx, w
+
+
+LAYERS = [(4, 2, 64, 32), (8, 4, 256, 384), (5, 3, 1440, 736), (16, 8, 512, 160), (3, 1, 2880, 2880)]
+
+
+@pytest.mark.parametrize("E,k,H,I", LAYERS)
+@pytest.mark.parametrize("T", [1, 3, 8, 33])
+def test_moe(E, k, H, I, T):
+    """The same layer through the decode call, the routed one and the prompts' one."""
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    x, (lg, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    want, err = ref.moe(x, idx, w, ex)
+    ref.check(ops.moe_decode(L, pool, idx, w, x), want, err, "decode")
+    y, i2, w2 = ops.moe_decode_routed(L, pool, slot, lg, x, k, return_routing=True)
+    assert torch.equal(i2, idx)
+    ref.check(y, want, err + want.abs() * 2.0**-20 * k, "routed")
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), want, err, "prefill")
+
+
+@pytest.mark.parametrize("xd,yd", [(F32, F32), (HF, HF), (BF, F32), (F32, BF)])
+@pytest.mark.parametrize("T", [2, 70])
+def test_moe_dtypes(xd, yd, T):
+    E, k, H, I = 6, 2, 288, 416
+    ex = experts(3, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    x, (_, idx, w) = acts(T, T, H, dtype=xd), routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, ex)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    ref.check(ops.moe_decode(L, pool, idx, w, x, out_dtype=yd), want, err)
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x, out_dtype=yd), want, err)
+
+
+@pytest.mark.parametrize("T", [1, 4, 90])
+def test_moe_missing_and_moved(T):
+    """Experts in other slots, some not resident; tokens all of whose experts are missing give zeros."""
+    E, k, H, I = 6, 2, 256, 128
+    ex = experts(3, E, H, I)
+    order = [7, 2, 9, 0, 5, 3]
+    L, pool = pool_of(ex, H, I, order)
+    slot = torch.tensor([7, -1, 9, 0, -1, 99], dtype=torch.int32, device=DEV)  # 99: past the pool
+    left = [ex[0], None, ex[2], ex[3], None, None]
+    x, (lg, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    idx[0] = torch.tensor([1, 4], device=DEV)
+    want, err = ref.moe(x, idx, w, left)
+    y = ops.moe_prefill(L, pool, slot, idx, w, x)
+    ref.check(y, want, err)
+    assert not y[0].any()
+    y = ops.moe_decode(L, pool, slot[idx.long()], w, x)
+    ref.check(y, want, err)
+    _, idx, w = routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, left)
+    ref.check(ops.moe_decode_routed(L, pool, slot, lg, x, k), want, err + want.abs() * 2.0**-20 * k + err * 2.0**-18)
+
+
+def test_moe_swiglu_limits():
+    E, k, H, I, T = 4, 2, 256, 256, 5
+    ex = experts(3, E, H, I)
+    for e in ex:  # gates and ups past the limits of 7
+        e["gate_proj_scale_inv"] *= 8
+        e["up_proj_scale_inv"] *= 8
+    L, pool = pool_of(ex, H, I)
+    from tinyserve_amd import _lib
+
+    L.act = _lib.ACT_SWIGLU_OAI
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, ex, act="swiglu")
+    ref.check(ops.moe_decode(L, pool, idx, w, x), want, err)
+
+
+@pytest.mark.parametrize("T", [1, 50])
+def test_moe_same_expert_twice(T):
+    """A token that names one expert twice counts it twice."""
+    E, k, H, I = 3, 2, 128, 256
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    idx[:] = 2
+    want, err = ref.moe(x, idx, w, ex)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    ref.check(ops.moe_decode(L, pool, idx, w, x), want, err)
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), want, err)
+
+
+@pytest.mark.parametrize("T", [1, 6, 80])
+def test_moe_nan_token(T):
+    """A token with a NaN comes out NaN, the others as without it."""
+    E, k, H, I = 4, 2, 256, 160
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    for f in (lambda v: ops.moe_decode(L, pool, idx, w, v), lambda v: ops.moe_prefill(L, pool, slot, idx, w, v)):
+        y = f(x)
+        bad = x.clone()
+        bad[T // 2, 7] = float("nan")
+        z = f(bad)
+        keep = torch.arange(T, device=DEV) != T // 2
+        assert torch.isnan(z[T // 2]).all() and torch.equal(z[keep], y[keep])
+
+
+def test_moe_captured():
+    """A decode step captured once and replayed with other inputs, eager work in between."""
+    E, k, H, I, T = 8, 2, 512, 256, 2
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    x, lg = acts(0, T, H), torch.randn((T, E), device=DEV, generator=gen(0))
+    ws, y = ops.moe_decode_workspace(L, T, k, DEV), torch.empty((T, H), dtype=BF, device=DEV)
+    ws.fill_(255)
+    step = lambda: ops.moe_decode_routed(L, pool, slot, lg, x, k, out=y, workspace=ws)  # noqa: E731
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for i in range(4):
+        x.copy_(acts(20 + i, T, H))
+        lg.copy_(torch.randn((T, E), device=DEV, generator=gen(30 + i)))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.moe_decode_routed(L, pool, slot, lg, x, k))
+
+
+def test_chain_other_stream():
+    """Quantise once, three projections, router, experts: on a stream of its own, equal to one by one."""
+    T, H, I, E, k = 20, 512, 256, 8, 2
+    x, ex = acts(1, T, H), experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    ws = [weights(i, n, H) for i, n in enumerate((512, 128, 128))]
+    wo = weights(7, H, 512)
+    wr = torch.randn((E, H), device=DEV, generator=gen(3)).to(BF)
+
+    def chain():
+        c, s = ops.fp8_quantize(x)
+        q, k_, v = (ops.fp8_matmul(c, s, *w) for w in ws)
+        h = x + ops.fp8_linear(q, *wo)
+        idx, wt = ops.route_topk(ops.router_logits(h, wr), k)
+        return q, k_, v, ops.moe_prefill(L, pool, slot, idx, wt, h)
+
+    want = chain()
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        got = chain()
+    st.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

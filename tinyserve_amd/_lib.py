@@ -5,6 +5,7 @@ Loading fails loudly: there is no fallback implementation behind these calls.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -29,7 +30,7 @@ _TORCH_TO_TSA = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 # routing modes / activations / expert formats
 ROUTE_TOPK_SOFTMAX, ROUTE_SOFTMAX_TOPK, ROUTE_SOFTMAX_TOPK_RENORM = 0, 1, 2
 ACT_SILU, ACT_SWIGLU_OAI = 0, 1
-EXPERT_MXFP4, EXPERT_GGUF = 1, 2
+EXPERT_MXFP4, EXPERT_GGUF, EXPERT_FP8 = 1, 2, 3
 PREFILL_FP6, PREFILL_BF16 = 0, 1
 
 
@@ -74,6 +75,10 @@ SIGNATURES = {
     "tsa_mxfp4_tile_sizes": (_I32, [_I64, _I64, _P, _P]),
     "tsa_mxfp4_tile": (_I32, [_P, _P, _I64, _I64, _P, _P, _P]),
     "tsa_mxfp4_matvec": (_I32, [_P, _P, _P, _I32, _P, _I32, _I64, _P, _I32, _I64, _I64, _P]),
+    "tsa_fp8_quantize": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P]),
+    "tsa_fp8_matmul": (_I32, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I32, _P]),
+    "tsa_fp8_linear_workspace_size": (_I32, [_I64, _I64, ctypes.POINTER(_I64)]),
+    "tsa_fp8_linear": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _P]),
     "tsa_route_topk": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P]),
     "tsa_router_logits": (_I32, [_P, _I32, _I64, _I64, _P, _I32, _P, _I32, _I64, _P, _I32, _P]),
     "tsa_moe_decode_workspace_size": (_I32, [_LP, _I64, _I32, ctypes.POINTER(_I64)]),
@@ -140,6 +145,13 @@ def tensor_stream(t: torch.Tensor) -> int:
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def on_device(t: torch.Tensor):
+    """A context with the tensor's device current (kernels are launched on the current device);
+    nothing to do where it is already."""
+    d = t.get_device()
+    return contextlib.nullcontext() if d == torch.cuda.current_device() else torch.cuda.device(d)
 
 
 def require_device(*tensors: torch.Tensor, what: str = "tensor") -> None:

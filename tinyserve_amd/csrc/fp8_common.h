@@ -1,0 +1,142 @@
+// The FP8 block format on the device: e4m3 codes (OCP, v_cvt_pk_fp8_f32) and a float32 scale for
+// each block of 128 x 128 weights, or for each 128 values of a token.
+//
+// A token's group of 128 values x_k (the last one of a row may be shorter) is quantised as
+//     s = max(max|x_k| / 448, 2^-126),  c_k = e4m3(x_k / s),
+// both quotients rounded to float32 first. Ties in the second rounding are common (16-bit values
+// over 16-bit maxima), so the quotient has to be the correctly rounded one.
+#pragma once
+
+#include "fused_common.h"
+#include "mfma_tile.h"
+
+namespace tsa {
+namespace {
+
+constexpr int F8B = 128;  // values that share a scale
+
+typedef int f8_v8i __attribute__((ext_vector_type(8)));
+
+__host__ __device__ constexpr int64_t f8_blocks(int64_t n) { return (n + F8B - 1) / F8B; }
+
+// 8 codes (two words) as bf16, exactly.
+__device__ __forceinline__ bf16x8 f8_widen(uint32_t lo, uint32_t hi) {
+    return __builtin_bit_cast(bf16x8, u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))});
+}
+
+// The sums of one K block (128 values) of a 16 x 16 tile. Lane 16 q + i holds row i of A and column i
+// of B, the block's bytes 16 q .. and 64 + 16 q .. of either (A and B permute K alike); the result's
+// lane 16 q + i holds rows 4 q .. 4 q + 3 of column i. The zero scale operands select the
+// instruction's unscaled form.
+//
+// Precision. The FP8 matrix instructions add the (exact) products of 8 neighbouring values with 13
+// bits below the largest one's exponent, and those sums in float32: measured over normal data the
+// block's sum is off by 1.4e-5 of itself (rms), 300 times less than a bf16 result's rounding, 20 times
+// less than fp16's. WIDE, for float32 results, widens the codes to bf16 (exact), whose products the
+// bf16 instructions add to float32 accuracy (1e-8), at a quarter of the rate.
+template <bool WIDE = false>
+__device__ __forceinline__ v4f f8_mfma(const u32x4 (&a)[2], const u32x4 (&b)[2]) {
+    v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_widen(a[h][e], a[h][e + 1]), f8_widen(b[h][e], b[h][e + 1]), c, 0, 0, 0);
+        return c;
+    } else {
+        struct two { u32x4 v[2]; };
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(f8_v8i, two{{a[0], a[1]}}),
+                                                                __builtin_bit_cast(f8_v8i, two{{b[0], b[1]}}), c, 0, 0, 0, 0, 0, 0);
+    }
+}
+
+// 8 values of dtype XT from chunk c (8 values each) of a row; 16-byte aligned rows.
+template <int XT>
+__device__ __forceinline__ void f8_load8(const void* row, int c, float (&v)[8]) {
+    if constexpr (XT == TSA_F32) {
+        const float4 a = static_cast<const float4*>(row)[2 * c], b = static_cast<const float4*>(row)[2 * c + 1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const u32x4 w = static_cast<const u32x4*>(row)[c];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            v[2 * d] = XT == TSA_BF16 ? bf16_bits_to_f32(w[d] & 0xFFFFu) : f16_bits_to_f32(w[d]);
+            v[2 * d + 1] = XT == TSA_BF16 ? __uint_as_float(w[d] & 0xFFFF0000u) : f16_bits_to_f32(w[d] >> 16);
+        }
+    }
+}
+
+// The largest |v| of a group whose 16 chunks of 8 values are 16 lanes of one DPP row, as bits: for
+// non-negative floats the integer order is the order of the values, and a NaN is above them all.
+__device__ __forceinline__ uint32_t f8_group_max(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    m = max(m, (uint32_t)dpp_i<0x128, 0xF, 0xF>((int)m, 0));  // row_ror 8, 4, 2, 1
+    m = max(m, (uint32_t)dpp_i<0x124, 0xF, 0xF>((int)m, 0));
+    m = max(m, (uint32_t)dpp_i<0x122, 0xF, 0xF>((int)m, 0));
+    m = max(m, (uint32_t)dpp_i<0x121, 0xF, 0xF>((int)m, 0));
+    return m;
+}
+
+__device__ __forceinline__ float f8_scale(uint32_t max_bits) {
+    const float s = __uint_as_float(max_bits) / 448.0f;
+    return s < 0x1p-126f ? 0x1p-126f : s;  // a NaN stays one
+}
+
+// The codes of 8 values of a group with scale s. The quotient by Markstein's correction: with r the
+// rounded reciprocal of s, q = x r and the exact remainder e = x - q s, q + e r rounds to x / s. (For
+// every s and every bf16 or fp16 x it is the correctly rounded quotient, checked for all their
+// significands; 3 instructions instead of a division's 10.) EXACT (fp32 inputs) and groups whose
+// remainder could underflow or that hold an infinity or NaN divide.
+template <bool EXACT>
+__device__ __forceinline__ uint2 f8_codes8(const float (&v)[8], float s) {
+    float q[8];
+    if (EXACT || !(s > 0x1p-100f && s < INFINITY)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = v[e] / s;
+    } else {
+        const float r = 1.0f / s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = v[e] * r;
+            q[e] = fmaf(fmaf(-a, s, v[e]), r, a);
+        }
+    }
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+    return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// A row of K values (K % 16 == 0) quantised into LDS by `nthreads` threads, 16 lanes a group: codes
+// padded with zeros to whole groups, one scale per group.
+template <int XT>
+__device__ __forceinline__ void f8_stage_row(const void* row, int K, uint8_t* codes, float* scales, int tid, int nthreads) {
+    const int tasks = (int)f8_blocks(K) * 16;
+    for (int c = tid; c < tasks; c += nthreads) {
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (8 * c < K) f8_load8<XT>(row, c, v);
+        const float s = f8_scale(f8_group_max(v));
+        *reinterpret_cast<uint2*>(codes + 8 * c) = f8_codes8<XT == TSA_F32>(v, s);
+        if ((c & 15) == 0) scales[c >> 4] = s;
+    }
+}
+
+// Rows of 16 bytes from a matrix: a buffer over `records` bytes from p, whose offsets past the end
+// (f8_off's mark among them) read zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_buf(const void* p, int64_t records) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)records, 0x00020000);
+}
+__device__ __forceinline__ u32x4 f8_ld(const __amdgpu_buffer_rsrc_t& r, uint32_t o) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)o, 0, 0));
+}
+// Byte offset of column o (a multiple of 16) of a row that starts at `row`, or one past the buffer.
+__device__ __forceinline__ uint32_t f8_off(uint32_t row, uint32_t o, uint32_t K) { return o < K ? row + o : 0x80000000u; }
+
+}  // namespace
+}  // namespace tsa

@@ -218,6 +218,13 @@ int mxt_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots,
                int32_t* idx_out, float* w_out, int64_t T, int k, const void* x, void* y, int y_dtype, uint8_t* sync,
                uint8_t* ws, int64_t ws_bytes, hipStream_t st);
 
+const char* f8_unsupported(const tsa_expert_layout& L);
+bool f8_routes(int64_t T, int64_t E, int k);
+int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const int32_t* slots, const float* wts,
+              const void* logits, int logits_dtype, int mode, const int32_t* expert_slot, int64_t E, int32_t* idx_out,
+              float* w_out, int64_t T, int k, const void* x, int x_dtype, void* y, int y_dtype, uint8_t* ws,
+              int64_t ws_bytes, hipStream_t st);
+
 // Workspace: the sync area of the one-launch MXFP4 decode (MXT_SYNC_BYTES), then the
 // intermediate h of every path (float [T, k, I] at most), then int32 slots / ids and float
 // weights [T, k] for routed calls. Only the sync area carries state from one call to the
@@ -240,8 +247,8 @@ uint32_t mxt_wait_limit() { return g_mxt_wait_limit.load(std::memory_order_relax
 
 int validate_layout(const tsa_expert_layout* L) {
     TSA_REQUIRE(L != nullptr, TSA_ERR_INVALID_ARG, "layout is null");
-    TSA_REQUIRE(L->format == TSA_EXPERT_MXFP4 || L->format == TSA_EXPERT_GGUF, TSA_ERR_INVALID_ARG,
-                "layout.format %d is not MXFP4(1) or GGUF(2)", L->format);
+    TSA_REQUIRE(L->format == TSA_EXPERT_MXFP4 || L->format == TSA_EXPERT_GGUF || L->format == TSA_EXPERT_FP8,
+                TSA_ERR_INVALID_ARG, "layout.format %d is not MXFP4(1), GGUF(2) or FP8(3)", L->format);
     TSA_REQUIRE(L->act == TSA_ACT_SILU || L->act == TSA_ACT_SWIGLU_OAI, TSA_ERR_INVALID_ARG, "layout.act %d unknown",
                 L->act);
     TSA_REQUIRE(L->hidden > 0 && L->inter > 0 && L->slot_bytes > 0, TSA_ERR_SHAPE, "layout sizes must be positive");
@@ -258,7 +265,17 @@ int validate_layout(const tsa_expert_layout* L) {
         const char* why = mxt_unsupported(*L);
         TSA_REQUIRE(!*why, TSA_ERR_SHAPE, "%s", why);
     }
-    if (L->format == TSA_EXPERT_MXFP4) {
+    if (L->format == TSA_EXPERT_FP8) {
+        const int64_t H = L->hidden, I = L->inter, sb = 4 * ((H + 127) / 128) * ((I + 127) / 128);
+        const int64_t need[5][2] = {{L->gate_off, I * H}, {L->up_off, I * H}, {L->gate_scales_off, 2 * sb}, {L->down_off, H * I},
+                                    {L->down_scales_off, sb}};
+        for (auto& r : need)
+            TSA_REQUIRE(r[0] >= 0 && r[0] + r[1] <= L->slot_bytes, TSA_ERR_WEIGHT_TOO_SMALL,
+                        "tensor at offset %lld (%lld bytes) exceeds slot_bytes %lld", (long long)r[0],
+                        (long long)r[1], (long long)L->slot_bytes);
+        const char* why = f8_unsupported(*L);
+        TSA_REQUIRE(!*why, TSA_ERR_INVALID_ARG, "%s", why);
+    } else if (L->format == TSA_EXPERT_MXFP4) {
         const int64_t H = L->hidden, I = L->inter;
         const bool tl = L->mx_tiled != 0;
         const int64_t need[4][2] = {{L->gate_off, 2 * I * H / 2},
@@ -391,6 +408,9 @@ extern "C" int tsa_moe_decode(const tsa_expert_layout* layout, const void* pool,
         }
         return TSA_OK;
     }
+    if (L.format == TSA_EXPERT_FP8)
+        return f8_decode(L, pl, n_slots, slots, weights, nullptr, 0, 0, nullptr, 0, nullptr, nullptr, T, k, x, x_dtype, y,
+                         y_dtype, ws, wsb, st);
     rc = mx_fused_decode(L, pl, n_slots, slots, weights, nullptr, 0, 0, nullptr, 0, nullptr, nullptr, T, k, x, x_dtype,
                          y, y_dtype, ws, wsb, st);
     if (rc <= 0) return rc;
@@ -488,7 +508,10 @@ static int decode_routed(const tsa_expert_layout* layout, const void* pool, int6
         }
         return TSA_OK;
     }
-    if (!L.mx_tiled) {
+    if (L.format == TSA_EXPERT_FP8 && f8_routes(T, E, k))
+        return f8_decode(L, pl, n_slots, nullptr, nullptr, logits, logits_dtype, mode, expert_slot, E, idx_out, w_out, T, k, x,
+                         x_dtype, y, y_dtype, ws, wsb, st);
+    if (!L.mx_tiled && L.format != TSA_EXPERT_FP8) {
         rc = mx_fused_decode(L, pl, n_slots, nullptr, nullptr, logits, logits_dtype, mode, expert_slot, E, idx_out,
                              w_out, T, k, x, x_dtype, y, y_dtype, ws, wsb, st);
         if (rc <= 0) return rc;
@@ -510,6 +533,9 @@ static int decode_routed(const tsa_expert_layout* layout, const void* pool, int6
     if (L.mx_tiled)
         return tiled_decode(L, pl, n_slots, slots, w, nullptr, 0, 0, nullptr, 0, nullptr, nullptr, T, k, x, x_dtype, y,
                             y_dtype, sync, ws, wsb, st);
+    if (L.format == TSA_EXPERT_FP8)
+        return f8_decode(L, pl, n_slots, slots, w, nullptr, 0, 0, nullptr, 0, nullptr, nullptr, T, k, x, x_dtype, y, y_dtype, ws,
+                         h_region(L, T, k) + 2 * tk, st);
     return two_launch_decode(L, pl, n_slots, slots, w, T, k, x, x_dtype, y, y_dtype, ws, st);
 }
 

@@ -133,11 +133,51 @@ def gguf_expert_layout(layout: TensorLayout, ggml_types: dict, proj_shapes: dict
     return L
 
 
+_FP8_MATS = ("gate_proj", "up_proj", "down_proj")
+
+
+def is_fp8_layout(layout: TensorLayout) -> bool:
+    """Whether a slot holds an FP8 expert: e4m3 gate_proj / up_proj / down_proj and their block scales."""
+    return all(m in layout.specs and layout.specs[m][1] == torch.float8_e4m3fn and m + "_scale_inv" in layout.specs
+               for m in _FP8_MATS)
+
+
+def fp8_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout:
+    """tsa_expert_layout of an FP8 slot: ``gate_proj`` / ``up_proj`` [I, H] and ``down_proj`` [H, I] as
+    float8_e4m3fn, ``*_scale_inv`` float32 per 128 x 128 block, up's scales right behind gate's (the
+    order of synth.fp8_layout). act_fn None or SiLU."""
+    if not is_fp8_layout(layout):
+        raise ValueError(f"not an FP8 expert slot: {sorted(layout.specs)}")
+    if act_fn is not None and not _is_silu(act_fn):
+        raise NotImplementedError(f"unsupported activation {act_fn!r}")
+    (I, H), off = layout.specs["gate_proj"][0], layout.offsets
+    blocks = lambda n: -(-n // ops.FP8_BLOCK)  # noqa: E731
+    shapes = {"gate_proj": (I, H), "up_proj": (I, H), "down_proj": (H, I)}
+    for m, (r, c) in shapes.items():
+        got, scales = tuple(layout.specs[m][0]), layout.specs[m + "_scale_inv"]
+        if got != (r, c) or tuple(scales[0]) != (blocks(r), blocks(c)) or scales[1] != torch.float32:
+            raise ValueError(f"inconsistent FP8 expert shapes: {m} {got} with scales {scales}, hidden {H}, inter {I}")
+    if off["up_proj_scale_inv"] != off["gate_proj_scale_inv"] + layout.sizes["gate_proj_scale_inv"]:
+        raise ValueError("up_proj_scale_inv must follow gate_proj_scale_inv in the slot")
+    L = _lib.ExpertLayout()
+    L.format, L.act = _lib.EXPERT_FP8, _lib.ACT_SILU
+    L.hidden, L.inter = H, I
+    L.slot_bytes = slot_bytes or layout.total_bytes
+    L.gate_off, L.up_off, L.down_off = off["gate_proj"], off["up_proj"], off["down_proj"]
+    L.gate_scales_off, L.down_scales_off = off["gate_proj_scale_inv"], off["down_proj_scale_inv"]
+    L.gate_bias_off = L.down_bias_off = -1
+    L.bias_dtype = _lib.BF16
+    L.swiglu_limit, L.swiglu_alpha = _SWIGLU_LIMIT, _QUICK_GELU_COEFF
+    return L
+
+
 def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | None = None,
                         proj_shapes: dict | None = None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
     """The kernel-side layout of a packed expert, or None for unquantised layouts."""
     if "gate_up_proj_scales" in layout.specs:
         return mxfp4_expert_layout(layout, act_fn, slot_bytes)
+    if is_fp8_layout(layout):
+        return fp8_expert_layout(layout, act_fn, slot_bytes)
     if ggml_types is not None and {"gate", "up", "down"} <= set(layout.specs):
         return gguf_expert_layout(layout, ggml_types, proj_shapes, slot_bytes)
     return None

@@ -22,15 +22,16 @@ def _element_size(dtype: torch.dtype) -> int:
 
 class TensorLayout:
     """Byte map of one packed expert slot: each named tensor's (offset, size) in the slot,
-    tensors placed back to back in the order of ``tensor_specs``."""
+    tensors placed back to back in the order of ``tensor_specs``; ``align``: the slot size is
+    rounded up to a multiple of it."""
 
-    def __init__(self, tensor_specs: dict[str, tuple[tuple[int, ...], torch.dtype]]):
+    def __init__(self, tensor_specs: dict[str, tuple[tuple[int, ...], torch.dtype]], align: int = 1):
         self.specs = tensor_specs
         names = list(tensor_specs)
         sizes = [math.prod(int(d) for d in shape) * _element_size(dtype) for shape, dtype in tensor_specs.values()]
         self.sizes: dict[str, int] = dict(zip(names, sizes))
         self.offsets: dict[str, int] = dict(zip(names, itertools.accumulate([0] + sizes[:-1])))
-        self.total_bytes = sum(sizes)
+        self.total_bytes = -(-sum(sizes) // align) * align
 
     @staticmethod
     def from_tensors(tensors: dict[str, torch.Tensor]) -> "TensorLayout":

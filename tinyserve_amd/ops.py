@@ -128,6 +128,96 @@ def mxfp4_matvec(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
     return y
 
 
+# ----------------------------------------------------------------------------- FP8, blocks of 128
+FP8_BLOCK = 128
+_FP8_DTYPES = (torch.float8_e4m3fn, torch.uint8)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous memory from a multiple of 16 bytes on (a copy if it is not there already)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"all tensors must be on one device (got {first.device} and {t.device})")
+
+
+def _fp8_weight(w: torch.Tensor, scales: torch.Tensor, K: int) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """(codes, float32 scales, N) of a weight matrix [N, K], checked."""
+    if w.dtype not in _FP8_DTYPES or w.dim() != 2:
+        raise RuntimeError(f"FP8 weights must be float8_e4m3fn (or its bytes) [N, K], got {w.dtype} {tuple(w.shape)}")
+    N = w.shape[0]
+    if w.shape[1] != K:
+        raise RuntimeError(f"in_features differ: activations {K}, weight {w.shape[1]}")
+    want = (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK))
+    if tuple(scales.shape) != want:
+        raise RuntimeError(f"weight scales must be {list(want)} for an [{N}, {K}] weight, got {list(scales.shape)}")
+    return _aligned(w), scales.to(torch.float32).contiguous(), N
+
+
+def _fp8_bias(bias: torch.Tensor | None, N: int) -> torch.Tensor | None:
+    if bias is not None and bias.numel() != N:
+        raise RuntimeError(f"bias must have {N} elements, got {bias.numel()}")
+    return None if bias is None else bias.contiguous()
+
+
+def fp8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes float8_e4m3fn [T, K], scales float32 [T, ceil(K / 128)]) of x [..., K] (bf16, fp16 or fp32):
+    per token and 128 columns, scale = max(max|x| / 448, 2^-126) and code = e4m3(x / scale)."""
+    _lib.require_device(x, what="activation")
+    dt = _lib.tsa_dtype(x.dtype)
+    x2 = _rows(x, x.shape[-1])
+    T, K = x2.shape
+    codes = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((T, -(-K // FP8_BLOCK)), dtype=torch.float32, device=x.device)
+    with _lib.on_device(x2):
+        _lib.check(_lib.load().tsa_fp8_quantize(x2.data_ptr(), dt, T, K, codes.data_ptr(), scales.data_ptr(), _stream(x2)))
+    return codes, scales
+
+
+def fp8_matmul(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+               bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y [T, N] = deq(codes) @ deq(w)^T (+ bias): codes [T, K] and scales [T, ceil(K / 128)] as
+    fp8_quantize returns them, w [N, K] with scales [ceil(N / 128), ceil(K / 128)]; float32 sums. K
+    must be a multiple of 16. Projections that share their input share one fp8_quantize."""
+    _lib.require_device(codes, scales, w, w_scales, *([bias] if bias is not None else []), what="tensor")
+    _same_device(codes, scales, w, w_scales, bias)
+    if codes.dtype not in _FP8_DTYPES or codes.dim() != 2:
+        raise RuntimeError(f"FP8 activations must be float8_e4m3fn (or its bytes) [T, K], got {codes.dtype} {tuple(codes.shape)}")
+    T, K = codes.shape
+    if tuple(scales.shape) != (T, -(-K // FP8_BLOCK)) or scales.dtype != torch.float32:
+        raise RuntimeError(f"activation scales must be float32 [{T}, {-(-K // FP8_BLOCK)}], got {scales.dtype} {list(scales.shape)}")
+    c, sc, (w, ws, N), b = _aligned(codes), scales.contiguous(), _fp8_weight(w, w_scales, K), _fp8_bias(bias, w.shape[0])
+    y = torch.empty((T, N), dtype=out_dtype, device=codes.device)
+    with _lib.on_device(c):
+        _lib.check(_lib.load().tsa_fp8_matmul(c.data_ptr(), sc.data_ptr(), T, K, w.data_ptr(), ws.data_ptr(), N, _lib.ptr(b),
+                                              _lib.tsa_dtype(b.dtype) if b is not None else 0, y.data_ptr(),
+                                              _lib.tsa_dtype(out_dtype), _stream(c)))
+    return y
+
+
+def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y [T, N] = deq(fp8_quantize(x)) @ deq(w)^T (+ bias) for x [..., K] in bf16, fp16 or fp32; y in
+    x's dtype unless ``out_dtype`` says otherwise. K must be a multiple of 16."""
+    _lib.require_device(x, w, w_scales, *([bias] if bias is not None else []), what="tensor")
+    _same_device(x, w, w_scales, bias)
+    dt, K = _lib.tsa_dtype(x.dtype), x.shape[-1]
+    w, ws, N = _fp8_weight(w, w_scales, K)
+    x2, b = _aligned(_rows(x, K)), _fp8_bias(bias, N)
+    T = x2.shape[0]
+    y = torch.empty((T, N), dtype=out_dtype or x.dtype, device=x.device)
+    scratch = torch.empty(T * K + 4 * T * ws.shape[1] + 256, dtype=torch.uint8, device=x.device)
+    with _lib.on_device(x2):
+        _lib.check(_lib.load().tsa_fp8_linear(x2.data_ptr(), dt, T, K, w.data_ptr(), ws.data_ptr(), N, _lib.ptr(b),
+                                              _lib.tsa_dtype(b.dtype) if b is not None else 0, y.data_ptr(),
+                                              _lib.tsa_dtype(y.dtype), scratch.data_ptr(), scratch.numel(), _stream(x2)))
+    return y
+
+
 # ----------------------------------------------------------------------------- routing
 ROUTE_MODES = {
     "topk_then_softmax": _lib.ROUTE_TOPK_SOFTMAX,
@@ -177,6 +267,12 @@ def _n_slots(pool: torch.Tensor, layout: _lib.ExpertLayout) -> int:
     return n
 
 
+def _moe_rows(layout: _lib.ExpertLayout, x: torch.Tensor) -> torch.Tensor:
+    """x as contiguous rows of ``hidden`` values (from a multiple of 16 bytes on for FP8 experts)."""
+    x2 = x.reshape(-1, layout.hidden).contiguous()
+    return _aligned(x2) if layout.format == _lib.EXPERT_FP8 else x2
+
+
 def moe_decode_workspace_size(layout: _lib.ExpertLayout, T: int, k: int) -> int:
     """Bytes of the decode workspace for T tokens, k experts each; validates the layout
     (host only, raises RuntimeError with the library's message)."""
@@ -211,7 +307,7 @@ def moe_decode(layout: _lib.ExpertLayout, pool: torch.Tensor, slots: torch.Tenso
     """y[t] = sum_j weights[t, j] * FFN_{slots[t, j]}(x[t]) over the resident slot pool."""
     _lib.require_device(pool, slots, weights, x, what="tensor")
     H = layout.hidden
-    x2 = x.reshape(-1, H).contiguous()
+    x2 = _moe_rows(layout, x)
     T = x2.shape[0]
     slots = slots.reshape(T, -1).to(torch.int32).contiguous()
     weights = weights.reshape(T, -1).to(torch.float32).contiguous()
@@ -221,10 +317,11 @@ def moe_decode(layout: _lib.ExpertLayout, pool: torch.Tensor, slots: torch.Tenso
         out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
     if workspace is None:
         workspace = moe_decode_workspace(layout, T, k, x.device)
-    _lib.check(_lib.load().tsa_moe_decode(ctypes.byref(layout), pool.data_ptr(), n_slots, slots.data_ptr(),
-                                          weights.data_ptr(), T, k, x2.data_ptr(), _lib.tsa_dtype(x2.dtype),
-                                          out.data_ptr(), _lib.tsa_dtype(out.dtype), workspace.data_ptr(),
-                                          workspace.numel(), _stream(x)))
+    with _lib.on_device(x2):
+        _lib.check(_lib.load().tsa_moe_decode(ctypes.byref(layout), pool.data_ptr(), n_slots, slots.data_ptr(),
+                                              weights.data_ptr(), T, k, x2.data_ptr(), _lib.tsa_dtype(x2.dtype),
+                                              out.data_ptr(), _lib.tsa_dtype(out.dtype), workspace.data_ptr(),
+                                              workspace.numel(), _stream(x)))
     return out
 
 
@@ -235,7 +332,7 @@ def moe_decode_routed(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot
     """Router top-k + fused expert FFN in one call (a single launch for MXFP4, T <= 4)."""
     _lib.require_device(pool, expert_slot, logits, x, what="tensor")
     H = layout.hidden
-    x2 = x.reshape(-1, H).contiguous()
+    x2 = _moe_rows(layout, x)
     T = x2.shape[0]
     lg = logits.reshape(T, -1).contiguous()
     E = lg.shape[1]
@@ -246,11 +343,12 @@ def moe_decode_routed(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot
         workspace = moe_decode_workspace(layout, T, top_k, x.device)
     idx = torch.empty((T, top_k), dtype=torch.int32, device=x.device) if return_routing else None
     w = torch.empty((T, top_k), dtype=torch.float32, device=x.device) if return_routing else None
-    _lib.check(_lib.load().tsa_moe_decode_routed(
-        ctypes.byref(layout), pool.data_ptr(), _n_slots(pool, layout), expert_slot.data_ptr(), E, lg.data_ptr(),
-        _lib.tsa_dtype(lg.dtype), ROUTE_MODES[mode], T, int(top_k), x2.data_ptr(), _lib.tsa_dtype(x2.dtype),
-        out.data_ptr(), _lib.tsa_dtype(out.dtype), _lib.ptr(idx), _lib.ptr(w), workspace.data_ptr(), workspace.numel(),
-        _stream(x)))
+    with _lib.on_device(x2):
+        _lib.check(_lib.load().tsa_moe_decode_routed(
+            ctypes.byref(layout), pool.data_ptr(), _n_slots(pool, layout), expert_slot.data_ptr(), E, lg.data_ptr(),
+            _lib.tsa_dtype(lg.dtype), ROUTE_MODES[mode], T, int(top_k), x2.data_ptr(), _lib.tsa_dtype(x2.dtype),
+            out.data_ptr(), _lib.tsa_dtype(out.dtype), _lib.ptr(idx), _lib.ptr(w), workspace.data_ptr(), workspace.numel(),
+            _stream(x)))
     return (out, idx, w) if return_routing else out
 
 
@@ -289,7 +387,7 @@ def moe_prefill(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot: torc
     """Batched (prefill) MoE: out[t] = sum_j weights[t, j] * FFN_{expert_slot[idx[t, j]]}(x[t])."""
     _lib.require_device(pool, expert_slot, idx, weights, x, what="tensor")
     H = layout.hidden
-    x2 = x.reshape(-1, H).contiguous()
+    x2 = _moe_rows(layout, x)
     T = x2.shape[0]
     idx = idx.reshape(T, -1).to(torch.int32).contiguous()
     weights = weights.reshape(T, -1).to(torch.float32).contiguous()
@@ -300,8 +398,9 @@ def moe_prefill(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot: torc
         out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
     if workspace is None:
         workspace = moe_prefill_workspace(layout, T, k, E, x.device)
-    _lib.check(_lib.load().tsa_moe_prefill(ctypes.byref(layout), pool.data_ptr(), n_slots, expert_slot.data_ptr(), E,
-                                           idx.data_ptr(), weights.data_ptr(), T, k, x2.data_ptr(),
-                                           _lib.tsa_dtype(x2.dtype), out.data_ptr(), _lib.tsa_dtype(out.dtype),
-                                           workspace.data_ptr(), workspace.numel(), _stream(x)))
+    with _lib.on_device(x2):
+        _lib.check(_lib.load().tsa_moe_prefill(ctypes.byref(layout), pool.data_ptr(), n_slots, expert_slot.data_ptr(), E,
+                                               idx.data_ptr(), weights.data_ptr(), T, k, x2.data_ptr(),
+                                               _lib.tsa_dtype(x2.dtype), out.data_ptr(), _lib.tsa_dtype(out.dtype),
+                                               workspace.data_ptr(), workspace.numel(), _stream(x)))
     return out

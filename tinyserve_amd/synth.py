@@ -224,3 +224,36 @@ def workload(n: int, n_experts: int | None = None, tokens: int | None = None) ->
         return {"hidden": H, "inter": I, "E": E, "top_k": 8, "experts": experts, "layout": lay, "pool": pool,
                 "logits": zipf_logits(rng, T, E), "x_bits": bf16_normal(rng, (T, H)), "route": "softmax_then_topk"}
     raise ValueError(f"unknown workload {n}")
+
+
+# ----------------------------------------------------------------------------- FP8 experts
+def fp8_layout(hidden: int, inter: int) -> TensorLayout:
+    """An FP8 expert's slot: the e4m3 matrices, then their float32 scales per 128 x 128 block,
+    filled up to a multiple of 16 bytes."""
+    b = lambda n: -(-n // 128)  # noqa: E731
+    return TensorLayout({
+        "gate_proj": ((inter, hidden), torch.float8_e4m3fn),
+        "up_proj": ((inter, hidden), torch.float8_e4m3fn),
+        "down_proj": ((hidden, inter), torch.float8_e4m3fn),
+        "gate_proj_scale_inv": ((b(inter), b(hidden)), torch.float32),
+        "up_proj_scale_inv": ((b(inter), b(hidden)), torch.float32),
+        "down_proj_scale_inv": ((b(hidden), b(inter)), torch.float32),
+    }, align=16)
+
+
+def make_fp8(rng: np.random.Generator, rows: int, cols: int, sigma: float = 0.03) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of an N(0, sigma) matrix [rows, cols], the largest value of each block at 448."""
+    n, k = -(-rows // 128), -(-cols // 128)
+    w = np.zeros((n * 128, k * 128), dtype=np.float32)
+    w[:rows, :cols] = rng.normal(0.0, sigma, (rows, cols))
+    s = np.abs(w.reshape(n, 128, k, 128)).max((1, 3)) / np.float32(448)
+    w /= s.repeat(128, 0).repeat(128, 1)
+    return torch.from_numpy(w[:rows, :cols].copy()).to(torch.float8_e4m3fn), torch.from_numpy(s)
+
+
+def make_fp8_expert(rng: np.random.Generator, hidden: int, inter: int, sigma: float = 0.03) -> dict[str, torch.Tensor]:
+    """The tensors of fp8_layout."""
+    e = {}
+    for name, (r, c) in (("gate_proj", (inter, hidden)), ("up_proj", (inter, hidden)), ("down_proj", (hidden, inter))):
+        e[name], e[name + "_scale_inv"] = make_fp8(rng, r, c, sigma)
+    return e
