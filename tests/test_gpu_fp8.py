@@ -249,6 +249,24 @@ def test_moe(E, k, H, I, T):
     ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), want, err, "prefill")
 
 
+@pytest.mark.parametrize("E,k,H,I", [(4, 2, 256, 384), (3, 1, 1440, 736), (9, 3, 544, 96)])
+@pytest.mark.parametrize("T", [101, 300, 1031])
+@pytest.mark.parametrize("route", ["even", "one", "skewed"])
+def test_moe_many(E, k, H, I, T, route):
+    """Every token tile, with loads that fill it, leave it nearly empty, or all fall on one expert."""
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    x, g = acts(T, T, H), gen(T)
+    p = torch.ones(E, device=DEV) if route != "skewed" else 4.0 ** -torch.arange(E, device=DEV)
+    idx = torch.multinomial(p.expand(T, E), k, generator=g).to(torch.int32)
+    if route == "one":
+        idx[:] = E - 1
+    w = torch.rand((T, k), device=DEV, generator=g)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    want, err = ref.moe(x, idx, w, ex)
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), want, err)
+
+
 @pytest.mark.parametrize("xd,yd", [(F32, F32), (HF, HF), (BF, F32), (F32, BF)])
 @pytest.mark.parametrize("T", [2, 70])
 def test_moe_dtypes(xd, yd, T):

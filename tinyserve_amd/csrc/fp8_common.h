@@ -113,6 +113,24 @@ __device__ __forceinline__ uint2 f8_codes8(const float (&v)[8], float s) {
     return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
+// The codes of 4 computed (fp32) values of a group with scale s, as one word: the same quotient.
+__device__ __forceinline__ uint32_t f8_codes4(const v4f& v, float s) {
+    float q[4];
+    if (!(s > 0x1p-100f && s < INFINITY)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = v[e] / s;
+    } else {
+        const float r = 1.0f / s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float a = v[e] * r;
+            q[e] = fmaf(fmaf(-a, s, v[e]), r, a);
+        }
+    }
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+}
+
 // A row of K values (K % 16 == 0) quantised into LDS by `nthreads` threads, 16 lanes a group: codes
 // padded with zeros to whole groups, one scale per group.
 template <int XT>

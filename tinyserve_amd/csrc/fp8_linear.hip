@@ -1,6 +1,6 @@
 // FP8 quantisation of activations and the block-scaled FP8 product
 //     y[t, n] = sum_b sx[t, b] sw[n / 128, b] sum_{k in block b} cx[t, k] cw[n, k]  (+ bias[n]).
-#include "fp8_common.h"
+#include "fp8_gemm.h"
 
 namespace tsa {
 namespace {
@@ -156,6 +156,117 @@ hipError_t launch_rows(const F8Rows& p, hipStream_t st) {
     return hipLaunchKernel(fn, dim3((unsigned)(p.tiles_n * ((p.T + 15) / 16))), dim3(256), args, lds, st);
 }
 
+// ---------------------------------------------------------------- many tokens
+struct F8Gemm {
+    const uint8_t* w;
+    const float* ws;
+    const uint8_t* x;
+    const float* xs;
+    const void* bias;
+    int bias_dtype;
+    void* y;
+    int y_dtype;
+    int T, N, K, G, tiles_t;
+    int y_vec;  // y rows of whole 4-value pieces
+};
+
+template <class C, bool WIDE>
+__global__ void __launch_bounds__(C::THREADS) fp8_gemm_kernel(F8Gemm p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    // Workgroups are dealt round the 8 XCDs by linear id: renumbered so that each XCD takes a run, and
+    // within it bands of 8 row tiles, token tile by token tile (about square pieces of the product at
+    // a time share one L2: 3% at 4096 x 5760 against whole rows of token tiles).
+    const int total = (int)gridDim.x, lin = (int)blockIdx.x, xcd = lin & 7, q8 = total >> 3, rem = total & 7;
+    const int wid = xcd * q8 + (xcd < rem ? xcd : rem) + (lin >> 3);  // a bijection of [0, total)
+    constexpr int BAND = 8;
+    const int rows = total / p.tiles_t, band = wid / (BAND * p.tiles_t), in = wid - band * BAND * p.tiles_t;
+    const int deep = rows - BAND * band < BAND ? rows - BAND * band : BAND;  // row tiles of the band
+    const int n0 = (BAND * band + in % deep) * C::RN, t0 = in / deep * C::TM;
+    const int tn = p.T - t0 < C::TM ? p.T - t0 : C::TM;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
+    const int wr = wave % C::WR, wt = wave / C::WR;
+    const int nw = n0 + wr * C::MR * 16;  // this wave's first row; all of them are in one 128-row block
+    static_assert(F8B % (C::MR * 16) == 0, "a wave's rows share their scales");
+    F8Operands<1> o;
+    o.w[0] = p.w + (int64_t)n0 * p.K;
+    o.w_rows = p.N - n0;
+    o.ws[0] = p.ws + (int64_t)(nw < p.N ? nw / F8B : 0) * p.G;  // rows past N are not stored
+    o.x = p.x + (int64_t)t0 * p.K;
+    o.xs = p.xs + (int64_t)t0 * p.G;
+    o.x_records = (uint32_t)tn * (uint32_t)p.K;
+    o.xs_records = (uint32_t)tn * (uint32_t)p.G * 4u;
+    o.K = p.K;
+    o.G = p.G;
+    v4f acc[C::MR][C::MT];
+    f8_tile<C, 1, WIDE>(o, smem, [&](int r) { return r < tn ? r : -1; }, acc);
+#pragma unroll
+    for (int m = 0; m < C::MR; ++m) {
+        const int n = nw + 16 * m + 4 * q;
+        float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n + r < p.N) b[r] = load_act(p.bias, p.bias_dtype, n + r);
+        }
+#pragma unroll
+        for (int t = 0; t < C::MT; ++t) {
+            const int tk = 16 * (C::MT * wt + t) + i;
+            if (tk >= tn || n >= p.N) continue;
+            const int64_t at = (int64_t)(t0 + tk) * p.N + n;
+            const v4f v = acc[m][t] + v4f{b[0], b[1], b[2], b[3]};
+            if (p.y_vec && p.y_dtype == TSA_BF16) {
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+            } else if (p.y_vec && p.y_dtype == TSA_F32) {
+                *reinterpret_cast<v4f*>(static_cast<float*>(p.y) + at) = v;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < p.N) store_out(p.y, p.y_dtype, at + r, v[r]);
+            }
+        }
+    }
+}
+
+template <class C, bool WIDE>
+hipError_t launch_gemm(const F8Gemm& p, hipStream_t st) {
+    const void* fn = reinterpret_cast<const void*>(&fp8_gemm_kernel<C, WIDE>);
+    const hipError_t e = ensure_dynamic_lds(fn, C::LDS);
+    if (e != hipSuccess) return e;
+    F8Gemm q = p;
+    q.tiles_t = (p.T + C::TM - 1) / C::TM;
+    void* args[] = {&q};
+    const int64_t grid = (int64_t)((p.N + C::RN - 1) / C::RN) * q.tiles_t;
+    return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(C::THREADS), args, C::LDS, st);
+}
+
+using TileA = F8Tile<2, 4, 8, 4, 2>;  // 256 rows x 256 tokens
+using TileB = F8Tile<4, 2, 4, 4, 3>;  // 256 x 128
+using TileC = F8Tile<2, 2, 4, 4, 2>;  // 128 x 128
+using TileD = F8Tile<4, 1, 2, 4, 3>;  // 128 x 64
+using TileE = F8Tile<4, 1, 1, 2, 4>;  // 64 x 32
+
+// The tile with the least rounds x round time, a round being `per` workgroups on every CU.
+template <bool WIDE>
+hipError_t pick_gemm(const F8Gemm& p, hipStream_t st) {
+    struct Tile { int rows, tok, per, cost; };
+    constexpr Tile tiles[5] = {{256, 256, 1, 45}, {256, 128, 1, 26}, {128, 128, 2, 32}, {128, 64, 2, 20}, {64, 32, 3, 13}};
+    const int64_t cus = num_cus() > 0 ? num_cus() : 256;
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < 5; ++i) {
+        const int64_t wgs = (int64_t)((p.N + tiles[i].rows - 1) / tiles[i].rows) * ((p.T + tiles[i].tok - 1) / tiles[i].tok);
+        const int64_t cost = (wgs + cus * tiles[i].per - 1) / (cus * tiles[i].per) * tiles[i].cost;
+        if (cost < least) least = cost, best = i;
+    }
+    switch (best) {
+        case 0: return launch_gemm<TileA, WIDE>(p, st);
+        case 1: return launch_gemm<TileB, WIDE>(p, st);
+        case 2: return launch_gemm<TileC, WIDE>(p, st);
+        case 3: return launch_gemm<TileD, WIDE>(p, st);
+        default: return launch_gemm<TileE, WIDE>(p, st);
+    }
+}
+
 constexpr int64_t F8_MAX_K = 1 << 20;  // 32-bit offsets inside a tile of rows
 
 int check_matmul(int64_t T, int64_t K, int64_t N, const void* bias, int bias_dtype, int y_dtype) {
@@ -228,6 +339,24 @@ extern "C" int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T,
     if (T == 0) return TSA_OK;
     TSA_REQUIRE(codes && scales && w && w_scales && y, TSA_ERR_INVALID_ARG, "null pointer");
     TSA_REQUIRE(aligned16(codes) && aligned16(w), TSA_ERR_INVALID_ARG, "the codes must be 16-byte aligned");
+    if (T > 16) {
+        F8Gemm p{};
+        p.w = static_cast<const uint8_t*>(w);
+        p.ws = w_scales;
+        p.x = static_cast<const uint8_t*>(codes);
+        p.xs = scales;
+        p.bias = bias;
+        p.bias_dtype = bias_dtype;
+        p.y = y;
+        p.y_dtype = y_dtype;
+        p.T = (int)T;
+        p.N = (int)N;
+        p.K = (int)K;
+        p.G = (int)f8_blocks(K);
+        p.y_vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
+        TSA_HIP_CHECK(y_dtype == TSA_F32 ? pick_gemm<true>(p, as_stream(stream)) : pick_gemm<false>(p, as_stream(stream)));
+        return TSA_OK;
+    }
     TSA_HIP_CHECK(launch_rows<-1>(rows_params(codes, scales, T, K, w, w_scales, N, bias, bias_dtype, y, y_dtype),
                                   as_stream(stream)));
     return TSA_OK;

@@ -8,7 +8,8 @@
 // output has one writer. Each is a stream of weights into the A operands of
 // v_mfma_f32_16x16x128_f8f6f4 (one column of B in use: the matrix cores are idle otherwise, and the
 // codes need no conversion).
-#include "fp8_common.h"
+#include "fp8_gemm.h"
+#include "moe_group.h"
 
 namespace tsa {
 namespace {
@@ -220,6 +221,253 @@ __global__ void __launch_bounds__(64 * F8D_NW) fp8_down_kernel(F8Moe p) {
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// ---------------------------------------------------------------- many tokens
+// Four launches: (1) the assignments grouped by expert with a table of token tiles (workgroup 0), x
+// quantised (the others); (2) gate_up over the tiles: 128 channels of gate and of up per workgroup, so
+// the epilogue holds whole groups of h and quantises them; (3) down, each assignment's output in
+// float32 at the assignment's place; (4) the weighted sums.
+struct F8Group {
+    tsa_expert_layout L;
+    const uint8_t* pool;
+    int64_t n_slots;
+    const int32_t* expert_slot;
+    int64_t E;
+    const int32_t* idx;
+    const float* wts;
+    int T, k;
+    const void* x;
+    void* y;
+    int y_dtype;
+    int32_t *counts, *offsets, *perm;
+    int* n_entries;
+    int4* table;  // (slot, first sorted row, rows, -)
+    int tile_rows;
+    uint8_t* xq;
+    float* xs;
+    uint8_t* hq;  // [sorted row, I]
+    float* hs;
+    float* yk;  // [T k, H]
+};
+
+constexpr int F8P_ROWS = 4;  // rows of x per quantising workgroup, 128 threads each
+
+template <int XT>
+__global__ void __launch_bounds__(GROUP_THREADS) fp8_prepare_kernel(F8Group p) {
+    extern __shared__ __align__(16) unsigned char gsm[];
+    if (blockIdx.x == 0) {
+        const GroupTiles tiles{p.expert_slot, p.n_slots, p.tile_rows, p.n_entries, p.table};
+        group_assignments<true>(p.idx, (int64_t)p.T * p.k, (int)p.E, p.counts, p.offsets, p.perm, tiles, GROUP_WAVES, gsm);
+        return;
+    }
+    const int H = (int)p.L.hidden, tasks = (int)f8_blocks(H) * 16, tid = (int)threadIdx.x & 127;
+    const int t = ((int)blockIdx.x - 1) * F8P_ROWS + ((int)threadIdx.x >> 7);
+    if (t >= p.T) return;
+    constexpr int ES = XT == TSA_F32 ? 4 : 2;
+    const uint8_t* row = static_cast<const uint8_t*>(p.x) + (int64_t)t * H * ES;
+    for (int c = tid; c < tasks; c += 128) {
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (8 * c < H) f8_load8<XT>(row, c, v);
+        const float s = f8_scale(f8_group_max(v));
+        const uint2 o = f8_codes8<XT == TSA_F32>(v, s);
+        if (8 * c < H) *reinterpret_cast<uint2*>(p.xq + (int64_t)t * H + 8 * c) = o;
+        if ((c & 15) == 0) p.xs[(int64_t)t * (tasks >> 4) + (c >> 4)] = s;
+    }
+}
+
+// The workgroup's (entry, tile) of n_entries x tiles: each XCD takes a run of the entries with all
+// their tiles (an expert's entries and an entry's tiles share an L2). False: none is left for it.
+__device__ __forceinline__ bool f8_work(const int* n_entries, int tiles, int& entry, int& tile) {
+    const int total = uniform(*n_entries) * tiles, lin = (int)blockIdx.x, xcd = lin & 7, q8 = total >> 3, rem = total & 7;
+    if ((lin >> 3) >= q8 + (xcd < rem ? 1 : 0)) return false;
+    const int wid = xcd * q8 + (xcd < rem ? xcd : rem) + (lin >> 3);
+    entry = wid / tiles;
+    tile = wid % tiles;
+    return true;
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    static_assert(C::RN == 2 * F8B && C::LDS >= C::TM * (F8B + 4 * C::WR), "one group of h per workgroup");
+    const tsa_expert_layout& L = p.L;
+    const int H = (int)L.hidden, I = (int)L.inter, GH = (int)f8_blocks(H), GI = (int)f8_blocks(I);
+    int entry, tile;
+    if (!f8_work(p.n_entries, GI, entry, tile)) return;
+    const int4 e = p.table[entry];
+    const int slot = uniform(e.x), row0 = uniform(e.y), tn = uniform(e.z), c0 = tile * F8B;
+    const uint8_t* base = p.pool + (int64_t)slot * L.slot_bytes;
+    const float* sg = reinterpret_cast<const float*>(base + L.gate_scales_off) + (int64_t)tile * GH;
+    F8Operands<2> o;
+    o.w[0] = base + L.gate_off + (int64_t)c0 * H;
+    o.w[1] = base + L.up_off + (int64_t)c0 * H;
+    o.w_rows = I - c0;
+    o.ws[0] = sg;
+    o.ws[1] = sg + (int64_t)GI * GH;
+    o.x = p.xq;
+    o.xs = p.xs;
+    o.x_records = (uint32_t)p.T * (uint32_t)H;
+    o.xs_records = (uint32_t)p.T * (uint32_t)GH * 4u;
+    o.K = H;
+    o.G = GH;
+    v4f acc[C::MR][C::MT];
+    f8_tile<C, 2, false>(o, smem, [&](int r) { return r < tn ? p.perm[row0 + r] / p.k : -1; }, acc);
+
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
+    const int wr = wave % C::WR, wt = wave / C::WR;
+    constexpr int MP = C::MR / 2;
+    uint8_t* stage = smem;                                              // [token][channel]
+    uint32_t* top = reinterpret_cast<uint32_t*>(smem + C::TM * F8B);    // [wr][token]
+    __syncthreads();  // the last block's reads
+#pragma unroll
+    for (int t = 0; t < C::MT; ++t) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < MP; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                acc[j][t][r] = f8_act(L, acc[j][t][r], acc[MP + j][t][r]);
+                m = max(m, __float_as_uint(acc[j][t][r]) & 0x7FFFFFFFu);
+            }
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        if (q == 0) top[wr * C::TM + 16 * (C::MT * wt + t) + i] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < C::MT; ++t) {
+        const int tk = 16 * (C::MT * wt + t) + i;
+        uint32_t m = 0;
+#pragma unroll
+        for (int w = 0; w < C::WR; ++w) m = max(m, top[w * C::TM + tk]);
+        const float s = f8_scale(m);
+#pragma unroll
+        for (int j = 0; j < MP; ++j)
+            *reinterpret_cast<uint32_t*>(stage + tk * F8B + 16 * (wr * MP + j) + 4 * q) = f8_codes4(acc[j][t], s);
+        if (wr == 0 && q == 0 && tk < tn) p.hs[(int64_t)(row0 + tk) * GI + tile] = s;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < tn * 8; c += C::THREADS) {
+        const int tk = c >> 3, col = 16 * (c & 7);
+        if (c0 + col < I)
+            *reinterpret_cast<u32x4*>(p.hq + (int64_t)(row0 + tk) * I + c0 + col) = *reinterpret_cast<const u32x4*>(stage + tk * F8B + col);
+    }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS) fp8_group_down_kernel(F8Group p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const tsa_expert_layout& L = p.L;
+    const int H = (int)L.hidden, I = (int)L.inter, GI = (int)f8_blocks(I);
+    int entry, tile;
+    if (!f8_work(p.n_entries, (H + C::RN - 1) / C::RN, entry, tile)) return;
+    const int4 e = p.table[entry];
+    const int slot = uniform(e.x), row0 = uniform(e.y), tn = uniform(e.z), n0 = tile * C::RN;
+    const uint8_t* base = p.pool + (int64_t)slot * L.slot_bytes;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
+    const int wr = wave % C::WR, wt = wave / C::WR, nw = n0 + wr * C::MR * 16;
+    static_assert(F8B % (C::MR * 16) == 0, "a wave's rows share their scales");
+    F8Operands<1> o;
+    o.w[0] = base + L.down_off + (int64_t)n0 * I;
+    o.w_rows = H - n0;
+    o.ws[0] = reinterpret_cast<const float*>(base + L.down_scales_off) + (int64_t)(nw < H ? nw / F8B : 0) * GI;
+    o.x = p.hq + (int64_t)row0 * I;
+    o.xs = p.hs + (int64_t)row0 * GI;
+    o.x_records = (uint32_t)tn * (uint32_t)I;
+    o.xs_records = (uint32_t)tn * (uint32_t)GI * 4u;
+    o.K = I;
+    o.G = GI;
+    v4f acc[C::MR][C::MT];
+    f8_tile<C, 1, false>(o, smem, [&](int r) { return r < tn ? r : -1; }, acc);
+#pragma unroll
+    for (int t = 0; t < C::MT; ++t) {
+        const int tk = 16 * (C::MT * wt + t) + i;
+        if (tk >= tn) continue;
+        float* dst = p.yk + (int64_t)p.perm[row0 + tk] * H;
+#pragma unroll
+        for (int m = 0; m < C::MR; ++m) {
+            const int n = nw + 16 * m + 4 * q;  // H % 32 == 0: all four or none
+            if (n < H) *reinterpret_cast<v4f*>(dst + n) = acc[m][t];
+        }
+    }
+}
+
+// y[t] = sum_j w[t, j] yk[t k + j], in order of j; a thread 4 values of a row.
+__global__ void __launch_bounds__(256) fp8_combine_kernel(F8Group p) {
+    const int H = (int)p.L.hidden, per = H / 4;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (int64_t)p.T * per) return;
+    const int t = (int)(at / per), c = 4 * (int)(at % per);
+    v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < p.k; ++j) {
+        const int64_t a = (int64_t)t * p.k + j;
+        const int e = p.idx[a], sl = e >= 0 && e < p.E ? p.expert_slot[e] : -1;
+        if (sl < 0 || sl >= p.n_slots) continue;  // not resident: nothing was written there
+        const float w = p.wts[a];
+        const v4f v = *reinterpret_cast<const v4f*>(p.yk + a * H + c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = fmaf(w, v[r], s[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) store_out(p.y, p.y_dtype, (int64_t)t * H + c + r, s[r]);
+}
+
+using GateUp128 = F8Tile<4, 2, 4, 4, 3>;  // 128 channels x 128 tokens, 8 waves
+using GateUp64 = F8Tile<8, 1, 2, 4, 3>;   // x 64
+using GateUp32 = F8Tile<4, 1, 4, 2, 2>;   // x 32, 4 waves
+using Down128 = F8Tile<2, 2, 4, 4, 2>;    // 128 rows x 128 tokens
+using Down64 = F8Tile<4, 1, 2, 4, 3>;
+using Down32 = F8Tile<4, 1, 2, 2, 3>;
+
+constexpr int64_t F8_CHUNK = 131072;  // assignments at a time: bounds the workspace (1.1 GiB at hidden 2048)
+
+int64_t group_tokens(int64_t T, int k) {
+    const int64_t c = F8_CHUNK / k > 0 ? F8_CHUNK / k : 1;
+    return T < c ? T : c;
+}
+
+struct F8Places {
+    int64_t counts, offsets, perm, n_entries, table, xq, xs, hq, hs, yk, bytes;
+};
+
+F8Places group_places(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
+    const int64_t n = T * k, H = L.hidden, I = L.inter;
+    F8Places w;
+    int64_t at = 0;
+    auto take = [&](int64_t b) {
+        const int64_t r = at;
+        at += align256(b);
+        return r;
+    };
+    w.counts = take(E * 4);
+    w.offsets = take((E + 1) * 4);
+    w.perm = take(n * 4);
+    w.n_entries = take(4);
+    w.table = take((n / 32 + E) * 16);
+    w.xq = take(T * H);
+    w.xs = take(T * f8_blocks(H) * 4);
+    w.hq = take(n * I);
+    w.hs = take(n * f8_blocks(I) * 4);
+    w.yk = take(n * H * 4);
+    w.bytes = at;
+    return w;
+}
+
+template <class GU, class DN>
+int group_gemms(const F8Group& p, int64_t entries, hipStream_t st) {
+    F8Group q = p;
+    void* args[] = {&q};
+    const void* fg = reinterpret_cast<const void*>(&fp8_group_gate_up_kernel<GU>);
+    const void* fd = reinterpret_cast<const void*>(&fp8_group_down_kernel<DN>);
+    TSA_HIP_CHECK(ensure_dynamic_lds(fg, GU::LDS));
+    TSA_HIP_CHECK(ensure_dynamic_lds(fd, DN::LDS));
+    static_assert(GU::TM == DN::TM, "one table of token tiles");
+    const int64_t tg = f8_blocks(p.L.inter), td = (p.L.hidden + DN::RN - 1) / DN::RN;
+    auto grid = [](int64_t n) { return dim3((unsigned)((n + 7) / 8 * 8)); };  // whole rounds of XCDs
+    TSA_HIP_CHECK(hipLaunchKernel(fg, grid(entries * tg), dim3(GU::THREADS), args, GU::LDS, st));
+    TSA_HIP_CHECK(hipLaunchKernel(fd, grid(entries * td), dim3(DN::THREADS), args, DN::LDS, st));
+    return TSA_OK;
+}
+
 }  // namespace
 
 // h [T k, I] fp32, then the routed selection.
@@ -275,6 +523,64 @@ int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, 
     void* args_b[] = {&pb};
     TSA_HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(&fp8_down_kernel), dim3((unsigned)((L.hidden + 15) / 16), (unsigned)T),
                                   dim3(64 * F8D_NW), args_b, lds_b, st));
+    return TSA_OK;
+}
+
+// Calls that the grouped kernels take.
+bool f8_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
+    return L.format == TSA_EXPERT_FP8 && T > 4 && E <= MAX_GROUP_E && k <= 64;
+}
+
+int64_t f8_group_workspace_bytes(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
+    return group_places(L, group_tokens(T, k), k, E).bytes;
+}
+
+int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const int32_t* expert_slot, int64_t E,
+                     const int32_t* idx, const float* weights, int64_t T, int k, const void* x, int x_dtype, void* y,
+                     int y_dtype, uint8_t* ws, hipStream_t st) {
+    const int64_t step = group_tokens(T, k), H = L.hidden;
+    const F8Places w = group_places(L, step, k, E);
+    const int lds = group_lds_bytes((int)E);
+    const void* fp = x_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_prepare_kernel<TSA_F32>)
+                     : x_dtype == TSA_F16 ? reinterpret_cast<const void*>(&fp8_prepare_kernel<TSA_F16>)
+                                          : reinterpret_cast<const void*>(&fp8_prepare_kernel<TSA_BF16>);
+    TSA_HIP_CHECK(ensure_dynamic_lds(fp, lds));
+    for (int64_t t0 = 0; t0 < T; t0 += step) {
+        F8Group p{};
+        p.L = L;
+        p.pool = pool;
+        p.n_slots = n_slots;
+        p.expert_slot = expert_slot;
+        p.E = E;
+        p.T = (int)(T - t0 < step ? T - t0 : step);
+        p.k = k;
+        p.idx = idx + t0 * k;
+        p.wts = weights + t0 * k;
+        p.x = static_cast<const uint8_t*>(x) + t0 * H * dtype_size(x_dtype);
+        p.y = static_cast<uint8_t*>(y) + t0 * H * dtype_size(y_dtype);
+        p.y_dtype = y_dtype;
+        p.counts = reinterpret_cast<int32_t*>(ws + w.counts);
+        p.offsets = reinterpret_cast<int32_t*>(ws + w.offsets);
+        p.perm = reinterpret_cast<int32_t*>(ws + w.perm);
+        p.n_entries = reinterpret_cast<int*>(ws + w.n_entries);
+        p.table = reinterpret_cast<int4*>(ws + w.table);
+        p.xq = ws + w.xq;
+        p.xs = reinterpret_cast<float*>(ws + w.xs);
+        p.hq = ws + w.hq;
+        p.hs = reinterpret_cast<float*>(ws + w.hs);
+        p.yk = reinterpret_cast<float*>(ws + w.yk);
+        const int64_t n = (int64_t)p.T * k;
+        p.tile_rows = n <= 16 * E ? 32 : n <= 64 * E ? 64 : 128;
+        const int64_t entries = n / p.tile_rows + (E < n ? E : n);
+        void* args[] = {&p};
+        TSA_HIP_CHECK(hipLaunchKernel(fp, dim3((unsigned)(1 + (p.T + F8P_ROWS - 1) / F8P_ROWS)), dim3(GROUP_THREADS), args, lds, st));
+        const int rc = p.tile_rows == 32 ? group_gemms<GateUp32, Down32>(p, entries, st)
+                       : p.tile_rows == 64 ? group_gemms<GateUp64, Down64>(p, entries, st)
+                                           : group_gemms<GateUp128, Down128>(p, entries, st);
+        if (rc) return rc;
+        hipLaunchKernelGGL(fp8_combine_kernel, dim3((unsigned)(((int64_t)p.T * (H / 4) + 255) / 256)), dim3(256), 0, st, p);
+        TSA_LAUNCH_CHECK();
+    }
     return TSA_OK;
 }
 

@@ -16,6 +16,12 @@ int gf_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots,
                const int32_t* idx, const float* weights, int64_t T, int k, const uint16_t* x, void* y, int y_dtype,
                uint8_t* ws, hipStream_t stream);
 
+bool f8_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E);
+int64_t f8_group_workspace_bytes(const tsa_expert_layout& L, int64_t T, int k, int64_t E);
+int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const int32_t* expert_slot, int64_t E,
+                     const int32_t* idx, const float* weights, int64_t T, int k, const void* x, int x_dtype, void* y,
+                     int y_dtype, uint8_t* ws, hipStream_t stream);
+
 namespace {
 
 __global__ void __launch_bounds__(GROUP_THREADS) group_kernel(const int32_t* __restrict__ idx, int64_t n, int E,
@@ -84,6 +90,7 @@ static int64_t prefill_ws(const tsa_expert_layout& L, int64_t T, int k, int64_t 
     int64_t g = 0;
     if (L.format == TSA_EXPERT_MXFP4 && L.mx_tiled) g = pf_mxt_workspace_bytes(L, T, k, E);
     if (gf_supported(L, TSA_BF16, T, k)) g = gf_workspace_bytes(L, T, k, E);
+    if (f8_group_supported(L, T, k, E)) g = f8_group_workspace_bytes(L, T, k, E);
     return g > c ? g : c;
 }
 
@@ -123,6 +130,14 @@ extern "C" int tsa_moe_prefill(const tsa_expert_layout* layout, const void* pool
         return gf_prefill(*layout, static_cast<const uint8_t*>(pool), n_slots, expert_slot, E, idx, weights, T, k,
                           static_cast<const uint16_t*>(x), y, y_dtype, static_cast<uint8_t*>(workspace),
                           as_stream(stream));
+    }
+    if (f8_group_supported(*layout, T, k, E)) {
+        TSA_REQUIRE(pool && x && y, TSA_ERR_INVALID_ARG, "null pointer");
+        TSA_REQUIRE(valid_dtype(x_dtype) && valid_dtype(y_dtype), TSA_ERR_INVALID_ARG, "bad dtype (x %d, y %d)", x_dtype, y_dtype);
+        TSA_REQUIRE(((reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(workspace)) & 15u) == 0,
+                    TSA_ERR_INVALID_ARG, "FP8 experts: pool, x and workspace must be 16-byte aligned");
+        return f8_group_prefill(*layout, static_cast<const uint8_t*>(pool), n_slots, expert_slot, E, idx, weights, T, k, x, x_dtype,
+                                y, y_dtype, static_cast<uint8_t*>(workspace), as_stream(stream));
     }
     int32_t* slots = static_cast<int32_t*>(workspace);
     const int64_t off = ((T * k * 4 + 255) / 256) * 256;
