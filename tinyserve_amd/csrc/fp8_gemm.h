@@ -7,7 +7,7 @@
 // (r / 2 % 8): the 16 rows that a quarter wave reads at once then fall on distinct banks. One MFMA
 // (v_mfma_f32_16x16x128_f8f6f4) makes a tile's sum over the block, which joins the float32 result
 // times the token's and the weight block's scale: 4 fused multiply-adds beside 32 cycles of the matrix
-// core. The tokens' scales of a block travel with it (a wave copies those of its own tokens).
+// core. The tokens' scales of a block travel with it.
 #pragma once
 
 #include "fp8_common.h"
@@ -41,11 +41,14 @@ __device__ __forceinline__ void f8_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// WR x WT waves of MR x MT tiles of 16 x 16, S stages.
 template <int WR_, int WT_, int MR_, int MT_, int S_>
 struct F8Tile {
     static constexpr int WR = WR_, WT = WT_, MR = MR_, MT = MT_, S = S_;
     static constexpr int NW = WR * WT, THREADS = 64 * NW, RN = 16 * WR * MR, TM = 16 * WT * MT;
     static constexpr int NXW = RN / 8 / NW, NXT = TM / 8 / NW;  // copies of 8 rows, a wave's
+    static constexpr int NS = 16 * MT / WR;  // tokens whose scales a wave copies
+    static_assert(NS * WR == 16 * MT, "tile");
     static constexpr int PER = NXW + NXT + 1;                   // copies a wave issues per block
     static constexpr int STAGE = (RN + TM) * F8B, LDS = S * STAGE + S * NW * 256;
     static_assert(RN % (8 * NW) == 0 && TM % (8 * NW) == 0 && MT <= 4 && (S - 2) * PER < 63, "tile");
@@ -66,9 +69,9 @@ struct F8Operands {
 
 // acc[m][t]: rows 4 q .. 4 q + 3 of tile m, token 16 t + i, for lane 16 q + i of the wave. Tile m is
 // the wave's m-th: of its MR, the first MR / PARTS belong to part 0. `token(r)`: row of x of the
-// tile's token r, or -1.
+// tile's token r, -1 from `tokens` on.
 template <class C, int PARTS, bool WIDE, class Token>
-__device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* smem, Token token, v4f (&acc)[C::MR][C::MT]) {
+__device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* smem, int tokens, Token token, v4f (&acc)[C::MR][C::MT]) {
     constexpr int MR = C::MR, MT = C::MT, S = C::S, HALF = C::RN / PARTS;
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
     const int wr = wave % C::WR, wt = wave / C::WR;
@@ -94,27 +97,29 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
     }
     uint32_t so;
     {
-        const int r = lane < 16 * MT ? token(16 * MT * wt + lane) : -1;
+        // the waves of a token column share its scales' copies: a row's scale is a line of its own
+        const int r = lane < C::NS ? token(16 * MT * wt + C::NS * wr + lane) : -1;
         so = r < 0 ? 0x80000000u : (uint32_t)r * (uint32_t)p.G * 4u;
     }
-    auto issue = [&](int s, int stage) {
+    // copy j (of PER) of block s: the weights', the tokens', the scales'. Columns past K and blocks past
+    // the last read zeros, so every step issues as many.
+    uint32_t at[2];  // this lane's column in copies of even and odd number
+#pragma unroll
+    for (int n = 0; n < 2; ++n) at[n] = 16u * chunk(n);
+    auto issue = [&](int j, int s, int stage) {
         const uint32_t col = (uint32_t)F8B * (uint32_t)s, base = lds0 + (uint32_t)stage * C::STAGE;
-        const bool tail = col + F8B > K;  // the row ends in this block
-#pragma unroll
-        for (int j = 0; j < C::NXW; ++j) {
+        if (j < C::NXW) {
             const int n = C::NXW * wave + j;
-            uint32_t o = wo[j];
-            if (tail && col + 16u * chunk(n) >= K) o = 0x80000000u;
-            f8_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], o, col, base + 1024u * (uint32_t)n);
+            const bool in = col + (n & 1 ? at[1] : at[0]) < K;
+            f8_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], in ? wo[j] : 0x80000000u, col, base + 1024u * (uint32_t)n);
+        } else if (j < C::NXW + C::NXT) {
+            const int n = C::NXT * wave + j - C::NXW;
+            const bool in = col + (n & 1 ? at[1] : at[0]) < K;
+            f8_copy16(rx, in ? xo[j - C::NXW] : 0x80000000u, col, base + (uint32_t)C::RN * F8B + 1024u * (uint32_t)n);
+        } else {
+            f8_copy4(rs, s < steps ? so : 0x80000000u, 4u * (uint32_t)s,
+                     lds0 + (uint32_t)(S * C::STAGE) + 256u * (uint32_t)(C::NW * stage + wave));
         }
-#pragma unroll
-        for (int j = 0; j < C::NXT; ++j) {
-            const int n = C::NXT * wave + j;
-            uint32_t o = xo[j];
-            if (tail && col + 16u * chunk(n) >= K) o = 0x80000000u;
-            f8_copy16(rx, o, col, base + (uint32_t)C::RN * F8B + 1024u * (uint32_t)n);
-        }
-        f8_copy4(rs, so, 4u * (uint32_t)s, lds0 + (uint32_t)(S * C::STAGE) + 256u * (uint32_t)(C::NW * stage + wave));
     };
 
 #pragma unroll
@@ -139,42 +144,73 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
     load_ws(0);
 #pragma unroll
     for (int s = 0; s < S - 1; ++s)
-        if (s < steps) issue(s, s);
-    int stage = 0;
-    for (int s = 0; s < steps; ++s) {
-        if ((s & 63) == 0 && s) load_ws(s);
-        // block s has landed (every wave's part of it), and the stage read in step s - 1 is free
-        if (s + S - 1 <= steps) f8_wait_barrier<(S - 2) * C::PER>();
-        else f8_wait_barrier<0>();
-        if (s + S - 1 < steps) issue(s + S - 1, stage == 0 ? S - 1 : stage - 1);
-        const uint8_t* wl = smem + stage * C::STAGE;
-        const uint8_t* xl = wl + C::RN * F8B + wt * (16 * MT * F8B);
-        const float* sl = reinterpret_cast<const float*>(smem + S * C::STAGE + 256 * (C::NW * stage + wave));
-        u32x4 Bv[MT][2];
+#pragma unroll
+        for (int j = 0; j < C::PER; ++j) issue(j, s, s);
+
+    // The blocks, for a wave whose first LIVE tiles of tokens hold any.
+    auto blocks = [&](auto live) {
+        constexpr int LIVE = decltype(live)::value, MP = MR / PARTS;
+        u32x4 A[2][2], Bv[MT][2];
         float sc[PARTS][MT];
+        v4f part[2][MT];
+        auto row_tile = [&](const uint8_t* wl, int m) { return wl + (m / MP * HALF + (wr * MP + m % MP) * 16) * F8B; };
+        auto scales = [&](int s, int stage) {
+            const float* sl = reinterpret_cast<const float*>(smem + S * C::STAGE + 256 * (C::NW * stage + C::WR * wt));
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            read(xl + t * (16 * F8B), Bv[t]);
-            const float sx = sl[16 * t + i];
+            for (int t = 0; t < LIVE; ++t) {
+                const float sx = sl[64 * ((16 * t + i) / C::NS) + (16 * t + i) % C::NS];
 #pragma unroll
-            for (int h = 0; h < PARTS; ++h)
-                sc[h][t] = sx * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wsv[h]), s & 63));
-        }
-#pragma unroll
-        for (int m = 0; m < MR; ++m) {
-            constexpr int MP = MR / PARTS;
-            const int h = m / MP;
-            u32x4 A[2];
-            read(wl + (h * HALF + (wr * MP + m % MP) * 16) * F8B, A);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const v4f part = f8_mfma<WIDE>(A, Bv[t]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(part[r], sc[h][t], acc[m][t][r]);
+                for (int h = 0; h < PARTS; ++h)
+                    sc[h][t] = sx * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wsv[h]), s & 63));
             }
+        };
+        auto fetch_b = [&](const uint8_t* wl) {
+#pragma unroll
+            for (int t = 0; t < LIVE; ++t) read(wl + C::RN * F8B + (wt * MT + t) * (16 * F8B), Bv[t]);
+        };
+        auto join = [&](int m, int t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(part[m & 1][t][r], sc[m / MP][t], acc[m][t][r]);
+        };
+        // The products of a block. A row tile's sums (part) join the results while the next row tile's
+        // are made: no multiply-add waits for the matrix core. The copies of block `next` go out between
+        // the row tiles: issued at once they hold up the wave until the memory pipe has taken them.
+        auto products = [&](const uint8_t* wl, int next, int stage) {
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+#pragma unroll
+                for (int t = 0; t < LIVE; ++t) {
+                    if (t == 0 && m + 1 < MR) read(row_tile(wl, m + 1), A[(m + 1) & 1]);
+                    part[m & 1][t] = f8_mfma<WIDE>(A[m & 1], Bv[t]);
+                    if (m) join(m - 1, t);
+                    if constexpr (!WIDE) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int j = m * C::PER / MR; j < (m + 1) * C::PER / MR; ++j) issue(j, next, stage);
+            }
+#pragma unroll
+            for (int t = 0; t < LIVE; ++t) join(MR - 1, t);
+        };
+        int stage = 0;
+        for (int s = 0; s < steps; ++s) {
+            if ((s & 63) == 0 && s) load_ws(s);
+            // block s has landed (every wave's part of it), and the stage read in step s - 1 is free
+            f8_wait_barrier<(S - 2) * C::PER>();
+            const uint8_t* wl = smem + stage * C::STAGE;
+            if (LIVE) read(row_tile(wl, 0), A[0]);
+            fetch_b(wl);
+            scales(s, stage);
+            products(wl, s + S - 1, stage == 0 ? S - 1 : stage - 1);
+            stage = stage + 1 == S ? 0 : stage + 1;
         }
-        stage = stage + 1 == S ? 0 : stage + 1;
-    }
+    };
+    // tiles without tokens (a short last tile of a prompt, an expert with few) are left out
+    const int live = (tokens - 16 * MT * wt + 15) / 16;
+    if (live >= MT || (MT == 4 && live == 3)) blocks(std::integral_constant<int, MT>{});
+    else if (live == 2) blocks(std::integral_constant<int, (MT > 2 ? 2 : MT)>{});
+    else if (live == 1) blocks(std::integral_constant<int, 1>{});
+    else blocks(std::integral_constant<int, 0>{});
+    f8_wait_barrier<0>();  // LDS is free
 }
 
 }  // namespace

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_gemm_kernel(F8Gemm p) {
     o.K = p.K;
     o.G = p.G;
     v4f acc[C::MR][C::MT];
-    f8_tile<C, 1, WIDE>(o, smem, [&](int r) { return r < tn ? r : -1; }, acc);
+    f8_tile<C, 1, WIDE>(o, smem, tn, [&](int r) { return r < tn ? r : -1; }, acc);
 #pragma unroll
     for (int m = 0; m < C::MR; ++m) {
         const int n = nw + 16 * m + 4 * q;
@@ -253,13 +253,15 @@ hipError_t pick_gemm(const F8Gemm& p, hipStream_t st) {
     const int64_t cus = num_cus() > 0 ? num_cus() : 256;
     int best = 0;
     int64_t least = INT64_MAX;
-    for (int i = 0; i < 5; ++i) {
+    for (int i = WIDE ? 1 : 0; i < 5; ++i) {  // 256 x 256 has no registers for the widened operands
         const int64_t wgs = (int64_t)((p.N + tiles[i].rows - 1) / tiles[i].rows) * ((p.T + tiles[i].tok - 1) / tiles[i].tok);
         const int64_t cost = (wgs + cus * tiles[i].per - 1) / (cus * tiles[i].per) * tiles[i].cost;
         if (cost < least) least = cost, best = i;
     }
     switch (best) {
-        case 0: return launch_gemm<TileA, WIDE>(p, st);
+        case 0:
+            if constexpr (!WIDE) return launch_gemm<TileA, WIDE>(p, st);
+            return hipErrorInvalidValue;
         case 1: return launch_gemm<TileB, WIDE>(p, st);
         case 2: return launch_gemm<TileC, WIDE>(p, st);
         case 3: return launch_gemm<TileD, WIDE>(p, st);

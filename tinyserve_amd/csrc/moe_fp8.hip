@@ -4,10 +4,10 @@
 // h = act(Wg x, Wu x) in float32, quantised the same way; y = sum_j w_j Wd h, rounded once.
 //
 // Few tokens: two launches ordered by the stream. gate_up: one workgroup per (token, expert) pair
-// and 16 channels; down: one per token and 16 outputs, over all the token's experts, so every
+// and 8 channels; down: one per token and 8 outputs, over all the token's experts, so every
 // output has one writer. Each is a stream of weights into the A operands of
-// v_mfma_f32_16x16x128_f8f6f4 (one column of B in use: the matrix cores are idle otherwise, and the
-// codes need no conversion).
+// v_mfma_f32_16x16x128_f8f6f4 (one or two columns of B in use: the matrix cores are idle otherwise, and
+// the codes need no conversion).
 #include "fp8_gemm.h"
 #include "moe_group.h"
 
@@ -35,25 +35,46 @@ struct F8Moe {
     int chunk;  // down: experts staged in LDS at a time
 };
 
-constexpr int F8A_NW = 4, F8A_D = 4;  // gate_up: waves, K blocks in flight per wave
-constexpr int F8D_NW = 8, F8D_D = 6;  // down
+constexpr int F8A_NW = 8, F8A_D = 3, F8A_XC = 1;  // gate_up: waves; K blocks in flight per wave; chunks of x held per thread
+constexpr int F8D_NW = 8, F8D_D = 3, F8D_HC = 2;  // down: the same with its units and h
 
 __device__ __forceinline__ float f8_act(const tsa_expert_layout& L, float gate, float up) {
     if (L.act == TSA_ACT_SWIGLU_OAI) return swiglu_oai_fast(L, gate, up);
     return silu_mul_fast(gate, up);
 }
 
+// A chunk of 8 values of a group (16 lanes a group) into its place in LDS.
+template <bool EXACT>
+__device__ __forceinline__ void f8_put8(const float (&v)[8], int c, uint8_t* codes, float* scales) {
+    const float s = f8_scale(f8_group_max(v));
+    *reinterpret_cast<uint2*>(codes + 8 * c) = f8_codes8<EXACT>(v, s);
+    if ((c & 15) == 0) scales[c >> 4] = s;
+}
+
+// One workgroup per (token, expert) pair and 8 channels: rows 0 .. 7 of the tile are the channels' gate
+// rows, 8 .. 15 their up rows, so one pair gives enough workgroups (768 at inter 768 and top-8, three
+// whole rounds of the CUs; tiles of 16 channels give 384, one and a half: 9.5 us against 7.0). Loads
+// go out in the order of their use: x, the routing's inputs, then every weight of the tile; x is
+// quantised while the weights are on their way.
 template <int XT>
 __global__ void __launch_bounds__(64 * F8A_NW) fp8_gate_up_kernel(F8Moe p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), q = lane >> 4, i = lane & 15;
     const tsa_expert_layout& L = p.L;
-    const int H = (int)L.hidden, I = (int)L.inter, k = p.k, G = (int)f8_blocks(H);
-    const int a = blockIdx.y, t = a / k, jj = a % k, n0 = (int)blockIdx.x * 16;
+    const int H = (int)L.hidden, I = (int)L.inter, k = p.k, G = (int)f8_blocks(H), GI = (int)f8_blocks(I);
+    const int a = blockIdx.y, t = a / k, jj = a % k, n0 = (int)blockIdx.x * 8;
     uint8_t* xc = smem;
     float* xs = reinterpret_cast<float*>(smem + G * F8B);
-    float* red = xs + G;  // [wave][gate / up][row]
-
+    float* red = reinterpret_cast<float*>(smem + (G * (F8B + 4) + 15) / 16 * 16);  // [wave][gate / up][channel]
+    constexpr int ES = XT == TSA_F32 ? 4 : 2, NT = 64 * F8A_NW;
+    const uint8_t* xrow = static_cast<const uint8_t*>(p.x) + (int64_t)t * H * ES;
+    float xv[F8A_XC][8];
+#pragma unroll
+    for (int c = 0; c < F8A_XC; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) xv[c][e] = 0.0f;
+        if (8 * (tid + NT * c) < H) f8_load8<XT>(xrow, tid + NT * c, xv[c]);
+    }
     int64_t slot = -1;
     if (p.logits) {
         // every wave selects the pair's expert (round jj of the top-k); wave 0 of the token's first
@@ -86,28 +107,34 @@ __global__ void __launch_bounds__(64 * F8A_NW) fp8_gate_up_kernel(F8Moe p) {
     if (slot < 0 || slot >= p.n_slots) return;  // every wave of the workgroup: the pair's h is never read
 
     const uint8_t* base = p.pool + slot * L.slot_bytes;
-    const int64_t records = (int64_t)(I - n0 < 16 ? I - n0 : 16) * H;
-    const __amdgpu_buffer_rsrc_t rg = f8_buf(base + L.gate_off + (int64_t)n0 * H, records);
-    const __amdgpu_buffer_rsrc_t ru = f8_buf(base + L.up_off + (int64_t)n0 * H, records);
-    const float* sg = reinterpret_cast<const float*>(base + L.gate_scales_off) + n0 / F8B * G;
-    const float* su = sg + f8_blocks(I) * G;
-    u32x4 A[F8A_D][2][2];
+    const __amdgpu_buffer_rsrc_t r = f8_buf(base, L.slot_bytes);
+    const uint32_t row = n0 + (i & 7) < I ? (uint32_t)((i >> 3) ? L.up_off : L.gate_off) + (uint32_t)(n0 + (i & 7)) * (uint32_t)H
+                                          : 0x80000000u;
+    const uint32_t scale = (uint32_t)L.gate_scales_off + 4u * (uint32_t)(((q >> 1) * GI + n0 / F8B) * G);
+    u32x4 A[F8A_D][2];
+    float ws[F8A_D];
     auto load = [&](int j0) {
 #pragma unroll
         for (int d = 0; d < F8A_D; ++d) {
-            const uint32_t o = (uint32_t)(F8B * (wave + F8A_NW * (j0 + d)) + 16 * q);
-            const uint32_t o0 = f8_off((uint32_t)(i * H), o, (uint32_t)H), o1 = f8_off((uint32_t)(i * H), o + 64, (uint32_t)H);
-            A[d][0][0] = f8_ld(rg, o0);
-            A[d][0][1] = f8_ld(rg, o1);
-            A[d][1][0] = f8_ld(ru, o0);
-            A[d][1][1] = f8_ld(ru, o1);
+            const int b = wave + F8A_NW * (j0 + d);
+            if (b >= G) break;
+            const uint32_t o = (uint32_t)(F8B * b + 16 * q);
+            A[d][0] = f8_ld(r, o < (uint32_t)H ? row + o : 0x80000000u);
+            A[d][1] = f8_ld(r, o + 64 < (uint32_t)H ? row + o + 64 : 0x80000000u);
+            ws[d] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (int)(scale + 4u * (uint32_t)b), 0, 0));
         }
     };
     load(0);
-    constexpr int ES = XT == TSA_F32 ? 4 : 2;
-    f8_stage_row<XT>(static_cast<const uint8_t*>(p.x) + (int64_t)t * H * ES, H, xc, xs, tid, 64 * F8A_NW);
+#pragma unroll
+    for (int c = 0; c < F8A_XC; ++c)
+        if (tid + NT * c < 16 * G) f8_put8<XT == TSA_F32>(xv[c], tid + NT * c, xc, xs);
+    for (int c = tid + NT * F8A_XC; c < 16 * G; c += NT) {  // the rest of a long row
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (8 * c < H) f8_load8<XT>(xrow, c, v);
+        f8_put8<XT == TSA_F32>(v, c, xc, xs);
+    }
     __syncthreads();
-    v4f acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const int steps = (G + F8A_NW - 1) / F8A_NW;
     for (int j0 = 0; j0 < steps; j0 += F8A_D) {
         if (j0) load(j0);
@@ -120,101 +147,116 @@ __global__ void __launch_bounds__(64 * F8A_NW) fp8_gate_up_kernel(F8Moe p) {
                 Bv[0] = *reinterpret_cast<const u32x4*>(xc + F8B * b + 16 * q);
                 Bv[1] = *reinterpret_cast<const u32x4*>(xc + F8B * b + 64 + 16 * q);
             }
-            const float sx = xs[b], s[2] = {sg[b] * sx, su[b] * sx};
+            const float s = ws[d] * xs[b];
+            const v4f part = f8_mfma(A[d], Bv);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const v4f part = f8_mfma(A[d][m], Bv);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(s[m], part[r], acc[m][r]);
-            }
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(s, part[e], acc[e]);
         }
     }
-    if (i == 0) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) red[(wave * 2 + m) * 16 + 4 * q + r] = acc[m][r];
-    }
+    if (i == 0) *reinterpret_cast<v4f*>(red + wave * 16 + 4 * q) = acc;
     __syncthreads();
-    if (tid < 16 && n0 + tid < I) {
+    if (tid < 8 && n0 + tid < I) {
         float g = 0.0f, u = 0.0f;
 #pragma unroll
-        for (int w = 0; w < F8A_NW; ++w) g += red[(2 * w) * 16 + tid], u += red[(2 * w + 1) * 16 + tid];
+        for (int w = 0; w < F8A_NW; ++w) g += red[16 * w + tid], u += red[16 * w + 8 + tid];
         p.h[(int64_t)a * I + n0 + tid] = f8_act(L, g, u);
     }
 }
 
-__global__ void __launch_bounds__(64 * F8D_NW) fp8_down_kernel(F8Moe p) {
+__device__ const uint32_t f8_zeros[4] = {0, 0, 0, 0};  // what lanes past a matrix read
+
+// One workgroup per token and 8 outputs, over all the token's experts: rows 0 .. 7 of a tile are the
+// outputs' rows of an even expert, 8 .. 15 those of the next, which meet columns 0 and 1 (their h); a
+// unit is a K block of such a pair, and the waves take the units in turn.
+__global__ void __launch_bounds__(64 * F8D_NW, 4) fp8_down_kernel(F8Moe p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), q = lane >> 4, i = lane & 15;
     const tsa_expert_layout& L = p.L;
     const int H = (int)L.hidden, I = (int)L.inter, k = p.k, G = (int)f8_blocks(I);
-    const int t = blockIdx.y, n0 = (int)blockIdx.x * 16;
-    __shared__ float red[F8D_NW * 16];
+    const int t = blockIdx.y, n0 = (int)blockIdx.x * 8;
+    constexpr int NT = 64 * F8D_NW;
+    __shared__ __align__(16) float red[F8D_NW * 16];
     uint8_t* hc = smem;                                              // [expert of the chunk][G 128]
     float* hs = reinterpret_cast<float*>(smem + p.chunk * G * F8B);  // [expert of the chunk][G]
-    const int32_t* slots = p.slots + (int64_t)t * k;
-    const float* wts = p.wts + (int64_t)t * k;
+    // lane j: the token's j-th slot (-1: none) and weight
+    int my_slot = -1;
+    float my_w = 0.0f;
+    if (lane < k) {
+        my_slot = p.slots[(int64_t)t * k + lane];
+        my_w = p.wts[(int64_t)t * k + lane];
+    }
+    my_slot = my_slot < p.n_slots ? my_slot : -1;
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int c0 = 0; c0 < k; c0 += p.chunk) {  // workgroup-uniform
-        const int nc = k - c0 < p.chunk ? k - c0 : p.chunk, units = nc * G;
-        // unit u: K block u % G of the chunk's expert u / G, one wave's
-        auto live = [&](int j) {
-            const int s = uniform(slots[c0 + j]);
-            return s >= 0 && s < p.n_slots ? s : -1;
+        const int nc = k - c0 < p.chunk ? k - c0 : p.chunk, units = (nc + 1) / 2 * G, tasks = nc * G * 16;
+        // h of the chunk: [expert][group][16 chunks of 8], a dead expert's as zeros
+        const float* hrow = p.h + ((int64_t)t * k + c0) * I;
+        auto load_h = [&](int c, float (&v)[8]) {
+            const int j = c / (G * 16), o = 8 * (c % (G * 16));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            if (c < tasks && o < I && __shfl(my_slot, (c0 + j) & 63, 64) >= 0) f8_load8<TSA_F32>(hrow + (int64_t)j * I, o / 8, v);
         };
+        float hv[F8D_HC][8];
+#pragma unroll
+        for (int c = 0; c < F8D_HC; ++c) load_h(tid + NT * c, hv[c]);
         u32x4 A[F8D_D][2];
         float sc[F8D_D];
         auto load = [&](int u0) {
 #pragma unroll
             for (int d = 0; d < F8D_D; ++d) {
-                const int u = u0 + F8D_NW * d;
-                sc[d] = 0.0f;
-                if (u >= units) continue;
-                const int j = u / G, b = u % G, s = live(j);
-                if (s < 0) continue;
-                const uint8_t* base = p.pool + s * L.slot_bytes;
-                const __amdgpu_buffer_rsrc_t r =
-                    f8_buf(base + L.down_off + (int64_t)n0 * I, (int64_t)(H - n0 < 16 ? H - n0 : 16) * I);
-                const uint32_t o = (uint32_t)(F8B * b + 16 * q);
-                A[d][0] = f8_ld(r, f8_off((uint32_t)(i * I), o, (uint32_t)I));
-                A[d][1] = f8_ld(r, f8_off((uint32_t)(i * I), o + 64, (uint32_t)I));
-                sc[d] = wts[c0 + j] * reinterpret_cast<const float*>(base + L.down_scales_off)[n0 / F8B * G + b];
+                const int u = u0 + F8D_NW * d, pair = u / G, b = u % G;
+                if (u >= units) break;
+                const int ja = 2 * pair + (i >> 3), js = 2 * pair + (q >> 1);  // of the lane's row of A, of its sums
+                const int sa = ja < nc ? __shfl(my_slot, (c0 + ja) & 63, 64) : -1;
+                const int ss = js < nc ? __shfl(my_slot, (c0 + js) & 63, 64) : -1;
+                const float w = __shfl(my_w, (c0 + js) & 63, 64);
+                const int o = F8B * b + 16 * q, row = n0 + (i & 7);
+                const uint8_t* at = p.pool + (int64_t)sa * L.slot_bytes + L.down_off + (int64_t)row * I + o;
+                const bool ok = sa >= 0 && row < H;
+                const void* z = f8_zeros;
+                A[d][0] = *static_cast<const u32x4*>(ok && o < I ? at : z);
+                A[d][1] = *static_cast<const u32x4*>(ok && o + 64 < I ? at + 64 : z);
+                const float* sp = reinterpret_cast<const float*>(p.pool + (int64_t)ss * L.slot_bytes + L.down_scales_off) + n0 / F8B * G + b;
+                sc[d] = w * *(ss >= 0 ? sp : static_cast<const float*>(z));
             }
         };
         load(wave);
         if (c0) __syncthreads();  // the chunk before is used up
-        for (int j = 0; j < nc; ++j)
-            if (live(j) >= 0)
-                f8_stage_row<TSA_F32>(p.h + ((int64_t)t * k + c0 + j) * I, I, hc + j * G * F8B, hs + j * G, tid, 64 * F8D_NW);
+#pragma unroll
+        for (int c = 0; c < F8D_HC; ++c)
+            if (tid + NT * c < tasks) f8_put8<false>(hv[c], tid + NT * c, hc, hs);
+        for (int c = tid + NT * F8D_HC; c < (tasks + 63) / 64 * 64; c += NT) {  // whole waves: load_h shuffles
+            float v[8];
+            load_h(c, v);
+            if (c < tasks) f8_put8<false>(v, c, hc, hs);
+        }
         __syncthreads();
         for (int u0 = wave; u0 < units; u0 += F8D_NW * F8D_D) {
             if (u0 != wave) load(u0);
 #pragma unroll
             for (int d = 0; d < F8D_D; ++d) {
                 const int u = u0 + F8D_NW * d;
-                if (u >= units || live(u / G) < 0) continue;
+                if (u >= units) break;
+                const int pair = u / G, b = u % G, j = 2 * pair + i, js = 2 * pair + (q >> 1);
                 u32x4 Bv[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-                if (i == 0) {
-                    Bv[0] = *reinterpret_cast<const u32x4*>(hc + F8B * u + 16 * q);
-                    Bv[1] = *reinterpret_cast<const u32x4*>(hc + F8B * u + 64 + 16 * q);
+                if (i < 2 && j < nc) {
+                    Bv[0] = *reinterpret_cast<const u32x4*>(hc + F8B * (j * G + b) + 16 * q);
+                    Bv[1] = *reinterpret_cast<const u32x4*>(hc + F8B * (j * G + b) + 64 + 16 * q);
                 }
-                const float s = sc[d] * hs[u];
+                const float s = js < nc ? sc[d] * hs[js * G + b] : 0.0f;
                 const v4f part = f8_mfma(A[d], Bv);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[r] = fmaf(s, part[r], acc[r]);
+                for (int e = 0; e < 4; ++e) acc[e] = fmaf(s, part[e], acc[e]);
             }
         }
     }
-    if (i == 0) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) red[wave * 16 + 4 * q + r] = acc[r];
-    }
+    if (i == (q >> 1)) *reinterpret_cast<v4f*>(red + wave * 16 + 4 * q) = acc;  // an expert's rows in its own column
     __syncthreads();
-    if (tid < 16 && n0 + tid < H) {
+    if (tid < 8 && n0 + tid < H) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < F8D_NW; ++w) v += red[16 * w + tid];
+        for (int w = 0; w < F8D_NW; ++w) v += red[16 * w + tid] + red[16 * w + 8 + tid];
         store_out(p.y, p.y_dtype, (int64_t)t * H + n0 + tid, v);
     }
 }
@@ -310,14 +352,13 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p
     o.K = H;
     o.G = GH;
     v4f acc[C::MR][C::MT];
-    f8_tile<C, 2, false>(o, smem, [&](int r) { return r < tn ? p.perm[row0 + r] / p.k : -1; }, acc);
+    f8_tile<C, 2, false>(o, smem, tn, [&](int r) { return r < tn ? p.perm[row0 + r] / p.k : -1; }, acc);
 
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
     const int wr = wave % C::WR, wt = wave / C::WR;
     constexpr int MP = C::MR / 2;
     uint8_t* stage = smem;                                              // [token][channel]
     uint32_t* top = reinterpret_cast<uint32_t*>(smem + C::TM * F8B);    // [wr][token]
-    __syncthreads();  // the last block's reads
 #pragma unroll
     for (int t = 0; t < C::MT; ++t) {
         uint32_t m = 0;
@@ -377,7 +418,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_down_kernel(F8Group p) {
     o.K = I;
     o.G = GI;
     v4f acc[C::MR][C::MT];
-    f8_tile<C, 1, false>(o, smem, [&](int r) { return r < tn ? r : -1; }, acc);
+    f8_tile<C, 1, false>(o, smem, tn, [&](int r) { return r < tn ? r : -1; }, acc);
 #pragma unroll
     for (int t = 0; t < C::MT; ++t) {
         const int tk = 16 * (C::MT * wt + t) + i;
@@ -509,19 +550,19 @@ int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, 
     p.y_dtype = y_dtype;
     const int GH = (int)f8_blocks(L.hidden), GI = (int)f8_blocks(L.inter), row = GI * (F8B + 4);
     p.chunk = k * row <= 60 * 1024 ? k : 60 * 1024 / row;  // at least 3 rows of 16384
-    const int lds_a = GH * (F8B + 4) + F8A_NW * 32 * 4, lds_b = p.chunk * row;
+    const int lds_a = (GH * (F8B + 4) + 15) / 16 * 16 + F8A_NW * 16 * 4, lds_b = p.chunk * row;
     const void* fa = x_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_gate_up_kernel<TSA_F32>)
                      : x_dtype == TSA_F16 ? reinterpret_cast<const void*>(&fp8_gate_up_kernel<TSA_F16>)
                                           : reinterpret_cast<const void*>(&fp8_gate_up_kernel<TSA_BF16>);
     void* args[] = {&p};
-    TSA_HIP_CHECK(hipLaunchKernel(fa, dim3((unsigned)((L.inter + 15) / 16), (unsigned)(T * k)), dim3(64 * F8A_NW), args, lds_a, st));
+    TSA_HIP_CHECK(hipLaunchKernel(fa, dim3((unsigned)((L.inter + 7) / 8), (unsigned)(T * k)), dim3(64 * F8A_NW), args, lds_a, st));
     F8Moe pb = p;  // the down launch reads the routed table, or the caller's
     if (logits) {
         pb.slots = p.tab_slot;
         pb.wts = p.tab_w;
     }
     void* args_b[] = {&pb};
-    TSA_HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(&fp8_down_kernel), dim3((unsigned)((L.hidden + 15) / 16), (unsigned)T),
+    TSA_HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(&fp8_down_kernel), dim3((unsigned)((L.hidden + 7) / 8), (unsigned)T),
                                   dim3(64 * F8D_NW), args_b, lds_b, st));
     return TSA_OK;
 }
@@ -588,6 +629,7 @@ int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_
 const char* f8_unsupported(const tsa_expert_layout& L) {
     if (L.gate_bias_off >= 0 || L.down_bias_off >= 0) return "FP8 experts carry no biases";
     if ((L.slot_bytes | L.gate_off | L.up_off | L.down_off) & 15) return "FP8 slots and matrices must start on multiples of 16 bytes";
+    if (L.slot_bytes >= ((int64_t)1 << 31)) return "FP8 slots of 2^31 bytes and more are not supported";
     if ((L.gate_scales_off | L.down_scales_off) & 3) return "FP8 scales must start on multiples of 4 bytes";
     return "";
 }
