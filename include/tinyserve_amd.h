@@ -155,7 +155,7 @@ int tsa_fp8_quantize(const void* x, int x_dtype, int64_t T, int64_t K, void* cod
 int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T, int64_t K, const void* w, const float* w_scales,
                    int64_t N, const void* bias, int bias_dtype, void* y, int y_dtype, void* stream);
 
-/* Workspace bytes of tsa_fp8_linear (16-byte aligned, no initialisation). */
+/* Workspace bytes of tsa_fp8_linear (16-byte aligned, no initialisation); 0 for few tokens. */
 int tsa_fp8_linear_workspace_size(int64_t T, int64_t K, int64_t* bytes);
 
 /* tsa_fp8_quantize of x [T, K] followed by tsa_fp8_matmul; few tokens are quantised inside the

@@ -147,11 +147,15 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_HERE = contextlib.nullcontext()
+_device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # the first is not a public name
+
+
 def on_device(t: torch.Tensor):
-    """A context with the tensor's device current (kernels are launched on the current device);
+    """A context with the GPU tensor's device current (kernels are launched on the current device);
     nothing to do where it is already."""
     d = t.get_device()
-    return contextlib.nullcontext() if d == torch.cuda.current_device() else torch.cuda.device(d)
+    return _HERE if d == _device_index() else torch.cuda.device(d)
 
 
 def require_device(*tensors: torch.Tensor, what: str = "tensor") -> None:

@@ -131,18 +131,12 @@ __device__ __forceinline__ uint32_t f8_codes4(const v4f& v, float s) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
 }
 
-// A row of K values (K % 16 == 0) quantised into LDS by `nthreads` threads, 16 lanes a group: codes
-// padded with zeros to whole groups, one scale per group.
-template <int XT>
-__device__ __forceinline__ void f8_stage_row(const void* row, int K, uint8_t* codes, float* scales, int tid, int nthreads) {
-    const int tasks = (int)f8_blocks(K) * 16;
-    for (int c = tid; c < tasks; c += nthreads) {
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (8 * c < K) f8_load8<XT>(row, c, v);
-        const float s = f8_scale(f8_group_max(v));
-        *reinterpret_cast<uint2*>(codes + 8 * c) = f8_codes8<XT == TSA_F32>(v, s);
-        if ((c & 15) == 0) scales[c >> 4] = s;
-    }
+// Piece c (8 values) of a row, 16 lanes a group, quantised into the row's codes and scales in LDS.
+template <bool EXACT>
+__device__ __forceinline__ void f8_put8(const float (&v)[8], int c, uint8_t* codes, float* scales) {
+    const float s = f8_scale(f8_group_max(v));
+    *reinterpret_cast<uint2*>(codes + 8 * c) = f8_codes8<EXACT>(v, s);
+    if ((c & 15) == 0) scales[c >> 4] = s;
 }
 
 // Rows of 16 bytes from a matrix: a buffer over `records` bytes from p, whose offsets past the end

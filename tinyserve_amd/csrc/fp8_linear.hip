@@ -62,98 +62,138 @@ struct F8Rows {
     int tiles_n, rows;  // rows: tokens of the largest tile
 };
 
-constexpr int F8R_D = 6;  // K blocks a wave has in flight
+constexpr int F8R_NW = 8, F8R_D = 3;  // waves; K blocks a wave has in flight
 
-// Workgroup = 16 weight rows x 16 tokens, its NW waves take the K blocks in turn and their sums meet
-// in LDS. The weights come straight into the A operand's registers (every byte is read by one lane
-// of the workgroup), the tokens' codes from memory, or quantised here into LDS (XT: the dtype).
-template <int XT, int NW, bool WIDE>
-__global__ void __launch_bounds__(64 * NW) fp8_rows_kernel(F8Rows p) {
+// The linear id's place when each of the 8 XCDs (dealt round by id) takes a run: a bijection of [0, total).
+__device__ __forceinline__ int f8_run(int lin, int total) {
+    const int xcd = lin & 7, rem = total & 7;
+    return xcd * (total >> 3) + (xcd < rem ? xcd : rem) + (lin >> 3);
+}
+
+// Workgroup = 16 weight rows x 16 MT tokens; its waves take the K blocks in turn and their sums meet in
+// LDS. The weights come straight into the A operand's registers (every byte is read by one lane of
+// the workgroup), the tokens' codes from memory, or (XT: their dtype, up to 16 tokens) quantised here
+// into LDS while the weights are on their way.
+template <int XT, int MT, bool WIDE>
+__global__ void __launch_bounds__(64 * F8R_NW) fp8_rows_kernel(F8Rows p) {
     extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int NT = 64 * F8R_NW;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), q = lane >> 4, i = lane & 15;
-    const int64_t n0 = (int64_t)(blockIdx.x % p.tiles_n) * 16, t0 = (int64_t)(blockIdx.x / p.tiles_n) * 16;
-    const int tn = (int)(p.T - t0 < 16 ? p.T - t0 : 16), K = p.K, G = p.G;
-    const int ld = G * F8B + 16;  // LDS row of codes
+    const int wid = f8_run((int)blockIdx.x, (int)gridDim.x), tt = (int)gridDim.x / p.tiles_n;
+    const int64_t n0 = (int64_t)(wid / tt) * 16, t0 = (int64_t)(wid % tt) * (16 * MT);
+    const int tn = (int)(p.T - t0 < 16 * MT ? p.T - t0 : 16 * MT), K = p.K, G = p.G;
+    const int ld = G * F8B + 16, tasks = G * 16;  // LDS row of codes; pieces of 8 of a token
+    static_assert(XT < 0 || MT == 1, "one token tile is quantised here");
+    constexpr int ES = XT == TSA_F32 ? 4 : 2;
+    const uint8_t* xrow = static_cast<const uint8_t*>(p.x) + t0 * K * (XT < 0 ? 1 : ES);
+    float xv[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (XT >= 0) {  // the first token's values ahead of the weights
+        if (8 * tid < K) f8_load8<XT>(xrow, tid, xv);
+    }
     const __amdgpu_buffer_rsrc_t rw = f8_buf(p.w + n0 * K, (p.N - n0 < 16 ? p.N - n0 : 16) * K);
+    const __amdgpu_buffer_rsrc_t rx = f8_buf(xrow, XT >= 0 ? 0 : (int64_t)tn * K);
     const float* sw = p.ws + n0 / F8B * G;
-    u32x4 A[F8R_D][2];
+    const float* xs = p.xs + (XT < 0 ? t0 * G : 0);
+    u32x4 A[F8R_D][2], Bv[F8R_D][MT][2];
+    float sc[F8R_D][MT];
     auto load = [&](int j0) {
 #pragma unroll
         for (int d = 0; d < F8R_D; ++d) {
-            const uint32_t o = (uint32_t)(F8B * (wave + NW * (j0 + d)) + 16 * q);
-            A[d][0] = f8_ld(rw, f8_off((uint32_t)(i * K), o, (uint32_t)K));
-            A[d][1] = f8_ld(rw, f8_off((uint32_t)(i * K), o + 64, (uint32_t)K));
+            const int b = wave + F8R_NW * (j0 + d);
+            if (b >= G) break;
+            const uint32_t o = (uint32_t)(F8B * b + 16 * q), row = (uint32_t)(i * K);
+            A[d][0] = f8_ld(rw, f8_off(row, o, (uint32_t)K));
+            A[d][1] = f8_ld(rw, f8_off(row, o + 64, (uint32_t)K));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if constexpr (XT < 0) {
+                    Bv[d][m][0] = f8_ld(rx, f8_off(row + (uint32_t)(16 * m * K), o, (uint32_t)K));
+                    Bv[d][m][1] = f8_ld(rx, f8_off(row + (uint32_t)(16 * m * K), o + 64, (uint32_t)K));
+                    sc[d][m] = 16 * m + i < tn ? xs[(int64_t)(16 * m + i) * G + b] : 0.0f;
+                }
+            }
         }
     };
     load(0);
     uint8_t* xc = smem;
-    float* xs = reinterpret_cast<float*>(smem + p.rows * ld);
+    float* xl = reinterpret_cast<float*>(smem + p.rows * ld);
     if constexpr (XT >= 0) {
-        constexpr int ES = XT == TSA_F32 ? 4 : 2;
         for (int r = 0; r < tn; ++r)
-            f8_stage_row<XT>(static_cast<const uint8_t*>(p.x) + (t0 + r) * K * ES, K, xc + r * ld, xs + r * G, tid, 64 * NW);
+            for (int c = tid; c < tasks; c += NT) {
+                float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                if (r == 0 && c == tid) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = xv[e];
+                } else if (8 * c < K) {
+                    f8_load8<XT>(xrow + (int64_t)r * K * ES, c, v);
+                }
+                f8_put8<XT == TSA_F32>(v, c, xc + r * ld, xl + r * G);
+            }
         __syncthreads();
     }
-    const __amdgpu_buffer_rsrc_t rx = f8_buf(static_cast<const uint8_t*>(p.x) + t0 * K, XT >= 0 ? 0 : (int64_t)tn * K);
-    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int steps = (G + NW - 1) / NW;
+    v4f acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const int steps = (G + F8R_NW - 1) / F8R_NW;
     for (int j0 = 0; j0 < steps; j0 += F8R_D) {
         if (j0) load(j0);
 #pragma unroll
         for (int d = 0; d < F8R_D; ++d) {
-            const int b = wave + NW * (j0 + d);
+            const int b = wave + F8R_NW * (j0 + d);
             if (b >= G) break;
-            u32x4 Bv[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-            float s = sw[b];
-            if constexpr (XT >= 0) {
-                if (i < tn) {
-                    Bv[0] = *reinterpret_cast<const u32x4*>(xc + i * ld + F8B * b + 16 * q);
-                    Bv[1] = *reinterpret_cast<const u32x4*>(xc + i * ld + F8B * b + 64 + 16 * q);
-                    s *= xs[i * G + b];
-                }
-            } else {
-                const uint32_t o = (uint32_t)(F8B * b + 16 * q);
-                Bv[0] = f8_ld(rx, f8_off((uint32_t)(i * K), o, (uint32_t)K));
-                Bv[1] = f8_ld(rx, f8_off((uint32_t)(i * K), o + 64, (uint32_t)K));
-                if (i < tn) s *= p.xs[(t0 + i) * G + b];
-            }
-            const v4f part = f8_mfma<WIDE>(A[d], Bv);
+            const float s = sw[b];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r] = fmaf(s, part[r], acc[r]);
+            for (int m = 0; m < MT; ++m) {
+                if constexpr (XT >= 0) {
+                    Bv[d][0][0] = Bv[d][0][1] = u32x4{0, 0, 0, 0};
+                    sc[d][0] = 0.0f;
+                    if (i < tn) {
+                        Bv[d][0][0] = *reinterpret_cast<const u32x4*>(xc + i * ld + F8B * b + 16 * q);
+                        Bv[d][0][1] = *reinterpret_cast<const u32x4*>(xc + i * ld + F8B * b + 64 + 16 * q);
+                        sc[d][0] = xl[i * G + b];
+                    }
+                }
+                const v4f part = f8_mfma<WIDE>(A[d], Bv[d][m]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[m][r] = fmaf(s * sc[d][m], part[r], acc[m][r]);
+            }
         }
     }
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);  // [wave][token][row]
 #pragma unroll
-    for (int r = 0; r < 4; ++r) red[wave * 256 + i * 16 + 4 * q + r] = acc[r];
+    for (int m = 0; m < MT; ++m) *reinterpret_cast<v4f*>(red + ((wave * MT + m) * 16 + i) * 16 + 4 * q) = acc[m];
     __syncthreads();
-    if (tid < 256) {
-        const int64_t t = t0 + (tid >> 4), n = n0 + (tid & 15);
-        if (t < p.T && n < p.N) {
-            float v = 0.0f;
+    for (int o = tid; o < 256 * MT; o += NT) {
+        const int64_t t = t0 + (o >> 4), n = n0 + (o & 15);
+        if (t >= p.T || n >= p.N) continue;
+        float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) v += red[w * 256 + tid];
-            if (p.bias) v += load_act(p.bias, p.bias_dtype, n);
-            store_out(p.y, p.y_dtype, t * p.N + n, v);
-        }
+        for (int w = 0; w < F8R_NW; ++w) v += red[w * 256 * MT + o];
+        if (p.bias) v += load_act(p.bias, p.bias_dtype, n);
+        store_out(p.y, p.y_dtype, t * p.N + n, v);
     }
 }
 
-int f8r_lds(int xt, int G, int rows) {
-    const int red = 4 * 256 * 4, x = xt >= 0 ? rows * (G * F8B + 16 + G * 4) : 0;
+int f8r_lds(int xt, int mt, int G, int rows) {
+    const int red = F8R_NW * 256 * mt * 4, x = xt >= 0 ? rows * (G * F8B + 16 + G * 4) : 0;
     return x > red ? x : red;
 }
 
-template <int XT>
+template <int XT, int MT>
 hipError_t launch_rows(const F8Rows& p, hipStream_t st) {
-    const int lds = f8r_lds(XT, p.G, p.rows);
-    const void* fn = p.y_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_rows_kernel<XT, 4, true>)
-                                          : reinterpret_cast<const void*>(&fp8_rows_kernel<XT, 4, false>);
+    const int lds = f8r_lds(XT, MT, p.G, p.rows);
+    const void* fn = p.y_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_rows_kernel<XT, MT, true>)
+                                          : reinterpret_cast<const void*>(&fp8_rows_kernel<XT, MT, false>);
     const hipError_t e = ensure_dynamic_lds(fn, lds);
     if (e != hipSuccess) return e;
     F8Rows q = p;
     void* args[] = {&q};
-    return hipLaunchKernel(fn, dim3((unsigned)(p.tiles_n * ((p.T + 15) / 16))), dim3(256), args, lds, st);
+    return hipLaunchKernel(fn, dim3((unsigned)(p.tiles_n * ((p.T + 16 * MT - 1) / (16 * MT)))), dim3(64 * F8R_NW), args, lds, st);
+}
+
+hipError_t pick_rows(const F8Rows& p, hipStream_t st) {
+    return p.T <= 16 ? launch_rows<-1, 1>(p, st) : launch_rows<-1, 2>(p, st);
 }
 
 // ---------------------------------------------------------------- many tokens
@@ -176,8 +216,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_gemm_kernel(F8Gemm p) {
     // Workgroups are dealt round the 8 XCDs by linear id: renumbered so that each XCD takes a run, and
     // within it bands of 8 row tiles, token tile by token tile (about square pieces of the product at
     // a time share one L2: 3% at 4096 x 5760 against whole rows of token tiles).
-    const int total = (int)gridDim.x, lin = (int)blockIdx.x, xcd = lin & 7, q8 = total >> 3, rem = total & 7;
-    const int wid = xcd * q8 + (xcd < rem ? xcd : rem) + (lin >> 3);  // a bijection of [0, total)
+    const int total = (int)gridDim.x, wid = f8_run((int)blockIdx.x, total);
     constexpr int BAND = 8;
     const int rows = total / p.tiles_t, band = wid / (BAND * p.tiles_t), in = wid - band * BAND * p.tiles_t;
     const int deep = rows - BAND * band < BAND ? rows - BAND * band : BAND;  // row tiles of the band
@@ -341,7 +380,7 @@ extern "C" int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T,
     if (T == 0) return TSA_OK;
     TSA_REQUIRE(codes && scales && w && w_scales && y, TSA_ERR_INVALID_ARG, "null pointer");
     TSA_REQUIRE(aligned16(codes) && aligned16(w), TSA_ERR_INVALID_ARG, "the codes must be 16-byte aligned");
-    if (T > 16) {
+    if (T > 32) {
         F8Gemm p{};
         p.w = static_cast<const uint8_t*>(w);
         p.ws = w_scales;
@@ -359,12 +398,15 @@ extern "C" int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T,
         TSA_HIP_CHECK(y_dtype == TSA_F32 ? pick_gemm<true>(p, as_stream(stream)) : pick_gemm<false>(p, as_stream(stream)));
         return TSA_OK;
     }
-    TSA_HIP_CHECK(launch_rows<-1>(rows_params(codes, scales, T, K, w, w_scales, N, bias, bias_dtype, y, y_dtype),
-                                  as_stream(stream)));
+    TSA_HIP_CHECK(pick_rows(rows_params(codes, scales, T, K, w, w_scales, N, bias, bias_dtype, y, y_dtype), as_stream(stream)));
     return TSA_OK;
 }
 
-static int64_t linear_ws(int64_t T, int64_t K) { return (T * K + 255) / 256 * 256 + T * f8_blocks(K) * 4; }
+// Whether few enough tokens are quantised inside the product's launch.
+static bool linear_in_one(int64_t T, int64_t K) { return T <= 16 && f8r_lds(0, 1, (int)f8_blocks(K), (int)T) <= 128 * 1024; }
+static int64_t linear_ws(int64_t T, int64_t K) {
+    return linear_in_one(T, K) ? 0 : (T * K + 255) / 256 * 256 + T * f8_blocks(K) * 4;
+}
 
 extern "C" int tsa_fp8_linear_workspace_size(int64_t T, int64_t K, int64_t* bytes) {
     clear_error();
@@ -383,16 +425,17 @@ extern "C" int tsa_fp8_linear(const void* x, int x_dtype, int64_t T, int64_t K, 
     if (T == 0) return TSA_OK;
     TSA_REQUIRE(x && w && w_scales && y, TSA_ERR_INVALID_ARG, "null pointer");
     TSA_REQUIRE(aligned16(x) && aligned16(w), TSA_ERR_INVALID_ARG, "x and the weights must be 16-byte aligned");
+    hipStream_t st = as_stream(stream);
+    if (linear_in_one(T, K)) {
+        const F8Rows p = rows_params(x, nullptr, T, K, w, w_scales, N, bias, bias_dtype, y, y_dtype);
+        const hipError_t e = x_dtype == TSA_F32 ? launch_rows<TSA_F32, 1>(p, st)
+                             : x_dtype == TSA_F16 ? launch_rows<TSA_F16, 1>(p, st) : launch_rows<TSA_BF16, 1>(p, st);
+        TSA_HIP_CHECK(e);
+        return TSA_OK;
+    }
     TSA_REQUIRE(workspace && workspace_bytes >= linear_ws(T, K), TSA_ERR_WORKSPACE,
                 "workspace too small: got %lld bytes, need %lld", (long long)workspace_bytes, (long long)linear_ws(T, K));
     TSA_REQUIRE(aligned16(workspace), TSA_ERR_WORKSPACE, "the workspace must be 16-byte aligned");
-    hipStream_t st = as_stream(stream);
-    if (T <= 16 && f8r_lds(0, (int)f8_blocks(K), (int)T) <= 128 * 1024) {
-        const F8Rows p = rows_params(x, nullptr, T, K, w, w_scales, N, bias, bias_dtype, y, y_dtype);
-        TSA_HIP_CHECK(x_dtype == TSA_F32 ? launch_rows<TSA_F32>(p, st)
-                                         : x_dtype == TSA_F16 ? launch_rows<TSA_F16>(p, st) : launch_rows<TSA_BF16>(p, st));
-        return TSA_OK;
-    }
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     float* scales = reinterpret_cast<float*>(codes + (T * K + 255) / 256 * 256);
     rc = fp8_quantize(x, x_dtype, T, K, codes, scales, st);

@@ -43,14 +43,6 @@ __device__ __forceinline__ float f8_act(const tsa_expert_layout& L, float gate, 
     return silu_mul_fast(gate, up);
 }
 
-// A chunk of 8 values of a group (16 lanes a group) into its place in LDS.
-template <bool EXACT>
-__device__ __forceinline__ void f8_put8(const float (&v)[8], int c, uint8_t* codes, float* scales) {
-    const float s = f8_scale(f8_group_max(v));
-    *reinterpret_cast<uint2*>(codes + 8 * c) = f8_codes8<EXACT>(v, s);
-    if ((c & 15) == 0) scales[c >> 4] = s;
-}
-
 // One workgroup per (token, expert) pair and 8 channels: rows 0 .. 7 of the tile are the channels' gate
 // rows, 8 .. 15 their up rows, so one pair gives enough workgroups (768 at inter 768 and top-8, three
 // whole rounds of the CUs; tiles of 16 channels give 384, one and a half: 9.5 us against 7.0). Loads

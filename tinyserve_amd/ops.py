@@ -7,6 +7,7 @@ a CPU implementation.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -139,29 +140,49 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+def _call(t: torch.Tensor, fn, *args) -> None:
+    """fn(*args, stream) with t's device current, on that device's current stream."""
+    ctx = _lib.on_device(t)
+    if ctx is _lib._HERE:  # without the context: 1 us of a 7 us call
+        rc = fn(*args, _stream(t))
+    else:
+        with ctx:
+            rc = fn(*args, _stream(t))
+    if rc:
+        _lib.check(rc)
+
+
+def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    d = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
+            _lib.require_device(first, *others, what="tensor")
             raise RuntimeError(f"all tensors must be on one device (got {first.device} and {t.device})")
+    if d < 0:
+        _lib.require_device(first, what="tensor")
 
 
 def _fp8_weight(w: torch.Tensor, scales: torch.Tensor, K: int) -> tuple[torch.Tensor, torch.Tensor, int]:
     """(codes, float32 scales, N) of a weight matrix [N, K], checked."""
     if w.dtype not in _FP8_DTYPES or w.dim() != 2:
         raise RuntimeError(f"FP8 weights must be float8_e4m3fn (or its bytes) [N, K], got {w.dtype} {tuple(w.shape)}")
-    N = w.shape[0]
-    if w.shape[1] != K:
-        raise RuntimeError(f"in_features differ: activations {K}, weight {w.shape[1]}")
-    want = (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK))
-    if tuple(scales.shape) != want:
-        raise RuntimeError(f"weight scales must be {list(want)} for an [{N}, {K}] weight, got {list(scales.shape)}")
-    return _aligned(w), scales.to(torch.float32).contiguous(), N
+    N, Kw = w.shape
+    if Kw != K:
+        raise RuntimeError(f"in_features differ: activations {K}, weight {Kw}")
+    if scales.shape != (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK)):
+        raise RuntimeError(f"weight scales must be {[-(-N // FP8_BLOCK), -(-K // FP8_BLOCK)]} for an [{N}, {K}] weight, "
+                           f"got {list(scales.shape)}")
+    return _aligned(w), (scales if scales.dtype == torch.float32 else scales.float()).contiguous(), N
 
 
-def _fp8_bias(bias: torch.Tensor | None, N: int) -> torch.Tensor | None:
-    if bias is not None and bias.numel() != N:
+def _fp8_bias(bias: torch.Tensor | None, N: int) -> tuple[torch.Tensor | None, int | None, int]:
+    """(contiguous bias, its pointer, its tsa_dtype)."""
+    if bias is None:
+        return None, None, 0
+    if bias.numel() != N:
         raise RuntimeError(f"bias must have {N} elements, got {bias.numel()}")
-    return None if bias is None else bias.contiguous()
+    b = bias.contiguous()
+    return b, b.data_ptr(), _lib.tsa_dtype(b.dtype)
 
 
 def fp8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -171,10 +192,9 @@ def fp8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dt = _lib.tsa_dtype(x.dtype)
     x2 = _rows(x, x.shape[-1])
     T, K = x2.shape
-    codes = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((T, -(-K // FP8_BLOCK)), dtype=torch.float32, device=x.device)
-    with _lib.on_device(x2):
-        _lib.check(_lib.load().tsa_fp8_quantize(x2.data_ptr(), dt, T, K, codes.data_ptr(), scales.data_ptr(), _stream(x2)))
+    codes = x2.new_empty((T, K), dtype=torch.float8_e4m3fn)
+    scales = x2.new_empty((T, -(-K // FP8_BLOCK)), dtype=torch.float32)
+    _call(x2, _lib.load().tsa_fp8_quantize, x2.data_ptr(), dt, T, K, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -183,38 +203,42 @@ def fp8_matmul(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_sca
     """y [T, N] = deq(codes) @ deq(w)^T (+ bias): codes [T, K] and scales [T, ceil(K / 128)] as
     fp8_quantize returns them, w [N, K] with scales [ceil(N / 128), ceil(K / 128)]; float32 sums. K
     must be a multiple of 16. Projections that share their input share one fp8_quantize."""
-    _lib.require_device(codes, scales, w, w_scales, *([bias] if bias is not None else []), what="tensor")
-    _same_device(codes, scales, w, w_scales, bias)
+    _one_device(codes, scales, w, w_scales, bias)
     if codes.dtype not in _FP8_DTYPES or codes.dim() != 2:
         raise RuntimeError(f"FP8 activations must be float8_e4m3fn (or its bytes) [T, K], got {codes.dtype} {tuple(codes.shape)}")
     T, K = codes.shape
-    if tuple(scales.shape) != (T, -(-K // FP8_BLOCK)) or scales.dtype != torch.float32:
+    if scales.shape != (T, -(-K // FP8_BLOCK)) or scales.dtype != torch.float32:
         raise RuntimeError(f"activation scales must be float32 [{T}, {-(-K // FP8_BLOCK)}], got {scales.dtype} {list(scales.shape)}")
-    c, sc, (w, ws, N), b = _aligned(codes), scales.contiguous(), _fp8_weight(w, w_scales, K), _fp8_bias(bias, w.shape[0])
-    y = torch.empty((T, N), dtype=out_dtype, device=codes.device)
-    with _lib.on_device(c):
-        _lib.check(_lib.load().tsa_fp8_matmul(c.data_ptr(), sc.data_ptr(), T, K, w.data_ptr(), ws.data_ptr(), N, _lib.ptr(b),
-                                              _lib.tsa_dtype(b.dtype) if b is not None else 0, y.data_ptr(),
-                                              _lib.tsa_dtype(out_dtype), _stream(c)))
+    c, sc, (w, ws, N) = _aligned(codes), scales.contiguous(), _fp8_weight(w, w_scales, K)
+    b, bp, bt = _fp8_bias(bias, N)
+    y = c.new_empty((T, N), dtype=out_dtype)
+    _call(c, _lib.load().tsa_fp8_matmul, c.data_ptr(), sc.data_ptr(), T, K, w.data_ptr(), ws.data_ptr(), N, bp, bt,
+          y.data_ptr(), _lib.tsa_dtype(out_dtype))
     return y
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp8_linear_workspace_size(T: int, K: int) -> int:
+    n = ctypes.c_int64()
+    _lib.check(_lib.load().tsa_fp8_linear_workspace_size(T, K, ctypes.byref(n)))
+    return n.value
 
 
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y [T, N] = deq(fp8_quantize(x)) @ deq(w)^T (+ bias) for x [..., K] in bf16, fp16 or fp32; y in
     x's dtype unless ``out_dtype`` says otherwise. K must be a multiple of 16."""
-    _lib.require_device(x, w, w_scales, *([bias] if bias is not None else []), what="tensor")
-    _same_device(x, w, w_scales, bias)
+    _one_device(x, w, w_scales, bias)
     dt, K = _lib.tsa_dtype(x.dtype), x.shape[-1]
     w, ws, N = _fp8_weight(w, w_scales, K)
-    x2, b = _aligned(_rows(x, K)), _fp8_bias(bias, N)
+    x2 = _aligned(_rows(x, K))
+    b, bp, bt = _fp8_bias(bias, N)
     T = x2.shape[0]
-    y = torch.empty((T, N), dtype=out_dtype or x.dtype, device=x.device)
-    scratch = torch.empty(T * K + 4 * T * ws.shape[1] + 256, dtype=torch.uint8, device=x.device)
-    with _lib.on_device(x2):
-        _lib.check(_lib.load().tsa_fp8_linear(x2.data_ptr(), dt, T, K, w.data_ptr(), ws.data_ptr(), N, _lib.ptr(b),
-                                              _lib.tsa_dtype(b.dtype) if b is not None else 0, y.data_ptr(),
-                                              _lib.tsa_dtype(y.dtype), scratch.data_ptr(), scratch.numel(), _stream(x2)))
+    y = x2.new_empty((T, N), dtype=out_dtype)
+    n = _fp8_linear_workspace_size(T, K)
+    scratch = x2.new_empty(n, dtype=torch.uint8) if n else None
+    _call(x2, _lib.load().tsa_fp8_linear, x2.data_ptr(), dt, T, K, w.data_ptr(), ws.data_ptr(), N, bp, bt, y.data_ptr(),
+          dt if out_dtype is None else _lib.tsa_dtype(out_dtype), _lib.ptr(scratch), n)
     return y
 
 
