@@ -395,3 +395,118 @@ def test_chain_other_stream():
         got = chain()
     st.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ----------------------------------------------------------------------------- refusals, modules, the pipeline
+def test_refusals():
+    x, (w, ws) = acts(1, 4, 256), weights(2, 160, 256)
+    c, s = ops.fp8_quantize(x)
+    for f, text in ((lambda: ops.fp8_linear(x, w, ws[:1]), "weight scales must be"),
+                    (lambda: ops.fp8_linear(x[:, :128], w, ws), "in_features differ"),
+                    (lambda: ops.fp8_linear(x, w.float(), ws), "must be float8_e4m3fn"),
+                    (lambda: ops.fp8_linear(x, w, ws, torch.zeros(3, device=DEV)), "bias must have"),
+                    (lambda: ops.fp8_linear(x, w.cpu(), ws), "must be on CUDA"),
+                    (lambda: ops.fp8_linear(x[:, :136], w[:, :136], ws), "multiple of 16"),
+                    (lambda: ops.fp8_matmul(c, s[:, :1], w, ws), "activation scales must be"),
+                    (lambda: ops.fp8_matmul(x, s, w, ws), "activations must be float8_e4m3fn"),
+                    (lambda: ops.fp8_matmul(c, s, w, ws.cpu()), "must be on CUDA")):
+        with pytest.raises(RuntimeError, match=text):
+            f()
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        ops.fp8_quantize(x.double())
+
+
+@pytest.mark.parametrize("T", [2, 9])
+def test_moe_long_rows(T):
+    """The longest rows: hidden past what a workgroup holds of x at once, inter past what it stages of h."""
+    for E, k, H, I in ((5, 5, 64, 16384), (3, 2, 16384, 64)):
+        ex = experts(1, E, H, I)
+        L, pool = pool_of(ex, H, I)
+        x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+        want, err = ref.moe(x, idx, w, ex)
+        ref.check(ops.moe_decode(L, pool, idx, w, x), want, err)
+
+
+def test_moe_routed_without_workspace_and_many_experts():
+    """The allocation-free call, and more experts than the in-kernel routing takes."""
+    from tinyserve_amd import _lib
+    import ctypes
+
+    for E, k, T in ((7, 3, 2), (300, 4, 3)):
+        H, I = 128, 64
+        ex = experts(1, 7, H, I)
+        L, pool = pool_of(ex, H, I)
+        slot = (torch.arange(E, device=DEV) % 7).to(torch.int32)
+        x, (lg, idx, w) = acts(T, T, H), routes(T, T, E, k)
+        want, err = ref.moe(x, slot[idx.long()], w, ex)
+        err = err + want.abs() * 2.0**-20 * k + err * 2.0**-18
+        ref.check(ops.moe_decode_routed(L, pool, slot, lg, x, k), want, err)
+        y = torch.empty((T, H), dtype=BF, device=DEV)
+        _lib.check(_lib.load().tsa_moe_decode_routed_noalloc(
+            ctypes.byref(L), pool.data_ptr(), 7, slot.data_ptr(), E, lg.data_ptr(), 0, 0, T, k, x.data_ptr(), 2, y.data_ptr(), 2,
+            None, None, torch.cuda.current_stream().cuda_stream))
+        ref.check(y, want, err)
+
+
+def test_modules_and_builders():
+    """FP8Linear, the template expert and the inline forward give the operators' results."""
+    from tinyserve_amd.expert_forward import (FP8ExpertModule, _build_cpp_layout_args, _build_fp8_inline_forward,
+                                              _precompute_param_refs, fast_expert_forward, forward_from_packed)
+    from tinyserve_amd.fp8 import FP8Linear
+
+    w, ws = weights(1, 96, 144)
+    b = torch.randn(96, device=DEV).to(BF)
+    x = acts(2, 2, 3, 144)
+    y = FP8Linear(w, ws, b)(x)
+    assert y.shape == (2, 3, 96) and torch.equal(y.view(6, 96), ops.fp8_linear(x.view(6, 144), w, ws, b))
+    H, I = 256, 160
+    ex = experts(3, 1, H, I)
+    L, pool = pool_of(ex, H, I)
+    lay = synth.fp8_layout(H, I)
+    mod = FP8ExpertModule(lay, device=DEV)
+    for T in (1, 5, 40):
+        h = acts(T, T, H)
+        zero, one = torch.zeros((T, 1), dtype=torch.int32, device=DEV), torch.ones((T, 1), device=DEV)
+        want, err = ref.moe(h, zero, one, ex)
+        ref.check(forward_from_packed(mod, pool[0], _precompute_param_refs(mod, lay), h), want, err)
+        ref.check(_build_fp8_inline_forward(lay, None)(pool[0], h), want, err)
+        ref.check(fast_expert_forward(h, zero, one, pool, **_build_cpp_layout_args(lay, None)), want, err)
+
+
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_pipeline_and_hook(tmp_path, T):
+    """A checkpoint on disk through the store, the pipeline and an installed MoE block."""
+    import numpy as np
+    import torch.nn as nn
+
+    from tests.test_fp8_host import _save
+    from tinyserve_amd.expert_batcher import BatchItem, ExpertBatcher
+    from tinyserve_amd.expert_pipeline import ExpertPipeline, install_offloaded_forward
+    from tinyserve_amd.expert_store import ExpertStore
+
+    E, k, H, I = 6, 2, 160, 96
+    disk = _save(tmp_path, np.random.default_rng(5), (0, 1), E, H, I)
+    store, _ = ExpertStore.from_safetensors(str(tmp_path))
+    pipe = ExpertPipeline(store, None, DEV)
+    for layer in (0, 1):
+        ex = [{n: t.to(DEV) for n, t in disk[layer, e].items()} for e in range(E)]
+        x, (lg, idx, w) = acts(T, T, H), routes(T + layer, T, E, k)
+        want, err = ref.moe(x, idx, w, ex)
+        ref.check(pipe.execute_layer_experts(x, layer, idx, w), want, err)
+        ref.check(pipe.execute_layer_experts_batched(x, layer, idx, w), want, err)
+        ref.check(pipe.execute_layer_logits(x, layer, lg, k), want, err + want.abs() * 2.0**-20 * k + err * 2.0**-18)
+        got = ExpertBatcher(pipe).batch_execute([BatchItem(x[t : t + 1], idx[t], w[t], t) for t in range(T)], layer)
+        ref.check(torch.cat(got), want, err)
+
+        class Block(nn.Module):
+            def __init__(self):
+                super().__init__()
+                self.gate = nn.Linear(H, E, bias=False).to(DEV, BF)
+
+        block = Block()
+        install_offloaded_forward(block, pipe, layer, "gate", k)
+        y = block.forward(x.view(1, T, H))
+        idx2, w2 = ops.route_topk(ops.router_logits(x, block.gate.weight), k)
+        w2 = w2 if T <= 4 else w2.to(BF).float()
+        want, err = ref.moe(x, idx2, w2, ex)
+        ref.check(y.view(T, H), want, err + want.abs() * 2.0**-20 * k + err * 2.0**-18)

@@ -287,6 +287,26 @@ class GGUFExpertModule(nn.Module):
         return ops.gguf_matvec(act, self.down.reshape(-1), self._types["down"], H, I)
 
 
+class FP8ExpertModule(nn.Module):
+    """An FP8 expert whose parameters are the slot's tensors (the names and shapes of an FP8 slot:
+    ``gate_proj``, ``up_proj``, ``down_proj`` and their ``_scale_inv``), for forward_from_packed /
+    swap_weights_and_forward; the forward is the fused kernels' layer in three FP8 linears: gate and up in
+    float32, silu(gate) * up quantised again for down."""
+
+    def __init__(self, layout: TensorLayout, device=None):
+        super().__init__()
+        if not is_fp8_layout(layout):
+            raise ValueError(f"not an FP8 expert slot: {sorted(layout.specs)}")
+        for name, (shape, dtype) in layout.specs.items():
+            self.register_parameter(name, nn.Parameter(torch.zeros(shape, dtype=dtype, device=device),
+                                                       requires_grad=False))
+
+    def forward(self, h: torch.Tensor) -> torch.Tensor:
+        g = ops.fp8_linear(h, self.gate_proj, self.gate_proj_scale_inv, out_dtype=torch.float32)
+        u = ops.fp8_linear(h, self.up_proj, self.up_proj_scale_inv, out_dtype=torch.float32)
+        return ops.fp8_linear(F.silu(g) * u, self.down_proj, self.down_proj_scale_inv, out_dtype=h.dtype)
+
+
 # ----------------------------------------------------------------------------- inline builders
 def _build_inline_forward(layout: TensorLayout, act_fn):
     """``(packed, h) -> y`` for an unquantised fused-expert slot (``gate_up_proj`` and
@@ -341,8 +361,10 @@ def _build_gpu_int4_forward(layout, act_fn):
 
 def _build_cpp_layout_args(layout: TensorLayout, act_fn):
     """Keyword arguments of fast_expert_forward for slots of this layout: the kernel layout
-    of an MXFP4 slot; None where the TensorLayout alone fixes no kernel layout (GGUF slots
+    of an MXFP4 or FP8 slot; None where the TensorLayout alone fixes no kernel layout (GGUF slots
     need their ggml types, see gguf_expert_layout; unquantised slots have no kernel)."""
+    if is_fp8_layout(layout):
+        return {"layout": fp8_expert_layout(layout, act_fn)}
     if "gate_up_proj_scales" not in layout.specs:
         return None
     return {"layout": mxfp4_expert_layout(layout, act_fn)}
@@ -352,7 +374,15 @@ def _build_mxfp4_inline_forward(layout: TensorLayout, act_fn):
     """``(packed [expert_bytes] u8, h [T, H]) -> [T, H]`` for an MXFP4 slot; None otherwise."""
     if "gate_up_proj_scales" not in layout.specs:
         return None
-    L = mxfp4_expert_layout(layout, act_fn)
+    return _layout_forward(mxfp4_expert_layout(layout, act_fn))
+
+
+def _build_fp8_inline_forward(layout: TensorLayout, act_fn):
+    """The same for an FP8 slot."""
+    return _layout_forward(fp8_expert_layout(layout, act_fn)) if is_fp8_layout(layout) else None
+
+
+def _layout_forward(L: _lib.ExpertLayout):
     one = {}
 
     def _forward(packed: torch.Tensor, h: torch.Tensor) -> torch.Tensor:

@@ -32,7 +32,7 @@ import torch.nn as nn
 
 from . import ops
 from .expert_cache import ExpertCache
-from .expert_forward import (_build_cpp_layout_args, _build_gpu_int4_forward, _build_inline_forward,
+from .expert_forward import (_build_cpp_layout_args, _build_fp8_inline_forward, _build_gpu_int4_forward, _build_inline_forward,
                              _build_mxfp4_inline_forward, _precompute_param_refs, mxfp4_expert_layout)
 
 
@@ -80,6 +80,7 @@ class ExpertPipeline:
             self._param_refs = _precompute_param_refs(template, store.layout) if template is not None else None
             self._inline_fwd = (_build_inline_forward(store.layout, self._act_fn)
                                 or _build_mxfp4_inline_forward(self.cache_layout, self._act_fn)
+                                or _build_fp8_inline_forward(self.cache_layout, self._act_fn)
                                 or _build_gpu_int4_forward(store.layout, self._act_fn))
             self._cpp_layout_args = _build_cpp_layout_args(self.cache_layout, self._act_fn)
         self._kernel_layouts: dict[int, object] = {}

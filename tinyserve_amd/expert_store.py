@@ -69,6 +69,25 @@ def mxfp4_tiled_specs(specs: dict) -> dict:
     return out
 
 
+def _stack_fp8(tensors: dict[str, torch.Tensor], layer: int) -> dict[str, torch.Tensor]:
+    """A layer's FP8 experts, ``<e>.<matrix>.weight`` and ``.weight_scale_inv``, as one tensor per name
+    with the experts first, in slot order (the matrices, then their scales as float32)."""
+    n = 1 + max((int(k.split(".")[0]) for k in tensors if k.split(".")[0].isdigit()), default=-1)
+    out: dict[str, torch.Tensor] = {}
+    for suffix, part in (("weight", ""), ("weight_scale_inv", "_scale_inv")):
+        for mat in ("gate_proj", "up_proj", "down_proj"):
+            keys = [f"{e}.{mat}.{suffix}" for e in range(n)]
+            missing = [k for k in keys if k not in tensors]
+            if missing:
+                raise ValueError(f"layer {layer}: FP8 expert tensors missing: {missing[:4]}")
+            out[mat + part] = torch.stack([tensors.pop(k).float() if part else tensors.pop(k) for k in keys])
+            if not part and out[mat].dtype != torch.float8_e4m3fn:
+                raise ValueError(f"layer {layer}: {mat} is {out[mat].dtype}, not float8_e4m3fn")
+    if tensors:
+        raise ValueError(f"layer {layer}: unexpected expert tensors {sorted(tensors)[:4]}")
+    return out
+
+
 class ExpertBuffer:
     """One expert's packed bytes on a device (tinyserve/expert_store.py:84-112)."""
 
@@ -85,7 +104,7 @@ class ExpertBuffer:
 class ExpertStore:
     """Every MoE layer's experts as packed slots in host memory, ``_data`` [layers, experts,
     expert_bytes] (tinyserve/expert_store.py:115-130: same attributes; the reference's
-    INT4 cache, FP8 and disk-offload options are out of scope here)."""
+    INT4 cache, FP8 storage of wider weights and disk-offload options are out of scope here)."""
 
     def __init__(self, data: torch.Tensor, layout: TensorLayout, num_layers: int, num_experts: int,
                  layer_indices: list[int] | None = None, tiled: bool = False):
@@ -109,7 +128,9 @@ class ExpertStore:
         / ``gate_up_proj_bias`` / ``down_proj`` ...), and the slot keeps the checkpoint's key
         order. ``tiled``: MXFP4 matrices are stored in the 16-row MFMA tile order of the fast
         decode instead (mx_tiles.tile_mxfp4; their scale tensors become the tile-scale areas).
-        Returns (store, num_experts)."""
+        FP8 checkpoints keep one tensor per expert: ``<e>.gate_proj.weight`` / ``up_proj`` / ``down_proj``
+        (e4m3) and their ``weight_scale_inv``; the slot is synth.fp8_layout's. Returns (store,
+        num_experts)."""
         import json
         import os
         import re
@@ -138,12 +159,17 @@ class ExpertStore:
         layers = sorted(layer_tensors) if layer_indices is None else [li for li in layer_indices if li in layer_tensors]
         if not layers:
             raise ValueError(f"No expert tensors found in {model_dir} (pattern *.layers.<i>.{prefix}*)")
+        fp8 = any(re.fullmatch(r"\d+\.\w+\.weight_scale_inv", n) for n in layer_tensors[layers[0]])
+        if fp8:
+            if tiled:
+                raise ValueError("tiled slots need MXFP4 experts; this checkpoint holds FP8 ones")
+            layer_tensors = {li: _stack_fp8(layer_tensors[li], li) for li in layers}
         first = layer_tensors[layers[0]]
         num_experts = int(next(iter(first.values())).shape[0])
         specs = {n: (tuple(t.shape[1:]), t.dtype) for n, t in first.items()}
         if tiled:
             specs = mxfp4_tiled_specs(specs)
-        layout = TensorLayout(specs)
+        layout = TensorLayout(specs, align=16 if fp8 else 1)
         data = torch.empty((len(layers), num_experts, layout.total_bytes), dtype=torch.uint8,
                            pin_memory=torch.cuda.is_available())
         host = data.numpy()
@@ -185,7 +211,9 @@ class ExpertStore:
         return self._data[layer_idx].to(device)
 
     def expert_layout(self, act_fn=None):
-        """The kernels' tsa_expert_layout of these slots (MXFP4 checkpoints)."""
-        from .expert_forward import mxfp4_expert_layout
+        """The kernels' tsa_expert_layout of these slots (MXFP4 and FP8 checkpoints)."""
+        from .expert_forward import fp8_expert_layout, is_fp8_layout, mxfp4_expert_layout
 
+        if is_fp8_layout(self.layout):
+            return fp8_expert_layout(self.layout, act_fn, self.expert_bytes)
         return mxfp4_expert_layout(self.layout, act_fn, self.expert_bytes, tiled=self.tiled)
