@@ -33,6 +33,7 @@ def lib():
     (-1, 128, 64, _lib.ERR_SHAPE, b"bad shape"),
     (4, (1 << 20) + 16, 64, _lib.ERR_SHAPE, b"multiple of 16"),
     (1 << 31, 128, 64, _lib.ERR_SHAPE, b"too large"),
+    (1, 128, (1 << 30) + 1, _lib.ERR_SHAPE, b"too large"),
 ])
 def test_matmul_refusals(lib, T, K, N, rc, text):
     assert lib.tsa_fp8_matmul(P, P, T, K, P, P, N, None, 0, P, 2, None) == rc and text in lib.tsa_last_error()

@@ -510,3 +510,68 @@ def test_pipeline_and_hook(tmp_path, T):
         w2 = w2 if T <= 4 else w2.to(BF).float()
         want, err = ref.moe(x, idx2, w2, ex)
         ref.check(y.view(T, H), want, err + want.abs() * 2.0**-20 * k + err * 2.0**-18)
+
+
+def test_moe_prompt_in_pieces():
+    """More assignments than the grouped kernels take at a time."""
+    E, k, H, I, T = 5, 2, 64, 32, 70000
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, ex)
+    ref.check(ops.moe_prefill(L, pool, torch.arange(E, dtype=torch.int32, device=DEV), idx, w, x), want, err)
+
+
+def test_moe_nothing_resident():
+    E, k, H, I, T = 4, 2, 96, 64, 9
+    L, pool = pool_of(experts(1, E, H, I), H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    slot = torch.full((E,), -1, dtype=torch.int32, device=DEV)
+    for n in (1, T):
+        assert not ops.moe_prefill(L, pool, slot, idx[:n], w[:n], x[:n]).any()
+        assert not ops.moe_decode(L, pool, slot[idx[:n].long()], w[:n], x[:n]).any()
+
+
+def test_linear_longest_rows():
+    """K past what one launch stages, more than 64 blocks."""
+    K, N = 131072, 48
+    w, ws = weights(1, N, K)
+    for T in (2, 40):
+        x = acts(T, T, K)
+        ref.check(ops.fp8_linear(x, w, ws), *ref.matmul(*ref.quantize(x.double()), w, ws))
+
+
+def test_prompt_captured():
+    """A quantisation, products and a layer of a prompt in one graph, replayed with other inputs; two
+    graphs' results do not disturb each other."""
+    E, k, H, I, T = 8, 2, 256, 160, 40
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    wq, wo = weights(3, 320, H), weights(4, H, 320)
+    xs = [acts(i, T, H) for i in range(2)]
+    lg = [torch.randn((T, E), device=DEV, generator=gen(i)) for i in range(2)]
+
+    def step(i):
+        c, s = ops.fp8_quantize(xs[i])
+        h = ops.fp8_linear(ops.fp8_matmul(c, s, *wq), *wo)
+        idx, w = ops.route_topk(lg[i], k)
+        return ops.moe_prefill(L, pool, slot, idx, w, h)
+
+    step(0)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+    for r in range(4):
+        for i in range(2):
+            xs[i].copy_(acts(50 + 2 * r + i, T, H))
+            lg[i].copy_(torch.randn((T, E), device=DEV, generator=gen(70 + 2 * r + i)))
+        for g in graphs:
+            g.replay()
+        want = [step(i) for i in range(2)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))

@@ -315,7 +315,7 @@ int check_matmul(int64_t T, int64_t K, int64_t N, const void* bias, int bias_dty
                 (long long)K);
     TSA_REQUIRE(K % 16 == 0 && K <= F8_MAX_K, TSA_ERR_SHAPE, "K (%lld) must be a multiple of 16 of at most %lld", (long long)K,
                 (long long)F8_MAX_K);
-    TSA_REQUIRE(T < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && (T + 15) / 16 * ((N + 15) / 16) < ((int64_t)1 << 31),
+    TSA_REQUIRE(T <= ((int64_t)1 << 30) && N <= ((int64_t)1 << 30) && (T + 15) / 16 * ((N + 15) / 16) < ((int64_t)1 << 31),
                 TSA_ERR_SHAPE, "T %lld x N %lld is too large", (long long)T, (long long)N);
     TSA_REQUIRE(valid_dtype(y_dtype), TSA_ERR_INVALID_ARG, "bad dtype (y %d)", y_dtype);
     TSA_REQUIRE(!bias || valid_dtype(bias_dtype), TSA_ERR_INVALID_ARG, "bad dtype (bias %d)", bias_dtype);
@@ -410,7 +410,7 @@ static int64_t linear_ws(int64_t T, int64_t K) {
 
 extern "C" int tsa_fp8_linear_workspace_size(int64_t T, int64_t K, int64_t* bytes) {
     clear_error();
-    TSA_REQUIRE(T >= 0 && K >= 1 && T < ((int64_t)1 << 31) && K <= F8_MAX_K && bytes, TSA_ERR_INVALID_ARG, "bad T/K/bytes");
+    TSA_REQUIRE(T >= 0 && K >= 1 && T <= ((int64_t)1 << 30) && K <= F8_MAX_K && bytes, TSA_ERR_INVALID_ARG, "bad T/K/bytes");
     *bytes = linear_ws(T, K);
     return TSA_OK;
 }
