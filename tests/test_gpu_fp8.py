@@ -575,3 +575,10 @@ def test_prompt_captured():
         want = [step(i) for i in range(2)]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("T,N,K", [(33, 1, 16), (40, 3, 32), (65, 2, 144)])
+def test_matmul_smallest_buffers(T, N, K):
+    """Weights of fewer bytes than the pipeline's blocks ahead of the last."""
+    x, (w, ws) = acts(T, T, K), weights(N, N, K)
+    ref.check(ops.fp8_linear(x, w, ws), *ref.matmul(*ref.quantize(x.double()), w, ws))

@@ -102,22 +102,24 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
         so = r < 0 ? 0x80000000u : (uint32_t)r * (uint32_t)p.G * 4u;
     }
     // copy j (of PER) of block s: the weights', the tokens', the scales'. Columns past K and blocks past
-    // the last read zeros, so every step issues as many.
+    // the last read zeros, so every step issues as many. (The scalar offset stays inside the buffers:
+    // the range check may subtract it from their size.)
     uint32_t at[2];  // this lane's column in copies of even and odd number
 #pragma unroll
     for (int n = 0; n < 2; ++n) at[n] = 16u * chunk(n);
     auto issue = [&](int j, int s, int stage) {
         const uint32_t col = (uint32_t)F8B * (uint32_t)s, base = lds0 + (uint32_t)stage * C::STAGE;
+        const uint32_t soff = s < steps ? col : 0u;
         if (j < C::NXW) {
             const int n = C::NXW * wave + j;
             const bool in = col + (n & 1 ? at[1] : at[0]) < K;
-            f8_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], in ? wo[j] : 0x80000000u, col, base + 1024u * (uint32_t)n);
+            f8_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], in ? wo[j] : 0x80000000u, soff, base + 1024u * (uint32_t)n);
         } else if (j < C::NXW + C::NXT) {
             const int n = C::NXT * wave + j - C::NXW;
             const bool in = col + (n & 1 ? at[1] : at[0]) < K;
-            f8_copy16(rx, in ? xo[j - C::NXW] : 0x80000000u, col, base + (uint32_t)C::RN * F8B + 1024u * (uint32_t)n);
+            f8_copy16(rx, in ? xo[j - C::NXW] : 0x80000000u, soff, base + (uint32_t)C::RN * F8B + 1024u * (uint32_t)n);
         } else {
-            f8_copy4(rs, s < steps ? so : 0x80000000u, 4u * (uint32_t)s,
+            f8_copy4(rs, s < steps ? so : 0x80000000u, soff / 32,
                      lds0 + (uint32_t)(S * C::STAGE) + 256u * (uint32_t)(C::NW * stage + wave));
         }
     };
