@@ -582,3 +582,16 @@ def test_matmul_smallest_buffers(T, N, K):
     """Weights of fewer bytes than the pipeline's blocks ahead of the last."""
     x, (w, ws) = acts(T, T, K), weights(N, N, K)
     ref.check(ops.fp8_linear(x, w, ws), *ref.matmul(*ref.quantize(x.double()), w, ws))
+
+
+@pytest.mark.parametrize("T", [2, 12])
+def test_moe_dead_expert_any_weight(T):
+    """The weight of an expert that is not resident is not used: NaN there changes nothing."""
+    E, k, H, I = 4, 3, 128, 96
+    L, pool = pool_of(experts(1, E, H, I), H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    slot = torch.tensor([0, -1, 2, 3], dtype=torch.int32, device=DEV)
+    bad = torch.where(idx == 1, float("nan"), w)
+    for f in (lambda v: ops.moe_decode(L, pool, slot[idx.long()], v, x), lambda v: ops.moe_prefill(L, pool, slot, idx, v, x)):
+        y = f(bad)
+        assert torch.isfinite(y).all() and torch.equal(y, f(w))
