@@ -9,8 +9,8 @@ and 7 small ones, the small ones are dropped below 2^-13 of it). Each of up to 7
 loses a part spread over at most 2^-13 of the largest, 2^-13 / sqrt(3) rms, sqrt(7 / 3) 2^-13 together;
 the eights' parts are independent, and six times their rms bounds them.
 
-Codes. A code's own rounding is part of the definition. h of an expert is computed, so a code of h may
-fall to the other side where h / s lies within h's error of the border between two codes, and then it
+Codes. A code's own rounding is part of the definition. h of an expert is computed (gate and up as float32
+sums, since a step of a code is far more than what they would lose otherwise), so a code of h may fall to the other side where h / s lies within h's error of the border between two codes, and then it
 is off by one step.
 """
 from __future__ import annotations
@@ -85,8 +85,8 @@ def check(got: torch.Tensor, want: torch.Tensor, err: torch.Tensor, what: str = 
 
 def expert(q: torch.Tensor, s: torch.Tensor, e: dict, act: str = "silu"):
     """(y, bound) of one expert (tensors of synth.fp8_layout) for quantised tokens."""
-    g, ge = matmul(q, s, e["gate_proj"], e["gate_proj_scale_inv"])
-    u, ue = matmul(q, s, e["up_proj"], e["up_proj_scale_inv"])
+    g, ge = matmul(q, s, e["gate_proj"], e["gate_proj_scale_inv"], wide=True)
+    u, ue = matmul(q, s, e["up_proj"], e["up_proj_scale_inv"], wide=True)
     if act == "silu":
         sg, slope = g * torch.sigmoid(g), 1.1  # |silu'| < 1.1
     else:

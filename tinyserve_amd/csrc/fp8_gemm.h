@@ -5,9 +5,9 @@
 // into one of S stages in LDS by buffer-to-LDS copies, S - 1 blocks ahead; rows and columns past the
 // matrices are offsets past the buffers, which copy zeros. The 16-byte chunk c of row r sits in slot c ^
 // (r / 2 % 8): the 16 rows that a quarter wave reads at once then fall on distinct banks. One MFMA
-// (v_mfma_f32_16x16x128_f8f6f4) makes a tile's sum over the block, which joins the float32 result
-// times the token's and the weight block's scale: 4 fused multiply-adds beside 32 cycles of the matrix
-// core. The tokens' scales of a block travel with it.
+// (v_mfma_f32_16x16x128_f8f6f4; WIDE: four bf16 ones) makes a tile's sum over the block, which joins the
+// float32 result times the token's and the weight block's scale: 4 fused multiply-adds beside 32 cycles
+// of the matrix core. The tokens' scales of a block travel with it.
 #pragma once
 
 #include "fp8_common.h"

@@ -5,9 +5,15 @@
 //
 // Few tokens: two launches ordered by the stream. gate_up: one workgroup per (token, expert) pair
 // and 8 channels; down: one per token and 8 outputs, over all the token's experts, so every
-// output has one writer. Each is a stream of weights into the A operands of
-// v_mfma_f32_16x16x128_f8f6f4 (one or two columns of B in use: the matrix cores are idle otherwise, and
-// the codes need no conversion).
+// output has one writer. Each is a stream of weights into the A operands of matrix
+// instructions (one or two columns of B in use: the matrix cores are idle otherwise).
+//
+// Gate and up are summed to float32 accuracy (f8_mfma's WIDE), here and for many tokens: their result is
+// quantised again, and a sum off by 1e-5 takes some 3 codes in 10000 to another side, off by 6% each.
+// A layer's bf16 result is then off by its own rounding (0.0017 rms over 12 to 785 tokens), with the FP8
+// instructions by 0.0018 to 0.0032. us, float32 accuracy / FP8 instructions: hidden 2880, 32 experts top-4,
+// 8 layers of 4 tokens 632 / 613, a layer of 2048 570 / 490; hidden 2048, 128 experts top-8, 24 tokens 58 / 57,
+// 1024 tokens 210 / 187.
 #include "fp8_gemm.h"
 #include "moe_group.h"
 
@@ -140,7 +146,7 @@ __global__ void __launch_bounds__(64 * F8A_NW) fp8_gate_up_kernel(F8Moe p) {
                 Bv[1] = *reinterpret_cast<const u32x4*>(xc + F8B * b + 64 + 16 * q);
             }
             const float s = ws[d] * xs[b];
-            const v4f part = f8_mfma(A[d], Bv);
+            const v4f part = f8_mfma<true>(A[d], Bv);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = fmaf(s, part[e], acc[e]);
         }
@@ -261,8 +267,8 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // quantised (the others); (2) gate_up over the tiles: 128 channels of gate and of up per workgroup, so
 // the epilogue holds whole groups of h and quantises them; (3) down, each assignment's output in
 // float32 at the assignment's place; (4) the weighted sums. (Outputs rounded to bf16 between (3) and (4)
-// save 12 us of 189 at 1024 tokens, 128 experts top-8, and take the result's error against 64 bits from
-// 0.0018 to 0.0026.)
+// save 12 us at 1024 tokens, 128 experts top-8, and add an error of 0.0019 to the result, more than its own
+// rounding's.)
 struct F8Group {
     tsa_expert_layout L;
     const uint8_t* pool;
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p
     o.K = H;
     o.G = GH;
     v4f acc[C::MR][C::MT];
-    f8_tile<C, 2, false>(o, smem, tn, [&](int r) { return r < tn ? p.perm[row0 + r] / p.k : -1; }, acc);
+    f8_tile<C, 2, true>(o, smem, tn, [&](int r) { return r < tn ? p.perm[row0 + r] / p.k : -1; }, acc);
 
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
     const int wr = wave % C::WR, wt = wave / C::WR;
@@ -579,7 +585,7 @@ int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, 
 }
 
 // Calls that the grouped kernels take (us of a layer grouped / as pairs: hidden 2048, 128 experts top-8, 5 / 8 /
-// 24 tokens 36 / 40 / 54 and 41 / 58 / 152; hidden 2880, 32 experts top-4, 5 / 8 tokens 75 / 78 and 96 / 140).
+// 24 tokens 36 / 38 / 52 and 42 / 59 / 153; hidden 2880, 32 experts top-4, 5 / 8 tokens 74 / 76 and 98 / 142).
 bool f8_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
     return L.format == TSA_EXPERT_FP8 && T > 4 && E <= MAX_GROUP_E && k <= 64;
 }
@@ -624,10 +630,9 @@ int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_
         p.yk = reinterpret_cast<float*>(ws + w.yk);
         const int64_t n = (int64_t)p.T * k;
         // Few tokens per expert fill tiles of 64 better, many read each weight for 128: us of a layer
-        // with tiles of 64 / 128, hidden 2048, 128 experts top-8, 24 / 300 / 600 / 1024 tokens 54 / 119 /
-        // 150 / 184 and 58 / 128 / 151 / 182; hidden 2880, 32 experts top-4, 100 / 300 / 700 / 2048 tokens
-        // 195 / 244 / 341 / 653 and 202 / 240 / 309 / 488. (Tiles of 32: 61 / 131 / 176 / 230 and 219 / 316 /
-        // 452 / 1055; 2% better only at 64 tokens of the first.)
+        // with tiles of 64 / 128, hidden 2048, 128 experts top-8, 24 / 300 / 600 / 1024 tokens 52 / 124 /
+        // 162 / 211 and 56 / 140 / 167 / 210; hidden 2880, 32 experts top-4, 100 / 300 / 700 / 2048 tokens
+        // 195 / 246 / 359 / 729 and 206 / 252 / 359 / 581. (Tiles of 32 measured 8 to 60% slower from 24 tokens.)
         p.tile_rows = n <= 48 * E ? 64 : 128;
         const int64_t entries = n / p.tile_rows + (E < n ? E : n);
         void* args[] = {&p};
