@@ -615,3 +615,24 @@ def test_moe_codes_of_h(T):
         want, _ = ref.moe(x, idx, w, ex)
         off += ((y.double() - want).norm(dim=1) / want.norm(dim=1)).tolist()
     assert sorted(off)[len(off) // 2] < 3.4e-4
+
+
+@pytest.mark.parametrize("E,k,H,I", [(20, 9, 256, 160), (20, 11, 64, 96), (20, 13, 128, 128), (16, 15, 96, 288), (24, 16, 64, 64),
+                                     (40, 33, 64, 32), (11, 10, 64, 6144), (13, 12, 32, 16384)])
+@pytest.mark.parametrize("T", [1, 3])
+def test_moe_many_experts_a_token(E, k, H, I, T):
+    """Each expert's own slot, scales and weight for odd numbers of experts past 8 and for odd pieces of
+    them staged at a time (inter 6144: 9 of 10; 16384: 3 of 12), together and each alone. Slot 0 holds no
+    expert."""
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I, list(range(E, 0, -1)))
+    slot = torch.arange(E, 0, -1, dtype=torch.int32, device=DEV)
+    x, (lg, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, ex)
+    ref.check(ops.moe_decode(L, pool, slot[idx.long()], w, x), want, err, "decode")
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), want, err, "prefill")
+    y, i2, w2 = ops.moe_decode_routed(L, pool, slot, lg, x, k, return_routing=True)
+    ref.check(y, *ref.moe(x, i2, w2, ex), "routed")
+    for j in range(k):
+        one = torch.nn.functional.one_hot(torch.full((T,), j, device=DEV), k).float()
+        ref.check(ops.moe_decode(L, pool, slot[idx.long()], one, x), *ref.moe(x, idx[:, j : j + 1], one[:, j : j + 1], ex), f"place {j}")

@@ -206,9 +206,10 @@ __global__ void __launch_bounds__(64 * F8D_NW, 4) fp8_down_kernel(F8Moe p) {
                 const int u = u0 + F8D_NW * d, pair = u / G, b = u % G;
                 if (u >= units) break;
                 const int ja = 2 * pair + (i >> 3), js = 2 * pair + (q >> 1);  // of the lane's row of A, of its sums
-                const int sa = ja < nc ? __shfl(my_slot, (c0 + ja) & 63, 64) : -1;
-                const int ss = js < nc ? __shfl(my_slot, (c0 + js) & 63, 64) : -1;
+                // every lane takes part in the shuffles: one that is off has 0 (a slot) read from it
+                const int la = __shfl(my_slot, (c0 + ja) & 63, 64), ls = __shfl(my_slot, (c0 + js) & 63, 64);
                 const float w = __shfl(my_w, (c0 + js) & 63, 64);
+                const int sa = ja < nc ? la : -1, ss = js < nc ? ls : -1;
                 const int o = F8B * b + 16 * q, row = n0 + (i & 7);
                 const uint8_t* at = p.pool + (int64_t)sa * L.slot_bytes + L.down_off + (int64_t)row * I + o;
                 const bool ok = sa >= 0 && row < H;
