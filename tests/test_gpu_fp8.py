@@ -636,3 +636,29 @@ def test_moe_many_experts_a_token(E, k, H, I, T):
     for j in range(k):
         one = torch.nn.functional.one_hot(torch.full((T,), j, device=DEV), k).float()
         ref.check(ops.moe_decode(L, pool, slot[idx.long()], one, x), *ref.moe(x, idx[:, j : j + 1], one[:, j : j + 1], ex), f"place {j}")
+
+
+@pytest.mark.parametrize("I", [32, 96, 288, 544])
+@pytest.mark.parametrize("T", [1, 3])
+def test_moe_dead_experts_stale_workspace(I, T):
+    """What the workspace holds in place of the h of an expert that is not resident (here NaN) does not
+    reach the result, for widths whose last group of channels is short."""
+    E, k, H = 20, 16, 64
+    ex = experts(1, E, H, I)
+    L, pool = pool_of(ex, H, I)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    slot[1::2] = -1
+    left = [None if e % 2 else x for e, x in enumerate(ex)]
+    x, (lg, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, left)
+    ws = ops.moe_decode_workspace(L, T, k, DEV)
+    sync = 32 << 10  # not written by these calls
+    ws[sync:] = 255
+    ref.check(ops.moe_decode(L, pool, slot[idx.long()], w, x, workspace=ws), want, err, "decode")
+    ws[sync:] = 255
+    y, i2, w2 = ops.moe_decode_routed(L, pool, slot, lg, x, k, workspace=ws, return_routing=True)
+    ref.check(y, *ref.moe(x, i2, w2, left), "routed")
+    for n in (T, 9):
+        x, (_, idx, w) = acts(n, n, H), routes(n, n, E, k)
+        wp = ops.moe_prefill_workspace(L, n, k, E, DEV).fill_(255)
+        ref.check(ops.moe_prefill(L, pool, slot, idx, w, x, workspace=wp), *ref.moe(x, idx, w, left), "prefill")

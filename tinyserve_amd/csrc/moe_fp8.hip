@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(64 * F8D_NW, 4) fp8_down_kernel(F8Moe p) {
             const int j = c / (G * 16), o = 8 * (c % (G * 16));
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            if (c < tasks && o < I && __shfl(my_slot, (c0 + j) & 63, 64) >= 0) f8_load8<TSA_F32>(hrow + (int64_t)j * I, o / 8, v);
+            const int slot = __shfl(my_slot, (c0 + j) & 63, 64);  // outside the condition: every lane takes part
+            if (c < tasks && o < I && slot >= 0) f8_load8<TSA_F32>(hrow + (int64_t)j * I, o / 8, v);
         };
         float hv[F8D_HC][8];
 #pragma unroll
