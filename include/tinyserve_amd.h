@@ -61,7 +61,8 @@ typedef enum tsa_expert_format { TSA_EXPERT_MXFP4 = 1, TSA_EXPERT_GGUF = 2, TSA_
  *    gate_scales_off (gate's [ceil(I/128), ceil(H/128)], then up's) and at down_scales_off
  *    ([ceil(H/128), ceil(I/128)]), both multiples of 4. No biases (-1). Pool, x and workspaces
  *    16-byte aligned. Activations are quantised as tsa_fp8_quantize does, x before gate and up and
- *    h = act(gate, up) (float32) before down.
+ *    h = act(gate, up) (float32) before down. Sums are of float32 accuracy but for down's where y has
+ *    16 bits, which are tsa_fp8_matmul's.
  *  act: TSA_ACT_SWIGLU_OAI = (up+1)*g*sigmoid(alpha*g), g = min(gate, limit),
  *    up = clamp(up, -limit, limit); TSA_ACT_SILU = silu(gate)*up.
  *  prefill_mfma (tiled MXFP4 prefill GEMMs): TSA_PREFILL_FP6 (0, the default) multiplies the

@@ -662,3 +662,55 @@ def test_moe_dead_experts_stale_workspace(I, T):
         x, (_, idx, w) = acts(n, n, H), routes(n, n, E, k)
         wp = ops.moe_prefill_workspace(L, n, k, E, DEV).fill_(255)
         ref.check(ops.moe_prefill(L, pool, slot, idx, w, x, workspace=wp), *ref.moe(x, idx, w, left), "prefill")
+
+
+def _known_h(H, I, up, up_scales):
+    """An expert without down whose h is known exactly: a token of _known_x gives gate sums of 32, so that
+    silu(gate) is 32 in float32, and up sums of up_scales[:, b] up[:, b] of each K block b."""
+    e = {}
+    for n, (r, c) in (("gate_proj", (I, H)), ("up_proj", (I, H)), ("down_proj", (H, I))):
+        e[n] = torch.zeros((r, c), device=DEV)
+        e[n + "_scale_inv"] = torch.ones((ref.blocks(r), ref.blocks(c)), device=DEV)
+    e["gate_proj"][:, 1] = 32
+    e["gate_proj_scale_inv"][:] = 2.0**-8
+    e["up_proj"][:, 1::128] = up
+    e["up_proj_scale_inv"][:] = up_scales * 2.0**-8
+    return e
+
+
+def _known_x(T, H, dtype):
+    """Tokens whose scales are 1 and whose code in column 1 of each block is 256."""
+    x = torch.zeros((T, H), device=DEV)
+    x[:, ::128], x[:, 1::128] = 448, 256
+    return x.to(dtype)
+
+
+def _codes(e):
+    return {n: t.to(torch.float8_e4m3fn) if not n.endswith("_scale_inv") else t for n, t in e.items()}
+
+
+@pytest.mark.parametrize("T", [1, 9, 300])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_moe_float32_sums(T, dtype):
+    """A float32 layer result keeps what is 2^-17 of the largest product beside it: two products of 448
+    that cancel, the 14 of 2^-9 around them stay. Every sum and product here is exact in float32."""
+    from tinyserve_amd.expert_forward import FP8ExpertModule, _precompute_param_refs, forward_from_packed
+
+    H, I = 128, 128
+    up = torch.zeros((I, 1), device=DEV)
+    up[:16] = 2.0**-9
+    up[:16:8] = 448
+    e = _known_h(H, I, up, torch.ones((1, 1), device=DEV))
+    n = torch.arange(H, device=DEV) % 8 + 1
+    e["down_proj"][:, :16] = n.unsqueeze(1).float()
+    e["down_proj"][:, 0], e["down_proj"][:, 8] = 1, -1
+    L, pool = pool_of([_codes(e)], H, I)
+    x, want = _known_x(T, H, dtype), (32 * 14 * 2.0**-9 * n).expand(T, H).float()
+    zero, one = torch.zeros((T, 1), dtype=torch.int32, device=DEV), torch.ones((T, 1), device=DEV)
+    assert torch.equal(ops.moe_decode(L, pool, zero, one, x, out_dtype=F32), want)
+    assert torch.equal(ops.moe_decode_routed(L, pool, zero[0], one, x, 1, out_dtype=F32), want)
+    assert torch.equal(ops.moe_prefill(L, pool, zero[0], zero, one, x, out_dtype=F32), want)
+    if dtype == F32:
+        lay = synth.fp8_layout(H, I)
+        mod = FP8ExpertModule(lay, device=DEV)
+        assert torch.equal(forward_from_packed(mod, pool[0], _precompute_param_refs(mod, lay), x), want)

@@ -13,7 +13,8 @@
 // A layer's bf16 result is then off by its own rounding (0.0017 rms over 12 to 785 tokens), with the FP8
 // instructions by 0.0018 to 0.0032. us, float32 accuracy / FP8 instructions: hidden 2880, 32 experts top-4,
 // 8 layers of 4 tokens 632 / 613, a layer of 2048 570 / 490; hidden 2048, 128 experts top-8, 24 tokens 58 / 57,
-// 1024 tokens 210 / 187.
+// 1024 tokens 210 / 187. Down is summed so where the layer's result is float32; for 16-bit ones the FP8
+// instructions' sums are far below the last rounding.
 #include "fp8_gemm.h"
 #include "moe_group.h"
 
@@ -166,6 +167,7 @@ __device__ const uint32_t f8_zeros[4] = {0, 0, 0, 0};  // what lanes past a matr
 // One workgroup per token and 8 outputs, over all the token's experts: rows 0 .. 7 of a tile are the
 // outputs' rows of an even expert, 8 .. 15 those of the next, which meet columns 0 and 1 (their h); a
 // unit is a K block of such a pair, and the waves take the units in turn.
+template <bool WIDE>
 __global__ void __launch_bounds__(64 * F8D_NW, 4) fp8_down_kernel(F8Moe p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), q = lane >> 4, i = lane & 15;
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(64 * F8D_NW, 4) fp8_down_kernel(F8Moe p) {
                     Bv[1] = *reinterpret_cast<const u32x4*>(hc + F8B * (j * G + b) + 64 + 16 * q);
                 }
                 const float s = js < nc ? sc[d] * hs[js * G + b] : 0.0f;
-                const v4f part = f8_mfma(A[d], Bv);
+                const v4f part = f8_mfma<WIDE>(A[d], Bv);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] = fmaf(s, part[e], acc[e]);
             }
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p
     }
 }
 
-template <class C>
+template <class C, bool WIDE>
 __global__ void __launch_bounds__(C::THREADS) fp8_group_down_kernel(F8Group p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const tsa_expert_layout& L = p.L;
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_down_kernel(F8Group p) {
     o.K = I;
     o.G = GI;
     v4f acc[C::MR][C::MT];
-    f8_tile<C, 1, false>(o, smem, tn, [&](int r) { return r < tn ? r : -1; }, acc);
+    f8_tile<C, 1, WIDE>(o, smem, tn, [&](int r) { return r < tn ? r : -1; }, acc);
 #pragma unroll
     for (int t = 0; t < C::MT; ++t) {
         const int tk = 16 * (C::MT * wt + t) + i;
@@ -517,7 +519,8 @@ int group_gemms(const F8Group& p, int64_t entries, hipStream_t st) {
     F8Group q = p;
     void* args[] = {&q};
     const void* fg = reinterpret_cast<const void*>(&fp8_group_gate_up_kernel<GU>);
-    const void* fd = reinterpret_cast<const void*>(&fp8_group_down_kernel<DN>);
+    const void* fd = p.y_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_group_down_kernel<DN, true>)
+                                          : reinterpret_cast<const void*>(&fp8_group_down_kernel<DN, false>);
     TSA_HIP_CHECK(ensure_dynamic_lds(fg, GU::LDS));
     TSA_HIP_CHECK(ensure_dynamic_lds(fd, DN::LDS));
     static_assert(GU::TM == DN::TM, "one table of token tiles");
@@ -581,8 +584,9 @@ int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, 
         pb.wts = p.tab_w;
     }
     void* args_b[] = {&pb};
-    TSA_HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(&fp8_down_kernel), dim3((unsigned)((L.hidden + 7) / 8), (unsigned)T),
-                                  dim3(64 * F8D_NW), args_b, lds_b, st));
+    const void* fb = y_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_down_kernel<true>)
+                                        : reinterpret_cast<const void*>(&fp8_down_kernel<false>);
+    TSA_HIP_CHECK(hipLaunchKernel(fb, dim3((unsigned)((L.hidden + 7) / 8), (unsigned)T), dim3(64 * F8D_NW), args_b, lds_b, st));
     return TSA_OK;
 }
 
