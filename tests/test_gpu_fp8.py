@@ -714,3 +714,70 @@ def test_moe_float32_sums(T, dtype):
         lay = synth.fp8_layout(H, I)
         mod = FP8ExpertModule(lay, device=DEV)
         assert torch.equal(forward_from_packed(mod, pool[0], _precompute_param_refs(mod, lay), x), want)
+
+
+@pytest.mark.parametrize("value,scale", [("0x1.800002p-109", "0x1.000002p-100"), ("0x1.400004p-108", "0x1.000004p-100"),
+                                         ("0x1.b80004p-104", "0x1.400002p-97"), ("0x1p-104", "0x1.fffffep-95"),
+                                         ("0x1.800002p-19", "0x1.000002p-10"), ("0x1.b80004p3", "0x1.400002p10")])
+@pytest.mark.parametrize("T", [1, 9, 300])
+def test_moe_quotients_of_h(T, value, scale):
+    """Codes of h from the correctly rounded quotient: (value, scale) pairs whose quotient rounds onto a
+    border between two codes, or next to it."""
+    import numpy as np
+
+    v, s = (np.float32(float.fromhex(t)) for t in (value, scale))
+    top = next(m for m in (np.float32(448 * float(s)) * np.float32(1 + d * 2.0**-23) for d in (0, 1, -1, 2, -2)) if m / np.float32(448) == s)
+    H, I = 256, 128
+    up = torch.zeros((I, 2), device=DEV)
+    up[0, 0] = up[1, 1] = 1
+    e = _known_h(H, I, up, torch.tensor([[float(top) / 32, float(v) / 32]], device=DEV))
+    e["down_proj"][:, 1] = 1
+    L, pool = pool_of([_codes(e)], H, I)
+    code = ref.e4m3(torch.tensor(float(v / s), dtype=torch.float64))
+    want = torch.full((T, H), float(code) * float(s), dtype=F32, device=DEV)
+    zero, one = torch.zeros((T, 1), dtype=torch.int32, device=DEV), torch.ones((T, 1), device=DEV)
+    x = _known_x(T, H, F32)
+    assert torch.equal(ops.moe_decode(L, pool, zero, one, x), want)
+    assert torch.equal(ops.moe_prefill(L, pool, zero[0], zero, one, x), want)
+
+
+def _fma(a, b, c):
+    """a b + c of float32 values (held in 64 bits) rounded once to float32: the 64-bit sum's own error moves it
+    off the border that it may have been rounded onto."""
+    p = a * b  # exact
+    t = c + p
+    big = torch.maximum(c.abs(), p.abs()) == c.abs()
+    err = torch.where(big, (c - t) + p, (p - t) + c)
+    return torch.where(err != 0, torch.nextafter(t, t + err.sign() * t.abs()), t).float().double()
+
+
+def test_corrected_quotient_is_the_division():
+    """x / s by a rounded reciprocal and one correction equals the division for every significand of s and
+    the x within 3 steps of a border between two codes (normal ones: odd 16ths; subnormal ones: odd numbers)."""
+    borders = [o / 16 for o in range(17, 32, 2)] + [o / 2 ** (o.bit_length() - 1) for o in range(1, 16, 2)]
+    for lo in range(0, 1 << 23, 1 << 20):
+        s = 1 + torch.arange(lo, lo + (1 << 20), device=DEV).double() / 2**23
+        r = (1 / s).float().double()
+        for b in borders:
+            x0 = (b * s).float().view(torch.int32)
+            for d in range(-3, 4):
+                x = (x0 + d).view(torch.float32).double()
+                a = (x * r).float().double()
+                assert torch.equal(_fma(_fma(-a, s, x), r, a), (x / s).float().double())
+
+
+@pytest.mark.parametrize("dtype,top,low", [(HF, 15, -5), (BF, 10, -10)])
+def test_quantize_every_quotient(dtype, top, low):
+    """All significands of a group's maximum with all significands of smaller values down to the ones
+    whose code is zero: the codes are the division's."""
+    bits = {HF: 10, BF: 7}[dtype]
+    sig = 1 + torch.arange(2**bits, device=DEV).double() / 2**bits
+    m = sig * 2.0**top
+    v = torch.cat([sig * 2.0**e for e in range(low, top + 1)])
+    v = torch.nn.functional.pad(v, (0, -len(v) % 127)).view(-1, 127)
+    for part in m.split(64):
+        x = torch.minimum(v.expand(len(part), -1, -1), part.view(-1, 1, 1))
+        x = torch.cat([part.view(-1, 1, 1).expand(-1, len(v), 1), x], 2).reshape(-1, 128)
+        c, s = ops.fp8_quantize(x.to(dtype))
+        q64, s64 = ref.quantize(x)
+        assert torch.equal(s.double(), s64) and torch.equal(c.double(), q64)

@@ -88,15 +88,19 @@ __device__ __forceinline__ float f8_scale(uint32_t max_bits) {
     return s < 0x1p-126f ? 0x1p-126f : s;  // a NaN stays one
 }
 
+constexpr float F8_MIN_CORRECTED = 0x1p-90f;  // scales below it divide
+
 // The codes of 8 values of a group with scale s. The quotient by Markstein's correction: with r the
-// rounded reciprocal of s, q = x r and the exact remainder e = x - q s, q + e r rounds to x / s. (For
-// every s and every bf16 or fp16 x it is the correctly rounded quotient, checked for all their
-// significands; 3 instructions instead of a division's 10.) EXACT (fp32 inputs) and groups whose
-// remainder could underflow or that hold an infinity or NaN divide.
+// rounded reciprocal of s, q = x r and the remainder e = x - q s, q + e r rounds to x / s: 3 instructions
+// instead of a division's 10. Compared with the division for the float32 x that lie within 3 steps of
+// (a border between two codes) s, for every significand of s, it gives the same quotient; elsewhere a
+// step of the quotient changes no code. That holds where no bit of e underflows, from s = 2^-93 on for
+// codes that are not zero. (At 2^-100 .. 2^-94 a few borders come out on the other side.) EXACT (fp32
+// inputs), groups of smaller scales and ones that hold an infinity or NaN divide.
 template <bool EXACT>
 __device__ __forceinline__ uint2 f8_codes8(const float (&v)[8], float s) {
     float q[8];
-    if (EXACT || !(s > 0x1p-100f && s < INFINITY)) {
+    if (EXACT || !(s > F8_MIN_CORRECTED && s < INFINITY)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] = v[e] / s;
     } else {
@@ -116,7 +120,7 @@ __device__ __forceinline__ uint2 f8_codes8(const float (&v)[8], float s) {
 // The codes of 4 computed (fp32) values of a group with scale s, as one word: the same quotient.
 __device__ __forceinline__ uint32_t f8_codes4(const v4f& v, float s) {
     float q[4];
-    if (!(s > 0x1p-100f && s < INFINITY)) {
+    if (!(s > F8_MIN_CORRECTED && s < INFINITY)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) q[e] = v[e] / s;
     } else {
