@@ -781,3 +781,40 @@ def test_quantize_every_quotient(dtype, top, low):
         c, s = ops.fp8_quantize(x.to(dtype))
         q64, s64 = ref.quantize(x)
         assert torch.equal(s.double(), s64) and torch.equal(c.double(), q64)
+
+
+def _swiglu_layer(E, H, I):
+    """Experts whose gates and ups pass the limits of 7, under the clamped activation."""
+    from tinyserve_amd import _lib
+
+    ex = experts(3, E, H, I)
+    for e in ex:
+        e["gate_proj_scale_inv"] *= 8
+        e["up_proj_scale_inv"] *= 8
+    L, pool = pool_of(ex, H, I)
+    L.act = _lib.ACT_SWIGLU_OAI
+    return ex, L, pool
+
+
+@pytest.mark.parametrize("T", [2, 9, 300])
+def test_moe_swiglu_nan_token(T):
+    """The limits of the clamped activation let a NaN through: its token comes out NaN, no other changes."""
+    E, k, H, I = 4, 2, 256, 160
+    _, L, pool = _swiglu_layer(E, H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    slot = torch.arange(E, dtype=torch.int32, device=DEV)
+    bad = x.clone()
+    bad[T // 2, 7] = float("nan")
+    keep = torch.arange(T, device=DEV) != T // 2
+    for f in (lambda v: ops.moe_decode(L, pool, idx, w, v), lambda v: ops.moe_prefill(L, pool, slot, idx, w, v)):
+        y, z = f(x), f(bad)
+        assert torch.isnan(z[T // 2]).all() and torch.equal(z[keep], y[keep])
+
+
+@pytest.mark.parametrize("T", [9, 60, 300])
+def test_moe_swiglu_prompt(T):
+    E, k, H, I = 4, 2, 256, 352
+    ex, L, pool = _swiglu_layer(E, H, I)
+    x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
+    want, err = ref.moe(x, idx, w, ex, act="swiglu")
+    ref.check(ops.moe_prefill(L, pool, torch.arange(E, dtype=torch.int32, device=DEV), idx, w, x), want, err)

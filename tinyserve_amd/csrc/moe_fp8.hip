@@ -46,7 +46,12 @@ constexpr int F8A_NW = 8, F8A_D = 3, F8A_XC = 1;  // gate_up: waves; K blocks in
 constexpr int F8D_NW = 8, F8D_D = 3, F8D_HC = 2;  // down: the same with its units and h
 
 __device__ __forceinline__ float f8_act(const tsa_expert_layout& L, float gate, float up) {
-    if (L.act == TSA_ACT_SWIGLU_OAI) return swiglu_oai_fast(L, gate, up);
+    if (L.act == TSA_ACT_SWIGLU_OAI) {
+        // the limits by comparisons: a minimum or maximum would give its other operand for a NaN
+        const float lim = L.swiglu_limit, g = gate > lim ? lim : gate, u = up > lim ? lim : up < -lim ? -lim : up;
+        const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * (L.swiglu_alpha * g));
+        return (u + 1.0f) * g * __builtin_amdgcn_rcpf(1.0f + e);
+    }
     return silu_mul_fast(gate, up);
 }
 
