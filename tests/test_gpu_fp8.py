@@ -818,3 +818,34 @@ def test_moe_swiglu_prompt(T):
     x, (_, idx, w) = acts(T, T, H), routes(T, T, E, k)
     want, err = ref.moe(x, idx, w, ex, act="swiglu")
     ref.check(ops.moe_prefill(L, pool, torch.arange(E, dtype=torch.int32, device=DEV), idx, w, x), want, err)
+
+
+@pytest.mark.parametrize("T,K", [((1 << 28) + 5, 1), ((1 << 28) + 300, 8)])
+def test_quantize_past_2_28_groups(T, K):
+    """More groups than one launch has room for: every one is quantised."""
+    x = acts(1, 1 << 20, K).repeat(-(-T // (1 << 20)), 1)[:T]
+    c, s = ops.fp8_quantize(x)
+    c1, s1 = ops.fp8_quantize(x[: 1 << 20])
+    for t in range(0, T, 1 << 20):
+        n = min(1 << 20, T - t)
+        assert torch.equal(c[t : t + n].view(torch.uint8), c1[:n].view(torch.uint8)) and torch.equal(s[t : t + n], s1[:n])
+
+
+@pytest.mark.parametrize("T,K", [(2, (1 << 31) - 1), (9, (1 << 31) - 8)])
+def test_quantize_longest_rows(T, K):
+    """Rows up to 2^31 values, more of them than a launch takes (8)."""
+    x = torch.empty((T, K), dtype=BF, device=DEV)
+    part = acts(2, 1 << 20)
+    for t in range(T):
+        for o in range(0, K, 1 << 20):
+            x[t, o : o + (1 << 20)] = part[: min(1 << 20, K - o)]
+    c, s = ops.fp8_quantize(x)
+    del x
+    q, qs = ops.fp8_quantize(part.unsqueeze(0))
+    last = (K - 1) >> 20 << 20
+    for t in range(T):
+        for o in (0, 1 << 30, last - (1 << 20)):
+            assert torch.equal(c[t, o : o + (1 << 20)].view(torch.uint8), q[0].view(torch.uint8))
+            assert torch.equal(s[t, o // 128 : (o + (1 << 20)) // 128], qs[0])
+        e, es = ops.fp8_quantize(part[: K - last].unsqueeze(0))
+        assert torch.equal(c[t, last:].view(torch.uint8), e[0].view(torch.uint8)) and torch.equal(s[t, last // 128 :], es[0])

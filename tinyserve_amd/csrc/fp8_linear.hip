@@ -14,37 +14,47 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const void* __restric
     if (g >= T * G) return;  // the 16 lanes of a group return together
     const int64_t t = g / G;
     const int c = (int)(g - t * G) * 16 + (int)(task & 15);
+    const uint32_t col = 8u * (uint32_t)c;  // up to 2^31 + 120
     constexpr int ES = XT == TSA_F32 ? 4 : 2;
     const uint8_t* row = static_cast<const uint8_t*>(x) + t * K * ES;
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (VEC) {
-        if (8 * c < K) f8_load8<XT>(row, c, v);
+        if (col < (uint32_t)K) f8_load8<XT>(row, c, v);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (8 * c + e < K) v[e] = load_act(row, XT, 8 * c + e);
+            if (col + e < (uint32_t)K) v[e] = load_act(row, XT, (int64_t)(col + e));
     }
     const float s = f8_scale(f8_group_max(v));
     const uint2 o = f8_codes8<XT == TSA_F32>(v, s);
-    uint8_t* dst = codes + t * K + 8 * c;
+    uint8_t* dst = codes + t * K + col;
     if constexpr (VEC) {
-        if (8 * c < K) *reinterpret_cast<uint2*>(dst) = o;
+        if (col < (uint32_t)K) *reinterpret_cast<uint2*>(dst) = o;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (8 * c + e < K) dst[e] = (uint8_t)((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
+            if (col + e < (uint32_t)K) dst[e] = (uint8_t)((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
     }
     if ((task & 15) == 0) scales[g] = s;
 }
 
+// A launch ends at 2^32 threads (2^28 groups): more rows than that go in several.
 template <int XT>
 hipError_t launch_quantize(const void* x, int64_t T, int64_t K, uint8_t* codes, float* scales, hipStream_t st) {
     constexpr uintptr_t AL = 15;
+    constexpr int ES = XT == TSA_F32 ? 4 : 2;
     const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & AL) == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
-    const dim3 grid((unsigned)((T * f8_blocks(K) * 16 + 255) / 256));
-    if (vec) hipLaunchKernelGGL((fp8_quantize_kernel<XT, true>), grid, dim3(256), 0, st, x, T, (int)K, codes, scales);
-    else hipLaunchKernelGGL((fp8_quantize_kernel<XT, false>), grid, dim3(256), 0, st, x, T, (int)K, codes, scales);
-    return hipGetLastError();
+    const int64_t G = f8_blocks(K), step = ((int64_t)1 << 27) / G;  // K < 2^31: 8 rows and more
+    for (int64_t t = 0; t < T; t += step) {
+        const int64_t n = T - t < step ? T - t : step;
+        const uint8_t* xt = static_cast<const uint8_t*>(x) + t * K * ES;
+        const dim3 grid((unsigned)((n * G * 16 + 255) / 256));
+        if (vec) hipLaunchKernelGGL((fp8_quantize_kernel<XT, true>), grid, dim3(256), 0, st, xt, n, (int)K, codes + t * K, scales + t * G);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<XT, false>), grid, dim3(256), 0, st, xt, n, (int)K, codes + t * K, scales + t * G);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // ---------------------------------------------------------------- few tokens
