@@ -154,8 +154,8 @@ int tsa_fp8_quantize(const void* x, int x_dtype, int64_t T, int64_t K, void* cod
  * (+ bias[n], may be NULL), one rounding to y_dtype. Blocks are summed in float32; inside a block
  * 16-bit results come from the FP8 matrix instructions, which add the products of 8 neighbouring
  * values with 13 bits below the largest (1.4e-5 of the sum, rms), float32 results from the bf16 ones
- * (float32 accuracy). K a multiple of 16 of at most 2^20, T and N at most 2^30; codes and w 16-byte
- * aligned. */
+ * (float32 accuracy). K a multiple of 16 of at most 2^20, T and N at most 2^30 (products of more than 32
+ * tokens that no launch covers, from about 2^37 results on, are refused); codes and w 16-byte aligned. */
 int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T, int64_t K, const void* w, const float* w_scales,
                    int64_t N, const void* bias, int bias_dtype, void* y, int y_dtype, void* stream);
 

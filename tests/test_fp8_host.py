@@ -40,6 +40,16 @@ def test_matmul_refusals(lib, T, K, N, rc, text):
     assert lib.tsa_fp8_linear(P, 2, T, K, P, P, N, None, 0, P, 2, P, 1 << 50, None) == rc and text in lib.tsa_last_error()
 
 
+@pytest.mark.parametrize("T,N,y,ok", [(129, 1 << 30, 0, False), (1 << 30, 1 << 20, 2, False), (1 << 30, 1 << 30, 2, False),
+                                      (33, 1 << 30, 0, True), (128, 1 << 30, 2, True), (1 << 30, 128, 0, True)])
+def test_matmul_more_than_a_launch(lib, T, N, y, ok):
+    """Products that no tile covers in one launch are refused before anything runs; the largest others get as
+    far as the check of their pointers."""
+    assert lib.tsa_fp8_matmul(None, None, T, 16, None, None, N, None, 0, None, y, None) == (_lib.ERR_INVALID_ARG if ok else _lib.ERR_SHAPE)
+    assert (b"null pointer" if ok else b"too large") in lib.tsa_last_error()
+    assert lib.tsa_fp8_linear(None, 2, T, 16, None, None, N, None, 0, None, y, None, 0, None) == (_lib.ERR_INVALID_ARG if ok else _lib.ERR_SHAPE)
+
+
 def test_matmul_argument_errors(lib):
     bad = _lib.ERR_INVALID_ARG
     assert lib.tsa_fp8_matmul(None, P, 4, 128, P, P, 64, None, 0, P, 2, None) == bad

@@ -849,3 +849,21 @@ def test_quantize_longest_rows(T, K):
             assert torch.equal(s[t, o // 128 : (o + (1 << 20)) // 128], qs[0])
         e, es = ops.fp8_quantize(part[: K - last].unsqueeze(0))
         assert torch.equal(c[t, last:].view(torch.uint8), e[0].view(torch.uint8)) and torch.equal(s[t, last // 128 :], es[0])
+
+
+@pytest.mark.parametrize("T,dtype", [(1, F32), (17, BF), (33, BF)])
+def test_matmul_past_2_27_rows(T, dtype):
+    """More weight rows than one launch of the row kernel has room for (2^26 a launch), and as many in tiles."""
+    N, K = (1 << 27) + 1000, 16
+    g = gen(1)
+    w = torch.randint(0, 0x60, (N, K), dtype=torch.uint8, device=DEV, generator=g).view(torch.float8_e4m3fn)
+    ws = torch.rand((ref.blocks(N), 1), device=DEV, generator=g) * 1e-2
+    b = torch.randn(N, device=DEV, generator=g).to(BF)
+    x = acts(2, T, K)
+    y = ops.fp8_linear(x, w, ws, b, out_dtype=dtype)
+    q, s = ref.quantize(x.double())
+    for n in (0, (1 << 26) - 256, (1 << 27) - 256, N // 128 * 128 - 512):
+        r = slice(n, min(n + 1024, N))
+        want, err = ref.matmul(q, s, w[r], ws[n // 128 :][: ref.blocks(r.stop - n)], wide=dtype == F32)
+        bias = b[r].double()
+        ref.check(y[:, r], want + bias, err + (bias.abs() + want.abs()) * 2.0**-23)

@@ -67,7 +67,7 @@ struct F8Rows {
     int bias_dtype;
     void* y;
     int y_dtype;
-    int64_t T, N;
+    int64_t T, N, ldy;  // ldy: y's row, N of the whole product
     int K, G;
     int tiles_n, rows;  // rows: tokens of the largest tile
 };
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(64 * F8R_NW) fp8_rows_kernel(F8Rows p) {
 #pragma unroll
         for (int w = 0; w < F8R_NW; ++w) v += red[w * 256 * MT + o];
         if (p.bias) v += load_act(p.bias, p.bias_dtype, n);
-        store_out(p.y, p.y_dtype, t * p.N + n, v);
+        store_out(p.y, p.y_dtype, t * p.ldy + n, v);
     }
 }
 
@@ -197,9 +197,21 @@ hipError_t launch_rows(const F8Rows& p, hipStream_t st) {
                                           : reinterpret_cast<const void*>(&fp8_rows_kernel<XT, MT, false>);
     const hipError_t e = ensure_dynamic_lds(fn, lds);
     if (e != hipSuccess) return e;
-    F8Rows q = p;
-    void* args[] = {&q};
-    return hipLaunchKernel(fn, dim3((unsigned)(p.tiles_n * ((p.T + 16 * MT - 1) / (16 * MT)))), dim3(64 * F8R_NW), args, lds, st);
+    // a launch ends at 2^32 threads, 2^23 of these workgroups: more rows than that go in several
+    const int64_t tiles_t = (p.T + 16 * MT - 1) / (16 * MT), step = ((int64_t)1 << 22) / tiles_t * 16 / F8B * F8B;
+    for (int64_t n = 0; n < p.N; n += step) {
+        F8Rows q = p;
+        q.N = p.N - n < step ? p.N - n : step;
+        q.tiles_n = (int)((q.N + 15) / 16);
+        q.w = p.w + n * p.K;
+        q.ws = p.ws + n / F8B * p.G;
+        if (p.bias) q.bias = static_cast<const uint8_t*>(p.bias) + n * dtype_size(p.bias_dtype);
+        q.y = static_cast<uint8_t*>(p.y) + n * dtype_size(p.y_dtype);
+        void* args[] = {&q};
+        const hipError_t l = hipLaunchKernel(fn, dim3((unsigned)(q.tiles_n * tiles_t)), dim3(64 * F8R_NW), args, lds, st);
+        if (l != hipSuccess) return l;
+    }
+    return hipSuccess;
 }
 
 hipError_t pick_rows(const F8Rows& p, hipStream_t st) {
@@ -294,20 +306,30 @@ using TileC = F8Tile<2, 2, 4, 4, 2>;  // 128 x 128
 using TileD = F8Tile<4, 1, 2, 4, 3>;  // 128 x 64
 using TileE = F8Tile<4, 1, 1, 2, 4>;  // 64 x 32
 
-// The tile with the least rounds x round time, a round being `per` workgroups on every CU.
-template <bool WIDE>
-hipError_t pick_gemm(const F8Gemm& p, hipStream_t st) {
-    struct Tile { int rows, tok, per, cost; };
-    constexpr Tile tiles[5] = {{256, 256, 1, 45}, {256, 128, 1, 26}, {128, 128, 2, 32}, {128, 64, 2, 20}, {64, 32, 3, 13}};
+// The tile (A .. E as 0 .. 4) with the least rounds x round time, a round being `per` workgroups on
+// every CU; -1 if every tile needs more workgroups than a launch takes (2^32 threads).
+int gemm_tile(int64_t T, int64_t N, bool wide) {
+    struct Tile { int rows, tok, threads, per, cost; };
+    constexpr Tile tiles[5] = {{TileA::RN, TileA::TM, TileA::THREADS, 1, 45},
+                               {TileB::RN, TileB::TM, TileB::THREADS, 1, 26},
+                               {TileC::RN, TileC::TM, TileC::THREADS, 2, 32},
+                               {TileD::RN, TileD::TM, TileD::THREADS, 2, 20},
+                               {TileE::RN, TileE::TM, TileE::THREADS, 3, 13}};
     const int64_t cus = num_cus() > 0 ? num_cus() : 256;
-    int best = 0;
+    int best = -1;
     int64_t least = INT64_MAX;
-    for (int i = WIDE ? 1 : 0; i < 5; ++i) {  // 256 x 256 has no registers for the widened operands
-        const int64_t wgs = (int64_t)((p.N + tiles[i].rows - 1) / tiles[i].rows) * ((p.T + tiles[i].tok - 1) / tiles[i].tok);
+    for (int i = wide ? 1 : 0; i < 5; ++i) {  // 256 x 256 has no registers for the widened operands
+        const int64_t wgs = (N + tiles[i].rows - 1) / tiles[i].rows * ((T + tiles[i].tok - 1) / tiles[i].tok);
+        if (wgs * tiles[i].threads >= (int64_t)1 << 32) continue;
         const int64_t cost = (wgs + cus * tiles[i].per - 1) / (cus * tiles[i].per) * tiles[i].cost;
         if (cost < least) least = cost, best = i;
     }
-    switch (best) {
+    return best;
+}
+
+template <bool WIDE>
+hipError_t pick_gemm(const F8Gemm& p, hipStream_t st) {
+    switch (gemm_tile(p.T, p.N, WIDE)) {
         case 0:
             if constexpr (!WIDE) return launch_gemm<TileA, WIDE>(p, st);
             return hipErrorInvalidValue;
@@ -325,7 +347,7 @@ int check_matmul(int64_t T, int64_t K, int64_t N, const void* bias, int bias_dty
                 (long long)K);
     TSA_REQUIRE(K % 16 == 0 && K <= F8_MAX_K, TSA_ERR_SHAPE, "K (%lld) must be a multiple of 16 of at most %lld", (long long)K,
                 (long long)F8_MAX_K);
-    TSA_REQUIRE(T <= ((int64_t)1 << 30) && N <= ((int64_t)1 << 30) && (T + 15) / 16 * ((N + 15) / 16) < ((int64_t)1 << 31),
+    TSA_REQUIRE(T <= ((int64_t)1 << 30) && N <= ((int64_t)1 << 30) && (T <= 32 || gemm_tile(T, N, y_dtype == TSA_F32) >= 0),
                 TSA_ERR_SHAPE, "T %lld x N %lld is too large", (long long)T, (long long)N);
     TSA_REQUIRE(valid_dtype(y_dtype), TSA_ERR_INVALID_ARG, "bad dtype (y %d)", y_dtype);
     TSA_REQUIRE(!bias || valid_dtype(bias_dtype), TSA_ERR_INVALID_ARG, "bad dtype (bias %d)", bias_dtype);
@@ -349,7 +371,7 @@ F8Rows rows_params(const void* x, const float* xs, int64_t T, int64_t K, const v
     p.N = N;
     p.K = (int)K;
     p.G = (int)f8_blocks(K);
-    p.tiles_n = (int)((N + 15) / 16);
+    p.ldy = N;
     p.rows = (int)(T < 16 ? T : 16);
     return p;
 }
