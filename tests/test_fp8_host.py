@@ -181,3 +181,31 @@ def test_replace_linear():
         FP8Linear(torch.zeros(4, 24, dtype=torch.float8_e4m3fn), torch.zeros(1, 1), device="cpu")
     with pytest.raises(ValueError, match="float8_e4m3fn"):
         FP8Linear(torch.zeros(4, 32), torch.zeros(1, 1), device="cpu")
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.type(torch.float16),
+                                  lambda m: m.to("cpu", torch.float16), lambda m: m.float()])
+def test_casts_keep_the_format(cast):
+    """A model cast to another type keeps its FP8 weights and their scales; biases and the rest change."""
+    from tinyserve_amd.expert_forward import FP8ExpertModule
+
+    w, s = synth.make_fp8(np.random.default_rng(0), 160, 144)
+    model = nn.Sequential(FP8Linear(w, s, torch.randn(160), device="cpu"), nn.Linear(4, 4))
+    lin = cast(model)[0]
+    assert lin.weight.dtype == torch.float8_e4m3fn and torch.equal(lin.weight.view(torch.uint8), w.view(torch.uint8))
+    assert lin.weight_scale_inv.dtype == torch.float32 and torch.equal(lin.weight_scale_inv, s)
+    assert lin.bias.dtype == model[1].weight.dtype and not lin.weight.requires_grad
+    assert set(dict(lin.named_parameters())) == {"weight", "weight_scale_inv", "bias"}
+    lay = synth.fp8_layout(128, 96)
+    mod = cast(FP8ExpertModule(lay, device="cpu"))
+    assert {n: p.dtype for n, p in mod.named_parameters()} == {n: d for n, (_, d) in lay.specs.items()}
+
+
+def test_module_moves_and_loads():
+    w, s = synth.make_fp8(np.random.default_rng(0), 32, 48)
+    lin = FP8Linear(w, s, device="cpu")
+    other = FP8Linear(w, s, device="cpu").to("meta")
+    assert other.weight.is_meta and other.weight.dtype == torch.float8_e4m3fn and other.weight_scale_inv.is_meta
+    other = other.to_empty(device="cpu")
+    other.load_state_dict(lin.state_dict())
+    assert torch.equal(other.weight.view(torch.uint8), w.view(torch.uint8)) and torch.equal(other.weight_scale_inv, s)

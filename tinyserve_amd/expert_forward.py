@@ -36,6 +36,7 @@ import torch.nn.functional as F
 
 from . import _lib, ops
 from .expert_store import TensorLayout
+from .fp8 import FP8Module
 
 # sigmoid(1.702 x) ~ GELU(x): GPT-OSS SwiGLU coefficient (tinyserve/expert_forward.py:30).
 _QUICK_GELU_COEFF = 1.702
@@ -287,7 +288,7 @@ class GGUFExpertModule(nn.Module):
         return ops.gguf_matvec(act, self.down.reshape(-1), self._types["down"], H, I)
 
 
-class FP8ExpertModule(nn.Module):
+class FP8ExpertModule(FP8Module):
     """An FP8 expert whose parameters are the slot's tensors (the names and shapes of an FP8 slot:
     ``gate_proj``, ``up_proj``, ``down_proj`` and their ``_scale_inv``), for forward_from_packed /
     swap_weights_and_forward; the forward is the fused kernels' layer in three FP8 linears: gate and up in

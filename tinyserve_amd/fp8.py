@@ -18,8 +18,27 @@ from . import ops
 logger = logging.getLogger(__name__)
 
 
-class FP8Linear(nn.Module):
-    """y = deq(fp8_quantize(x)) @ deq(weight)^T + bias, in x's dtype; in_features a multiple of 16."""
+class FP8Module(nn.Module):
+    """A module whose e4m3 parameters and block scales (``*_scale_inv``) keep their types when the model around
+    it is cast (``.to(dtype)``, ``.half()``, ``.type(dtype)``): they are a format, not values of some precision."""
+
+    def _apply(self, fn, recurse=True):
+        fixed = {id(p) for n, p in self._parameters.items()
+                 if p is not None and (p.dtype == torch.float8_e4m3fn or n.endswith("_scale_inv"))}
+
+        def keep(t):
+            if id(t) not in fixed:
+                return fn(t)
+            raw = t.detach().view(torch.uint8 if t.element_size() == 1 else torch.int32)  # casts leave integers alone
+            out = fn(raw)
+            return (out if out.dtype == raw.dtype else raw.to(out.device)).view(t.dtype)
+
+        return super()._apply(keep, recurse)
+
+
+class FP8Linear(FP8Module):
+    """y = deq(fp8_quantize(x)) @ deq(weight)^T + bias, in x's dtype; in_features a multiple of 16. Casting
+    the model leaves codes and scales as they are."""
 
     def __init__(self, weight: torch.Tensor, weight_scale_inv: torch.Tensor, bias: torch.Tensor | None = None,
                  device: torch.device | str = "cuda"):
