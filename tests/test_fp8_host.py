@@ -209,3 +209,15 @@ def test_module_moves_and_loads():
     other = other.to_empty(device="cpu")
     other.load_state_dict(lin.state_dict())
     assert torch.equal(other.weight.view(torch.uint8), w.view(torch.uint8)) and torch.equal(other.weight_scale_inv, s)
+
+
+@pytest.mark.parametrize("H,I,k,E", [(2048, 768, 8, 128), (2880, 2880, 4, 32), (64, 16384, 16, 20)])
+def test_prompt_workspace(lib, H, I, k, E):
+    """The workspace of a prompt stops growing where it is worked through in pieces (131072 assignments), and a
+    workspace for more tokens serves fewer."""
+    L, n, got = fp8_expert_layout(synth.fp8_layout(H, I)), ctypes.c_int64(), []
+    for T in (1, 2, 4, 5, 6, 64, 1024, 131072 // k, 131072, 1 << 20, 1 << 24):
+        assert lib.tsa_moe_prefill_workspace_size(ctypes.byref(L), T, k, E, ctypes.byref(n)) == 0
+        got.append(n.value)
+    assert got == sorted(got) and got[7] == got[-1]
+    assert got[-1] < 131072 * (5 * H + 2 * I) + (1 << 20)

@@ -598,7 +598,7 @@ int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, 
 // Calls that the grouped kernels take (us of a layer grouped / as pairs: hidden 2048, 128 experts top-8, 5 / 8 /
 // 24 tokens 36 / 38 / 52 and 42 / 59 / 153; hidden 2880, 32 experts top-4, 5 / 8 tokens 74 / 76 and 98 / 142).
 bool f8_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
-    return L.format == TSA_EXPERT_FP8 && T > 4 && E <= MAX_GROUP_E && k <= 64;
+    return L.format == TSA_EXPERT_FP8 && T > F8_PAIR_TOKENS && E <= MAX_GROUP_E && k <= 64;
 }
 
 int64_t f8_group_workspace_bytes(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {

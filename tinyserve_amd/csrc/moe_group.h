@@ -10,6 +10,7 @@ constexpr int GROUP_THREADS = 512;
 constexpr int GROUP_WAVES = GROUP_THREADS / 64;
 constexpr int MAX_GROUP_E = 1024;
 constexpr int GROUP_AHEAD = 8;  // id batches loaded ahead per wave
+constexpr int F8_PAIR_TOKENS = 4;  // FP8 experts: calls of more tokens are grouped
 
 // Optional tile table (the grouped GGUF GEMMs' work list): per resident expert in id order,
 // entries of up to `rows` sorted rows {slot, first sorted row, rows, 0}; n_entries[0] = their

@@ -86,11 +86,14 @@ static int64_t chunked_ws(const tsa_expert_layout& L, int64_t T, int k) {
 // other call runs the decode kernels over chunks of tokens. The workspace covers the
 // largest form the layout can take (the x dtype is not known here).
 static int64_t prefill_ws(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
-    const int64_t c = chunked_ws(L, T, k);
+    // FP8 pools are grouped whatever x's type, but for the few tokens that f8_group_supported leaves (no
+    // fewer bytes for more tokens: a workspace serves every call of its size and below)
+    const bool f8 = f8_group_supported(L, T, k, E);
+    const int64_t c = chunked_ws(L, f8 ? F8_PAIR_TOKENS : T, k);
     int64_t g = 0;
     if (L.format == TSA_EXPERT_MXFP4 && L.mx_tiled) g = pf_mxt_workspace_bytes(L, T, k, E);
     if (gf_supported(L, TSA_BF16, T, k)) g = gf_workspace_bytes(L, T, k, E);
-    if (f8_group_supported(L, T, k, E)) g = f8_group_workspace_bytes(L, T, k, E);
+    if (f8) g = f8_group_workspace_bytes(L, T, k, E);
     return g > c ? g : c;
 }
 
