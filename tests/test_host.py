@@ -114,3 +114,60 @@ def test_bench_refuses_more_than_one_gpu():
     r = subprocess.run([sys.executable, os.path.join(ROOT, "bench.py"), "--gpus", "2"], capture_output=True,
                        text=True, timeout=300)
     assert r.returncode == 2 and "one GPU" in r.stderr
+
+
+def test_every_call_is_made_on_its_tensors_device(monkeypatch):
+    """Each entry point calls the library with the device of its tensors current, on that device's stream
+    (kernels are launched on the current device, whichever stream handle they get)."""
+    import contextlib
+
+    from tinyserve_amd import _lib, ops
+    from tinyserve_amd.synth import fp8_layout
+    from tinyserve_amd.expert_forward import fp8_expert_layout
+
+    inside, called = [], []
+
+    class Lib:
+        def __getattr__(self, name):
+            def fn(*args):
+                if not name.endswith("_size") and not name.endswith("_sizes"):
+                    assert inside and args[-1] == 41, name
+                    called.append(name)
+                return 0
+            return fn
+
+    @contextlib.contextmanager
+    def device(d):
+        assert d == -1  # get_device() of the tensors here
+        inside.append(d)
+        yield
+        inside.pop()
+
+    monkeypatch.setattr(_lib, "load", Lib)
+    monkeypatch.setattr(_lib, "device_index", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(_lib, "require_device", lambda *a, **k: None)
+    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda t: 41)
+    x, u8 = torch.zeros(2, 64), torch.zeros(1 << 16, dtype=torch.uint8)
+    w8, s8 = torch.zeros((3, 64), dtype=torch.uint8), torch.zeros((1, 1))
+    blocks, scales = torch.zeros((3, 2, 16), dtype=torch.uint8), torch.zeros((3, 2), dtype=torch.uint8)
+    L = fp8_expert_layout(fp8_layout(64, 32))
+    idx, w, slot = torch.zeros((2, 1), dtype=torch.int32), torch.ones((2, 1)), torch.zeros(1, dtype=torch.int32)
+    ops.gguf_dequant(u8[:34], 8, (32,))
+    ops.gguf_matvec(x, u8[: 3 * 68], 8, 3, 64)
+    ops.mxfp4_dequant(blocks, scales)
+    ops.mxfp4_tile(blocks, scales)
+    ops.mxfp4_matvec(x, blocks, scales)
+    ops.fp8_quantize(x)
+    ops.fp8_matmul(w8, torch.zeros((3, 1)), w8, s8)
+    ops.fp8_linear(x, w8, s8)
+    ops._fp8_linear_workspace_size.cache_clear()
+    ops.route_topk(x, 2)
+    ops.router_logits(x, x)
+    ops.moe_decode(L, u8, idx, w, x)
+    ops.moe_decode_routed(L, u8, slot, w, x, 1)
+    ops.group_by_expert(idx, 1)
+    ops.moe_prefill(L, u8, slot, idx, w, x)
+    ops.decode_workspace_poisoned(u8)
+    assert not inside and len(called) == len(set(called)) == 15

@@ -5,7 +5,6 @@ Loading fails loudly: there is no fallback implementation behind these calls.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -147,15 +146,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-_HERE = contextlib.nullcontext()
-_device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # the first is not a public name
-
-
-def on_device(t: torch.Tensor):
-    """A context with the GPU tensor's device current (kernels are launched on the current device);
-    nothing to do where it is already."""
-    d = t.get_device()
-    return _HERE if d == _device_index() else torch.cuda.device(d)
+device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # the first is not a public name
 
 
 def require_device(*tensors: torch.Tensor, what: str = "tensor") -> None:

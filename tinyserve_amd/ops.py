@@ -24,6 +24,19 @@ def _rows(x: torch.Tensor, K: int) -> torch.Tensor:
     return x.reshape(-1, K).contiguous()
 
 
+def _call(t: torch.Tensor, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of t's device, with that device current (kernels are launched on the
+    current device). The context only where it changes something: it costs 1 us of a 7 us call."""
+    d = t.get_device()
+    if d == _lib.device_index():
+        rc = fn(*args, _stream(t))
+    else:
+        with torch.cuda.device(d):
+            rc = fn(*args, _stream(t))
+    if rc:
+        _lib.check(rc)
+
+
 # ----------------------------------------------------------------------------- GGUF
 def gguf_block_info(ggml_type: int) -> tuple[int, int]:
     be, ts = ctypes.c_int64(), ctypes.c_int64()
@@ -42,8 +55,8 @@ def gguf_dequant(data: torch.Tensor, ggml_type: int, shape, dtype: torch.dtype =
     for s in shape:
         n *= s
     out = torch.empty(shape, dtype=dtype, device=data.device)
-    _lib.check(_lib.load().tsa_gguf_dequant(int(ggml_type), data.data_ptr(), data.numel(), n, out.data_ptr(),
-                                            _lib.tsa_dtype(dtype), _stream(data)))
+    _call(data, _lib.load().tsa_gguf_dequant, int(ggml_type), data.data_ptr(), data.numel(), n, out.data_ptr(),
+          _lib.tsa_dtype(dtype))
     return out
 
 
@@ -59,9 +72,8 @@ def gguf_matvec(x: torch.Tensor, w: torch.Tensor, ggml_type: int, out_features: 
     T = x2.shape[0]
     y = x.new_empty((T, N), dtype=out_dtype or x.dtype)
     w = w.contiguous()
-    _lib.check(_lib.load().tsa_gguf_matvec(int(ggml_type), w.data_ptr(), w.numel(), x2.data_ptr(),
-                                           _lib.tsa_dtype(x2.dtype), T, K, y.data_ptr(), _lib.tsa_dtype(y.dtype), N,
-                                           _stream(x)))
+    _call(x2, _lib.load().tsa_gguf_matvec, int(ggml_type), w.data_ptr(), w.numel(), x2.data_ptr(),
+          _lib.tsa_dtype(x2.dtype), T, K, y.data_ptr(), _lib.tsa_dtype(y.dtype), N)
     return y
 
 
@@ -79,8 +91,8 @@ def mxfp4_dequant(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype
         out = torch.empty(shape, dtype=dtype, device=blocks.device)
     elif not out.is_contiguous() or out.numel() != N * K or out.dtype != dtype:
         raise ValueError("out must be a contiguous tensor of N*K elements of the requested dtype")
-    _lib.check(_lib.load().tsa_mxfp4_dequant(blocks.data_ptr(), scales.data_ptr(), N, K, out.data_ptr(),
-                                             _lib.tsa_dtype(dtype), int(transpose), _stream(blocks)))
+    _call(blocks, _lib.load().tsa_mxfp4_dequant, blocks.data_ptr(), scales.data_ptr(), N, K, out.data_ptr(),
+          _lib.tsa_dtype(dtype), int(transpose))
     return out.view(shape)
 
 
@@ -106,8 +118,8 @@ def mxfp4_tile(blocks: torch.Tensor, scales: torch.Tensor, out_blocks: torch.Ten
         out_scales = torch.empty(sb, dtype=torch.uint8, device=blocks.device)
     if out_blocks.numel() * out_blocks.element_size() < bb or out_scales.numel() * out_scales.element_size() < sb:
         raise ValueError(f"outputs too small: need {bb} and {sb} bytes")
-    _lib.check(_lib.load().tsa_mxfp4_tile(blocks.data_ptr(), scales.data_ptr(), N, K, out_blocks.data_ptr(),
-                                          out_scales.data_ptr(), _stream(blocks)))
+    _call(blocks, _lib.load().tsa_mxfp4_tile, blocks.data_ptr(), scales.data_ptr(), N, K, out_blocks.data_ptr(),
+          out_scales.data_ptr())
     return out_blocks, out_scales
 
 
@@ -122,10 +134,9 @@ def mxfp4_matvec(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
     y = x.new_empty((T, N), dtype=out_dtype or x.dtype)
     blocks, scales = blocks.contiguous(), scales.contiguous()
     b = None if bias is None else bias.contiguous()
-    _lib.check(_lib.load().tsa_mxfp4_matvec(blocks.data_ptr(), scales.data_ptr(), _lib.ptr(b),
-                                            _lib.tsa_dtype(b.dtype) if b is not None else 0, x2.data_ptr(),
-                                            _lib.tsa_dtype(x2.dtype), T, y.data_ptr(), _lib.tsa_dtype(y.dtype), N, K,
-                                            _stream(x)))
+    _call(x2, _lib.load().tsa_mxfp4_matvec, blocks.data_ptr(), scales.data_ptr(), _lib.ptr(b),
+          _lib.tsa_dtype(b.dtype) if b is not None else 0, x2.data_ptr(), _lib.tsa_dtype(x2.dtype), T, y.data_ptr(),
+          _lib.tsa_dtype(y.dtype), N, K)
     return y
 
 
@@ -138,18 +149,6 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t with contiguous memory from a multiple of 16 bytes on (a copy if it is not there already)."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _call(t: torch.Tensor, fn, *args) -> None:
-    """fn(*args, stream) with t's device current, on that device's current stream."""
-    ctx = _lib.on_device(t)
-    if ctx is _lib._HERE:  # without the context: 1 us of a 7 us call
-        rc = fn(*args, _stream(t))
-    else:
-        with ctx:
-            rc = fn(*args, _stream(t))
-    if rc:
-        _lib.check(rc)
 
 
 def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -257,8 +256,8 @@ def route_topk(logits: torch.Tensor, top_k: int, mode: str = "topk_then_softmax"
     T, E = lg.shape
     idx = torch.empty((T, top_k), dtype=torch.int32, device=lg.device)
     w = torch.empty((T, top_k), dtype=torch.float32, device=lg.device)
-    _lib.check(_lib.load().tsa_route_topk(lg.data_ptr(), _lib.tsa_dtype(lg.dtype), T, E, int(top_k),
-                                          ROUTE_MODES[mode], idx.data_ptr(), w.data_ptr(), _stream(lg)))
+    _call(lg, _lib.load().tsa_route_topk, lg.data_ptr(), _lib.tsa_dtype(lg.dtype), T, E, int(top_k), ROUTE_MODES[mode],
+          idx.data_ptr(), w.data_ptr())
     return idx, w
 
 
@@ -273,9 +272,9 @@ def router_logits(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     w = weight.contiguous()
     b = bias.contiguous() if bias is not None else None
     out = x.new_empty((x2.shape[0], E), dtype=out_dtype or weight.dtype)
-    _lib.check(_lib.load().tsa_router_logits(
-        x2.data_ptr(), _lib.tsa_dtype(x2.dtype), x2.shape[0], H, w.data_ptr(), _lib.tsa_dtype(w.dtype), _lib.ptr(b),
-        _lib.tsa_dtype(b.dtype) if b is not None else 0, E, out.data_ptr(), _lib.tsa_dtype(out.dtype), _stream(x)))
+    _call(x2, _lib.load().tsa_router_logits, x2.data_ptr(), _lib.tsa_dtype(x2.dtype), x2.shape[0], H, w.data_ptr(),
+          _lib.tsa_dtype(w.dtype), _lib.ptr(b), _lib.tsa_dtype(b.dtype) if b is not None else 0, E, out.data_ptr(),
+          _lib.tsa_dtype(out.dtype))
     return out
 
 
@@ -320,8 +319,7 @@ def set_decode_options(tiled_form: int = 1, wait_limit: int = 1 << 18) -> None:
 def decode_workspace_poisoned(workspace: torch.Tensor) -> bool:
     """True if a one-launch wait gave up on this workspace (synchronises the current stream)."""
     out = ctypes.c_int()
-    _lib.check(_lib.load().tsa_moe_decode_workspace_status(workspace.data_ptr(), workspace.numel(), ctypes.byref(out),
-                                                           _lib.stream_handle(workspace.device)))
+    _call(workspace, _lib.load().tsa_moe_decode_workspace_status, workspace.data_ptr(), workspace.numel(), ctypes.byref(out))
     return bool(out.value)
 
 
@@ -341,11 +339,9 @@ def moe_decode(layout: _lib.ExpertLayout, pool: torch.Tensor, slots: torch.Tenso
         out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
     if workspace is None:
         workspace = moe_decode_workspace(layout, T, k, x.device)
-    with _lib.on_device(x2):
-        _lib.check(_lib.load().tsa_moe_decode(ctypes.byref(layout), pool.data_ptr(), n_slots, slots.data_ptr(),
-                                              weights.data_ptr(), T, k, x2.data_ptr(), _lib.tsa_dtype(x2.dtype),
-                                              out.data_ptr(), _lib.tsa_dtype(out.dtype), workspace.data_ptr(),
-                                              workspace.numel(), _stream(x)))
+    _call(x2, _lib.load().tsa_moe_decode, ctypes.byref(layout), pool.data_ptr(), n_slots, slots.data_ptr(),
+          weights.data_ptr(), T, k, x2.data_ptr(), _lib.tsa_dtype(x2.dtype), out.data_ptr(), _lib.tsa_dtype(out.dtype),
+          workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -367,12 +363,10 @@ def moe_decode_routed(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot
         workspace = moe_decode_workspace(layout, T, top_k, x.device)
     idx = torch.empty((T, top_k), dtype=torch.int32, device=x.device) if return_routing else None
     w = torch.empty((T, top_k), dtype=torch.float32, device=x.device) if return_routing else None
-    with _lib.on_device(x2):
-        _lib.check(_lib.load().tsa_moe_decode_routed(
-            ctypes.byref(layout), pool.data_ptr(), _n_slots(pool, layout), expert_slot.data_ptr(), E, lg.data_ptr(),
-            _lib.tsa_dtype(lg.dtype), ROUTE_MODES[mode], T, int(top_k), x2.data_ptr(), _lib.tsa_dtype(x2.dtype),
-            out.data_ptr(), _lib.tsa_dtype(out.dtype), _lib.ptr(idx), _lib.ptr(w), workspace.data_ptr(), workspace.numel(),
-            _stream(x)))
+    _call(x2, _lib.load().tsa_moe_decode_routed, ctypes.byref(layout), pool.data_ptr(), _n_slots(pool, layout),
+          expert_slot.data_ptr(), E, lg.data_ptr(), _lib.tsa_dtype(lg.dtype), ROUTE_MODES[mode], T, int(top_k), x2.data_ptr(),
+          _lib.tsa_dtype(x2.dtype), out.data_ptr(), _lib.tsa_dtype(out.dtype), _lib.ptr(idx), _lib.ptr(w),
+          workspace.data_ptr(), workspace.numel())
     return (out, idx, w) if return_routing else out
 
 
@@ -393,8 +387,8 @@ def group_by_expert(idx: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, 
     counts = torch.empty(num_experts, dtype=torch.int32, device=idx.device)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=idx.device)
     perm = torch.empty(max(T * k, 1), dtype=torch.int32, device=idx.device)
-    _lib.check(_lib.load().tsa_group_by_expert(idx2.data_ptr(), T, k, int(num_experts), counts.data_ptr(),
-                                               offsets.data_ptr(), perm.data_ptr(), _stream(idx)))
+    _call(idx2, _lib.load().tsa_group_by_expert, idx2.data_ptr(), T, k, int(num_experts), counts.data_ptr(),
+          offsets.data_ptr(), perm.data_ptr())
     return counts, offsets, perm[: T * k]
 
 
@@ -422,9 +416,7 @@ def moe_prefill(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot: torc
         out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
     if workspace is None:
         workspace = moe_prefill_workspace(layout, T, k, E, x.device)
-    with _lib.on_device(x2):
-        _lib.check(_lib.load().tsa_moe_prefill(ctypes.byref(layout), pool.data_ptr(), n_slots, expert_slot.data_ptr(), E,
-                                               idx.data_ptr(), weights.data_ptr(), T, k, x2.data_ptr(),
-                                               _lib.tsa_dtype(x2.dtype), out.data_ptr(), _lib.tsa_dtype(out.dtype),
-                                               workspace.data_ptr(), workspace.numel(), _stream(x)))
+    _call(x2, _lib.load().tsa_moe_prefill, ctypes.byref(layout), pool.data_ptr(), n_slots, expert_slot.data_ptr(), E,
+          idx.data_ptr(), weights.data_ptr(), T, k, x2.data_ptr(), _lib.tsa_dtype(x2.dtype), out.data_ptr(),
+          _lib.tsa_dtype(out.dtype), workspace.data_ptr(), workspace.numel())
     return out
