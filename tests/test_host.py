@@ -171,3 +171,48 @@ def test_every_call_is_made_on_its_tensors_device(monkeypatch):
     ops.moe_prefill(L, u8, slot, idx, w, x)
     ops.decode_workspace_poisoned(u8)
     assert not inside and len(called) == len(set(called)) == 15
+
+
+def _layer_calls(monkeypatch, called):
+    """The layer calls over FP8 experts (hidden 64, inter 32) on CPU tensors, against a library that only records."""
+    from tinyserve_amd import _lib, ops
+    from tinyserve_amd.synth import fp8_layout
+    from tinyserve_amd.expert_forward import fp8_expert_layout
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *args: 0 if name.endswith("_size") else called.append(name) or 0
+
+    L = fp8_expert_layout(fp8_layout(64, 32))
+    monkeypatch.setattr(_lib, "load", Lib)
+    monkeypatch.setattr(_lib, "device_index", lambda: -1)
+    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda t: 0)
+    pool = torch.zeros(1 << 16, dtype=torch.uint8)
+
+    def calls(T, out=None, weights=2, slots=4):
+        x, idx, w = torch.zeros(T, 64), torch.zeros((T, 2), dtype=torch.int32), torch.ones((T, weights))
+        slot = torch.zeros(slots, dtype=torch.int32)
+        return [lambda: ops.moe_decode(L, pool, idx, w, x, out=out), lambda: ops.moe_prefill(L, pool, slot, idx, w, x, out=out),
+                lambda: ops.moe_decode_routed(L, pool, slot, torch.zeros(T, 4), x, 2, out=out, return_routing=True)[0]]
+
+    return calls
+
+
+def test_layer_calls_refuse_what_they_would_overrun(monkeypatch):
+    """Results that are too small or not contiguous, fewer weights than experts, fewer slots than logits."""
+    called = []
+    calls = _layer_calls(monkeypatch, called)
+    for out in (torch.zeros(2, 64), torch.zeros(3, 128)[:, ::2], torch.zeros(64, 3).t()):
+        for f in calls(3, out=out):
+            with pytest.raises(RuntimeError, match="out must be contiguous"):
+                f()
+    for f in calls(3, weights=1)[:2]:
+        with pytest.raises(RuntimeError, match="weights a token"):
+            f()
+    with pytest.raises(RuntimeError, match="logits of 4 experts"):
+        calls(3, slots=3)[2]()
+    assert not called
+    for f in calls(3, out=torch.zeros(4, 64)):  # the start of a larger buffer is fine
+        f()
+    assert called == ["tsa_moe_decode", "tsa_moe_prefill", "tsa_moe_decode_routed"]

@@ -292,8 +292,17 @@ def _n_slots(pool: torch.Tensor, layout: _lib.ExpertLayout) -> int:
 
 def _moe_rows(layout: _lib.ExpertLayout, x: torch.Tensor) -> torch.Tensor:
     """x as contiguous rows of ``hidden`` values (from a multiple of 16 bytes on for FP8 experts)."""
-    x2 = x.reshape(-1, layout.hidden).contiguous()
+    x2 = _rows(x, layout.hidden)
     return _aligned(x2) if layout.format == _lib.EXPERT_FP8 else x2
+
+
+def _moe_out(out: torch.Tensor | None, x2: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The result of a layer call on rows x2: new, or the caller's, which the kernels fill from its start."""
+    if out is None:
+        return torch.empty(x2.shape, dtype=dtype, device=x2.device)
+    if not out.is_contiguous() or out.numel() < x2.numel():
+        raise RuntimeError(f"out must be contiguous and hold {list(x2.shape)} values, got {list(out.shape)}")
+    return out
 
 
 def moe_decode_workspace_size(layout: _lib.ExpertLayout, T: int, k: int) -> int:
@@ -327,16 +336,16 @@ def moe_decode(layout: _lib.ExpertLayout, pool: torch.Tensor, slots: torch.Tenso
                x: torch.Tensor, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] * FFN_{slots[t, j]}(x[t]) over the resident slot pool."""
-    _lib.require_device(pool, slots, weights, x, what="tensor")
-    H = layout.hidden
+    _one_device(x, pool, slots, weights, out, workspace)
     x2 = _moe_rows(layout, x)
     T = x2.shape[0]
+    n_slots = _n_slots(pool, layout)
+    out = _moe_out(out, x2, out_dtype or x.dtype)
     slots = slots.reshape(T, -1).to(torch.int32).contiguous()
     weights = weights.reshape(T, -1).to(torch.float32).contiguous()
     k = slots.shape[1]
-    n_slots = _n_slots(pool, layout)
-    if out is None:
-        out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
+    if weights.shape[1] != k:
+        raise RuntimeError(f"{k} slots but {weights.shape[1]} weights a token")
     if workspace is None:
         workspace = moe_decode_workspace(layout, T, k, x.device)
     _call(x2, _lib.load().tsa_moe_decode, ctypes.byref(layout), pool.data_ptr(), n_slots, slots.data_ptr(),
@@ -350,19 +359,19 @@ def moe_decode_routed(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot
                       workspace: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
                       return_routing: bool = False):
     """Router top-k + fused expert FFN in one call (a single launch for MXFP4, T <= 4)."""
-    _lib.require_device(pool, expert_slot, logits, x, what="tensor")
-    H = layout.hidden
+    _one_device(x, pool, expert_slot, logits, out, workspace)
     x2 = _moe_rows(layout, x)
     T = x2.shape[0]
+    out = _moe_out(out, x2, out_dtype or x.dtype)
+    idx = torch.empty((T, top_k), dtype=torch.int32, device=x.device) if return_routing else None
+    w = torch.empty((T, top_k), dtype=torch.float32, device=x.device) if return_routing else None
     lg = logits.reshape(T, -1).contiguous()
     E = lg.shape[1]
     expert_slot = expert_slot.to(torch.int32).contiguous()
-    if out is None:
-        out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
+    if expert_slot.numel() < E:
+        raise RuntimeError(f"logits of {E} experts but slots of {expert_slot.numel()}")
     if workspace is None:
         workspace = moe_decode_workspace(layout, T, top_k, x.device)
-    idx = torch.empty((T, top_k), dtype=torch.int32, device=x.device) if return_routing else None
-    w = torch.empty((T, top_k), dtype=torch.float32, device=x.device) if return_routing else None
     _call(x2, _lib.load().tsa_moe_decode_routed, ctypes.byref(layout), pool.data_ptr(), _n_slots(pool, layout),
           expert_slot.data_ptr(), E, lg.data_ptr(), _lib.tsa_dtype(lg.dtype), ROUTE_MODES[mode], T, int(top_k), x2.data_ptr(),
           _lib.tsa_dtype(x2.dtype), out.data_ptr(), _lib.tsa_dtype(out.dtype), _lib.ptr(idx), _lib.ptr(w),
@@ -403,17 +412,17 @@ def moe_prefill(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot: torc
                 weights: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = None,
                 workspace: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Batched (prefill) MoE: out[t] = sum_j weights[t, j] * FFN_{expert_slot[idx[t, j]]}(x[t])."""
-    _lib.require_device(pool, expert_slot, idx, weights, x, what="tensor")
-    H = layout.hidden
+    _one_device(x, pool, expert_slot, idx, weights, out, workspace)
     x2 = _moe_rows(layout, x)
     T = x2.shape[0]
+    n_slots = _n_slots(pool, layout)
+    out = _moe_out(out, x2, out_dtype or x.dtype)
     idx = idx.reshape(T, -1).to(torch.int32).contiguous()
     weights = weights.reshape(T, -1).to(torch.float32).contiguous()
+    if weights.shape != idx.shape:
+        raise RuntimeError(f"{idx.shape[1]} experts but {weights.shape[1]} weights a token")
     expert_slot = expert_slot.to(torch.int32).contiguous()
     k, E = idx.shape[1], expert_slot.numel()
-    n_slots = _n_slots(pool, layout)
-    if out is None:
-        out = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
     if workspace is None:
         workspace = moe_prefill_workspace(layout, T, k, E, x.device)
     _call(x2, _lib.load().tsa_moe_prefill, ctypes.byref(layout), pool.data_ptr(), n_slots, expert_slot.data_ptr(), E,
