@@ -199,6 +199,13 @@ def _layer_calls(monkeypatch, called):
     return calls
 
 
+def test_layer_calls_of_no_tokens(monkeypatch):
+    called = []
+    for f in _layer_calls(monkeypatch, called)(0):
+        assert f().shape == (0, 64)
+    assert not called
+
+
 def test_layer_calls_refuse_what_they_would_overrun(monkeypatch):
     """Results that are too small or not contiguous, fewer weights than experts, fewer slots than logits."""
     called = []

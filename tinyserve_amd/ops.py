@@ -341,6 +341,8 @@ def moe_decode(layout: _lib.ExpertLayout, pool: torch.Tensor, slots: torch.Tenso
     T = x2.shape[0]
     n_slots = _n_slots(pool, layout)
     out = _moe_out(out, x2, out_dtype or x.dtype)
+    if T == 0:
+        return out
     slots = slots.reshape(T, -1).to(torch.int32).contiguous()
     weights = weights.reshape(T, -1).to(torch.float32).contiguous()
     k = slots.shape[1]
@@ -365,6 +367,8 @@ def moe_decode_routed(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot
     out = _moe_out(out, x2, out_dtype or x.dtype)
     idx = torch.empty((T, top_k), dtype=torch.int32, device=x.device) if return_routing else None
     w = torch.empty((T, top_k), dtype=torch.float32, device=x.device) if return_routing else None
+    if T == 0:
+        return (out, idx, w) if return_routing else out
     lg = logits.reshape(T, -1).contiguous()
     E = lg.shape[1]
     expert_slot = expert_slot.to(torch.int32).contiguous()
@@ -417,6 +421,8 @@ def moe_prefill(layout: _lib.ExpertLayout, pool: torch.Tensor, expert_slot: torc
     T = x2.shape[0]
     n_slots = _n_slots(pool, layout)
     out = _moe_out(out, x2, out_dtype or x.dtype)
+    if T == 0:
+        return out
     idx = idx.reshape(T, -1).to(torch.int32).contiguous()
     weights = weights.reshape(T, -1).to(torch.float32).contiguous()
     if weights.shape != idx.shape:
