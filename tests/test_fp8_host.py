@@ -221,3 +221,17 @@ def test_prompt_workspace(lib, H, I, k, E):
         got.append(n.value)
     assert got == sorted(got) and got[7] == got[-1]
     assert got[-1] < 131072 * (5 * H + 2 * I) + (1 << 20)
+
+
+@pytest.mark.parametrize("E,H,I", [(3, 64, 32), (1, 64, 32), (2, 32, 64), (2, 64, 64)])
+def test_store_layers_differ(tmp_path, E, H, I):
+    """A layer with more or fewer experts than the first, or others' sizes, is refused (its rest was dropped)."""
+    from safetensors.torch import load_file, save_file
+
+    (tmp_path / "b").mkdir()
+    _save(tmp_path, np.random.default_rng(1), (0,), 2, 64, 32)
+    _save(tmp_path / "b", np.random.default_rng(2), (1,), E, H, I)
+    both = {**load_file(str(tmp_path / "model.safetensors")), **load_file(str(tmp_path / "b" / "model.safetensors"))}
+    save_file(both, str(tmp_path / "model.safetensors"))
+    with pytest.raises(ValueError, match="layer 1"):
+        ExpertStore.from_safetensors(str(tmp_path))

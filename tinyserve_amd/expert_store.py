@@ -167,6 +167,7 @@ class ExpertStore:
         first = layer_tensors[layers[0]]
         num_experts = int(next(iter(first.values())).shape[0])
         specs = {n: (tuple(t.shape[1:]), t.dtype) for n, t in first.items()}
+        shapes = {n: (tuple(t.shape), t.dtype) for n, t in first.items()}
         if tiled:
             specs = mxfp4_tiled_specs(specs)
         layout = TensorLayout(specs, align=16 if fp8 else 1)
@@ -177,6 +178,10 @@ class ExpertStore:
             tensors = layer_tensors[li]
             if set(tensors) != set(specs):
                 raise ValueError(f"layer {li}: expert tensors {sorted(tensors)} differ from {sorted(specs)}")
+            for n, t in tensors.items():
+                if (tuple(t.shape), t.dtype) != shapes[n]:
+                    raise ValueError(f"layer {li}: {n} is {t.dtype} {list(t.shape)}, in layer {layers[0]} "
+                                     f"{shapes[n][1]} {list(shapes[n][0])}")
             for e in range(num_experts):
                 parts = {n: t[e].contiguous() for n, t in tensors.items()}
                 if tiled:
