@@ -867,3 +867,17 @@ def test_matmul_past_2_27_rows(T, dtype):
         want, err = ref.matmul(q, s, w[r], ws[n // 128 :][: ref.blocks(r.stop - n)], wide=dtype == F32)
         bias = b[r].double()
         ref.check(y[:, r], want + bias, err + (bias.abs() + want.abs()) * 2.0**-23)
+
+
+@pytest.mark.parametrize("T", [1, 9, 150])
+def test_moe_largest_experts_past_four_gib(T):
+    """The largest hidden and inter, in a pool whose last slot starts past 2^32 bytes."""
+    H = I = 16384
+    ex = experts(1, 1, H, I)
+    L, pool = pool_of(ex, H, I, [6])
+    assert 6 * pool.shape[1] > 1 << 32
+    x, slot = acts(T, T, H), torch.full((1,), 6, dtype=torch.int32, device=DEV)
+    zero, w = torch.zeros((T, 1), dtype=torch.int32, device=DEV), torch.rand((T, 1), device=DEV, generator=gen(T))
+    want, err = ref.moe(x, zero, w, ex)
+    ref.check(ops.moe_prefill(L, pool, slot, zero, w, x), want, err, "prefill")
+    ref.check(ops.moe_decode(L, pool, slot[zero.long()], w, x), want, err, "decode")
