@@ -434,7 +434,11 @@ extern "C" int tsa_fp8_matmul(const void* codes, const float* scales, int64_t T,
     return TSA_OK;
 }
 
-// Whether few enough tokens are quantised inside the product's launch.
+// Whether few enough tokens are quantised inside the product's launch: the second launch costs a call that is
+// made by itself about 4 us of host time, while every token here adds a load latency to every workgroup. us of
+// one launch / two, 2880 x 2880 and 2048 x 4096: calls one by one, 8 tokens 7.4 / 11.2 and 8.2 / 11.6, 16 tokens
+// 11.2 / 11.2 and 12.1 / 11.6; inside a graph, 4 tokens 5.3 / 5.9 and 6.1 / 7.3, 8 tokens 7.3 / 6.0 and 8.1 / 7.7,
+// 16 tokens 11.4 / 6.5 and 12.2 / 9.0. (The limit is the calls' one by one; a graph's is 4 to 8.)
 static bool linear_in_one(int64_t T, int64_t K) { return T <= 16 && f8r_lds(0, 1, (int)f8_blocks(K), (int)T) <= 128 * 1024; }
 static int64_t linear_ws(int64_t T, int64_t K) {
     return linear_in_one(T, K) ? 0 : (T * K + 255) / 256 * 256 + T * f8_blocks(K) * 4;

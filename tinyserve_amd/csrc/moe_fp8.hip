@@ -14,7 +14,9 @@
 // instructions by 0.0018 to 0.0032. us, float32 accuracy / FP8 instructions: hidden 2880, 32 experts top-4,
 // 8 layers of 4 tokens 632 / 613, a layer of 2048 570 / 490; hidden 2048, 128 experts top-8, 24 tokens 58 / 57,
 // 1024 tokens 210 / 187. Down is summed so where the layer's result is float32; for 16-bit ones the FP8
-// instructions' sums are far below the last rounding.
+// instructions' sums are far below the last rounding. A layer's us for float32 / bf16 results: hidden 2880, 32
+// experts top-4, 4 and 2048 tokens 74 / 71 and 605 / 568; hidden 2048, 128 experts top-8, 1, 24 and 1024 tokens
+// 15.7 / 15.3, 48.5 / 47.0 and 220 / 208.
 #include "fp8_gemm.h"
 #include "moe_group.h"
 
@@ -57,7 +59,8 @@ __device__ __forceinline__ float f8_act(const tsa_expert_layout& L, float gate, 
 
 // One workgroup per (token, expert) pair and 8 channels: rows 0 .. 7 of the tile are the channels' gate
 // rows, 8 .. 15 their up rows, so one pair gives enough workgroups (768 at inter 768 and top-8, three
-// whole rounds of the CUs; tiles of 16 channels give 384, one and a half: 9.5 us against 7.7). Loads
+// whole rounds of the CUs; tiles of 16 channels give 384, one and a half: 9.5 us against 7.7, both with the
+// FP8 instructions; 8.1 with the widened products). Loads
 // go out in the order of their use: x, the routing's inputs, then every weight of the tile; x is
 // quantised while the weights are on their way.
 template <int XT>
