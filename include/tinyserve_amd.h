@@ -168,6 +168,51 @@ int tsa_fp8_linear(const void* x, int x_dtype, int64_t T, int64_t K, const void*
                    const void* bias, int bias_dtype, void* y, int y_dtype, void* workspace, int64_t workspace_bytes,
                    void* stream);
 
+/* ---- int8 with a float32 scale for each token and each weight row (no reference counterpart). A weight
+ * matrix w [N, K] is int8 codes and scales [N]. ---- */
+
+/* Quantise x [T, K] (any K): per token
+ *   scale = max(max|x| / 127, 2^-126),  code = round(x / scale)
+ * with both quotients rounded to float32 and codes to the nearest, ties to even. codes [T, K] int8,
+ * scales [T]. A token that holds a NaN or an infinity has NaN as its scale and zeros as its codes. T at most 2^30. */
+int tsa_int8_quantize(const void* x, int x_dtype, int64_t T, int64_t K, void* codes, float* scales, void* stream);
+
+/* y[t, n] = scales[t] w_scales[n] sum_k codes[t, k] w[n, k] (+ bias[n], may be NULL): the sum is exact, one
+ * rounding to float32, the scales and the bias in float32, one rounding to y_dtype. K a multiple of 16 of at
+ * most 131056 (the sums fit 32 bits), T and N at most 2^30 (products of more than 32 tokens that no launch covers,
+ * from about 2^37 results on, are refused); codes and w 16-byte aligned. */
+int tsa_int8_matmul(const void* codes, const float* scales, int64_t T, int64_t K, const void* w, const float* w_scales,
+                    int64_t N, const void* bias, int bias_dtype, void* y, int y_dtype, void* stream);
+
+/* Workspace bytes of tsa_int8_linear (16-byte aligned, no initialisation); 0 for few tokens. */
+int tsa_int8_linear_workspace_size(int64_t T, int64_t K, int64_t* bytes);
+
+/* tsa_int8_quantize of x [T, K] followed by tsa_int8_matmul; few tokens are quantised inside the
+ * product's launch. x and w 16-byte aligned. */
+int tsa_int8_linear(const void* x, int x_dtype, int64_t T, int64_t K, const void* w, const float* w_scales, int64_t N,
+                    const void* bias, int bias_dtype, void* y, int y_dtype, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* ---- products grouped by expert ---- */
+
+/* y[r, n] = sum_k x[a, k] w[e, n, k] (+ bias[e, n], may be NULL) for the expert e with offsets[e] <= r <
+ * offsets[e + 1], r < R: rows sorted by expert, any number of them for each, as tsa_group_by_expert's offsets [E + 1]
+ * (ascending in [0, R]) have them. a = r, or rows[r] / top_k where rows [R] is given (tsa_group_by_expert's perm); an a
+ * outside [0, x_rows) reads a row of zeros. Rows of no expert are set to zero, and their entry of `rows` is not used.
+ * x [x_rows, K] and w in dtype (BF16 or F16), w + e w_stride bytes [N, K]; float32 sums, one rounding to y_dtype; y [R, N],
+ * bias [E, N]. K a multiple of 8 of at most 131056; x and w 16-byte aligned, w_stride a multiple of 16; x
+ * below 2^31 bytes where rows is given; E at most 65536, N at most 2^24, R below 2^30 and (R / 16 + E + 2) ceil(N / 64)
+ * below 2^23. Replaces the per-expert loops over unquantised experts (tinyserve/expert_pipeline.py:287-337). */
+int tsa_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t K, const void* w, int64_t w_stride, int64_t E,
+                       int64_t N, const int32_t* offsets, const int32_t* rows, int64_t R, int top_k, const void* bias,
+                       int bias_dtype, void* y, int y_dtype, void* stream);
+
+/* The same for int8 codes [x_rows, K] with scales [x_rows], and w codes with w_scales [E, N]; sums as
+ * tsa_int8_matmul's. K a multiple of 16. */
+int tsa_int8_grouped_matmul(const void* codes, const float* scales, int64_t x_rows, int64_t K, const void* w, int64_t w_stride,
+                            const float* w_scales, int64_t E, int64_t N, const int32_t* offsets, const int32_t* rows, int64_t R,
+                            int top_k, const void* bias, int bias_dtype, void* y, int y_dtype, void* stream);
+
 /* Router top-k over logits [T, E] (logits_dtype F32/BF16/F16): idx [T, k] int32 and
  * weights [T, k] f32, descending, ties to the lower expert id.
  * Replaces the route closures of _extract_routing_fn (tinyserve/_model_hooks.py:424-476). */

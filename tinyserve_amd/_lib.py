@@ -78,6 +78,13 @@ SIGNATURES = {
     "tsa_fp8_matmul": (_I32, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I32, _P]),
     "tsa_fp8_linear_workspace_size": (_I32, [_I64, _I64, ctypes.POINTER(_I64)]),
     "tsa_fp8_linear": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _P]),
+    "tsa_int8_quantize": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P]),
+    "tsa_int8_matmul": (_I32, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I32, _P]),
+    "tsa_int8_linear_workspace_size": (_I32, [_I64, _I64, ctypes.POINTER(_I64)]),
+    "tsa_int8_linear": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _P]),
+    "tsa_grouped_matmul": (_I32, [_P, _I32, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _P, _I32, _P, _I32, _P]),
+    "tsa_int8_grouped_matmul": (_I32, [_P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _I32, _P, _I32,
+                                       _P]),
     "tsa_route_topk": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P]),
     "tsa_router_logits": (_I32, [_P, _I32, _I64, _I64, _P, _I32, _P, _I32, _I64, _P, _I32, _P]),
     "tsa_moe_decode_workspace_size": (_I32, [_LP, _I64, _I32, ctypes.POINTER(_I64)]),

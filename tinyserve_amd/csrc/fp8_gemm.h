@@ -11,35 +11,10 @@
 #pragma once
 
 #include "fp8_common.h"
+#include "lds_copy.h"
 
 namespace tsa {
 namespace {
-
-typedef int f8_v4i __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ f8_v4i f8_desc(const void* p, uint32_t bytes) {
-    const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return f8_v4i{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)),
-                  __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
-}
-
-// Lane l's 16 (or 4) bytes at buffer offset voff + soff land at LDS byte lds + 16 l (or 4 l).
-__device__ __forceinline__ void f8_copy16(const f8_v4i& r, uint32_t voff, uint32_t soff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %3\n\t" TSA_COPY_WAIT "buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff),
-                 "s"(__builtin_amdgcn_readfirstlane((int)lds))
-                 : "memory", "m0");
-}
-__device__ __forceinline__ void f8_copy4(const f8_v4i& r, uint32_t voff, uint32_t soff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %3\n\t" TSA_COPY_WAIT "buffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff),
-                 "s"(__builtin_amdgcn_readfirstlane((int)lds))
-                 : "memory", "m0");
-}
-
-// This wave's copies have landed but for the newest N, and its LDS reads are done; then the barrier.
-template <int N>
-__device__ __forceinline__ void f8_wait_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
 
 // WR x WT waves of MR x MT tiles of 16 x 16, S stages.
 template <int WR_, int WT_, int MR_, int MT_, int S_>
@@ -79,10 +54,10 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
     const int steps = p.G;
 
     // copy j of this wave fills rows 8 (NX wave + j) + lane / 8, slot lane % 8
-    f8_v4i rw[PARTS];
+    buf_v4i rw[PARTS];
 #pragma unroll
-    for (int h = 0; h < PARTS; ++h) rw[h] = f8_desc(p.w[h], (uint32_t)(p.w_rows < HALF ? p.w_rows : HALF) * K);
-    const f8_v4i rx = f8_desc(p.x, p.x_records), rs = f8_desc(p.xs, p.xs_records);
+    for (int h = 0; h < PARTS; ++h) rw[h] = buf_desc(p.w[h], (uint32_t)(p.w_rows < HALF ? p.w_rows : HALF) * K);
+    const buf_v4i rx = buf_desc(p.x, p.x_records), rs = buf_desc(p.xs, p.xs_records);
     uint32_t wo[C::NXW], xo[C::NXT];
     auto chunk = [&](int n) { return (uint32_t)((lane & 7) ^ ((4 * n + (lane >> 4)) & 7)); };  // of copy n's rows
 #pragma unroll
@@ -113,13 +88,13 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
         if (j < C::NXW) {
             const int n = C::NXW * wave + j;
             const bool in = col + (n & 1 ? at[1] : at[0]) < K;
-            f8_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], in ? wo[j] : 0x80000000u, soff, base + 1024u * (uint32_t)n);
+            lds_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], in ? wo[j] : 0x80000000u, soff, base + 1024u * (uint32_t)n);
         } else if (j < C::NXW + C::NXT) {
             const int n = C::NXT * wave + j - C::NXW;
             const bool in = col + (n & 1 ? at[1] : at[0]) < K;
-            f8_copy16(rx, in ? xo[j - C::NXW] : 0x80000000u, soff, base + (uint32_t)C::RN * F8B + 1024u * (uint32_t)n);
+            lds_copy16(rx, in ? xo[j - C::NXW] : 0x80000000u, soff, base + (uint32_t)C::RN * F8B + 1024u * (uint32_t)n);
         } else {
-            f8_copy4(rs, s < steps ? so : 0x80000000u, soff / 32,
+            lds_copy4(rs, s < steps ? so : 0x80000000u, soff / 32,
                      lds0 + (uint32_t)(S * C::STAGE) + 256u * (uint32_t)(C::NW * stage + wave));
         }
     };
@@ -197,7 +172,7 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
         for (int s = 0; s < steps; ++s) {
             if ((s & 63) == 0 && s) load_ws(s);
             // block s has landed (every wave's part of it), and the stage read in step s - 1 is free
-            f8_wait_barrier<(S - 2) * C::PER>();
+            wait_copies_barrier<(S - 2) * C::PER>();
             const uint8_t* wl = smem + stage * C::STAGE;
             if (LIVE) read(row_tile(wl, 0), A[0]);
             fetch_b(wl);
@@ -212,7 +187,7 @@ __device__ __forceinline__ void f8_tile(const F8Operands<PARTS>& p, uint8_t* sme
     else if (live == 2) blocks(std::integral_constant<int, (MT > 2 ? 2 : MT)>{});
     else if (live == 1) blocks(std::integral_constant<int, 1>{});
     else blocks(std::integral_constant<int, 0>{});
-    f8_wait_barrier<0>();  // LDS is free
+    wait_copies_barrier<0>();  // LDS is free
 }
 
 }  // namespace

@@ -1,0 +1,127 @@
+// int8 quantisation of activations, a float32 scale for each token:
+//     s = max(max|x_k| / 127, 2^-126),  c_k = round(x_k / s), ties to even,
+// both quotients rounded to float32 first. Ties in the second rounding are common (16-bit values over
+// 16-bit maxima), so the quotient has to be the correctly rounded one. A token that holds an infinity or a
+// NaN has a NaN as its scale and zeros as its codes: whatever is made of it is NaN.
+#pragma once
+
+#include "fp8_common.h"
+#include "mm_tile.h"
+
+namespace tsa {
+namespace {
+
+// The largest of the wave's values (magnitudes as bits: their integer order is the order of the values, an
+// infinity above all numbers, a NaN above it).
+template <int N>
+__device__ __forceinline__ uint32_t i8_wave_max(const float (&v)[N][8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[c][e]) & 0x7FFFFFFFu);
+    return wave_max_u32(m);
+}
+
+__device__ __forceinline__ float i8_scale(uint32_t max_bits) {
+    if (max_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    const float s = __uint_as_float(max_bits) / 127.0f;
+    return s < 0x1p-126f ? 0x1p-126f : s;
+}
+
+// The codes of 8 values of a token with scale s. The quotient by Markstein's correction, as the FP8 codes have
+// it (f8_codes8), which divides where bits of the remainder could underflow; EXACT (fp32 inputs) divides. |q| <=
+// 127 (1 + 2^-23), so adding 1.5 2^23 rounds it to an integer, ties to even, in the sum's low bits.
+template <bool EXACT>
+__device__ __forceinline__ uint2 i8_codes8(const float (&v)[8], float s) {
+    float q[8];
+    if (!(s == s)) return make_uint2(0u, 0u);
+    if (EXACT || !(s > F8_MIN_CORRECTED)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = v[e] / s;
+    } else {
+        const float r = 1.0f / s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = v[e] * r;
+            q[e] = fmaf(fmaf(-a, s, v[e]), r, a);
+        }
+    }
+    uint32_t b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(q[e] + 12582912.0f);
+    auto pack = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {  // the low bytes
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0c0c0400u), __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u), 0x05040100u);
+    };
+    return make_uint2(pack(b[0], b[1], b[2], b[3]), pack(b[4], b[5], b[6], b[7]));
+}
+
+// Chunk c (8 values) of a row of K values; past the row zeros. VEC: 16-byte aligned rows of whole chunks.
+template <int XT, bool VEC>
+__device__ __forceinline__ void i8_load8(const uint8_t* row, int64_t K, int c, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    if constexpr (VEC) {
+        if ((int64_t)8 * c < K) f8_load8<XT>(row, c, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if ((int64_t)8 * c + e < K) v[e] = load_act(row, XT, (int64_t)8 * c + e);
+    }
+}
+
+// One row quantised by the W waves that call this together (tid: the thread's number among their 64 W). A thread
+// holds its first D chunks; a longer row's others are read twice. `top`: W words of LDS that no one else uses
+// (the barrier is the workgroup's, so every wave of it has a row, or a dead one: row null).
+template <int XT, bool VEC, int W, int D>
+__device__ __forceinline__ void i8_quantize_row(const uint8_t* row, int64_t K, int tid, uint8_t* codes, float* scale, uint32_t* top) {
+    float v[D][8];
+    const int chunks = row ? (int)((K + 7) / 8) : 0;
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+        if (row) {
+            i8_load8<XT, VEC>(row, K, tid + 64 * W * d, v[d]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[d][e] = 0.0f;
+        }
+    }
+    uint32_t m = i8_wave_max(v);
+    for (int c = tid + 64 * W * D; c < (chunks + 63) / 64 * 64; c += 64 * W) {  // whole waves
+        float u[1][8];
+        i8_load8<XT, VEC>(row, K, c, u[0]);
+        m = max(m, i8_wave_max(u));
+    }
+    if constexpr (W > 1) {
+        if ((tid & 63) == 0) top[tid >> 6] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = max(m, top[w]);
+    }
+    const float s = i8_scale(m);
+    auto put = [&](int c, const float (&u)[8]) {
+        const uint2 o = i8_codes8<XT == TSA_F32>(u, s);
+        uint8_t* dst = codes + (int64_t)8 * c;
+        if constexpr (VEC) {
+            *reinterpret_cast<uint2*>(dst) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((int64_t)8 * c + e < K) dst[e] = (uint8_t)((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (tid + 64 * W * d < chunks) put(tid + 64 * W * d, v[d]);
+    for (int c = tid + 64 * W * D; c < chunks; c += 64 * W) {
+        float u[8];
+        i8_load8<XT, VEC>(row, K, c, u);
+        put(c, u);
+    }
+    if (row && tid == 0) *scale = s;
+}
+
+constexpr int64_t I8_MAX_K = 131056;  // K 2^14 < 2^31: the sums fit 32 bits whatever the codes
+
+}  // namespace
+}  // namespace tsa

@@ -174,7 +174,7 @@ def _fp8_weight(w: torch.Tensor, scales: torch.Tensor, K: int) -> tuple[torch.Te
     return _aligned(w), (scales if scales.dtype == torch.float32 else scales.float()).contiguous(), N
 
 
-def _fp8_bias(bias: torch.Tensor | None, N: int) -> tuple[torch.Tensor | None, int | None, int]:
+def _bias(bias: torch.Tensor | None, N: int) -> tuple[torch.Tensor | None, int | None, int]:
     """(contiguous bias, its pointer, its tsa_dtype)."""
     if bias is None:
         return None, None, 0
@@ -209,7 +209,7 @@ def fp8_matmul(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_sca
     if scales.shape != (T, -(-K // FP8_BLOCK)) or scales.dtype != torch.float32:
         raise RuntimeError(f"activation scales must be float32 [{T}, {-(-K // FP8_BLOCK)}], got {scales.dtype} {list(scales.shape)}")
     c, sc, (w, ws, N) = _aligned(codes), scales.contiguous(), _fp8_weight(w, w_scales, K)
-    b, bp, bt = _fp8_bias(bias, N)
+    b, bp, bt = _bias(bias, N)
     y = c.new_empty((T, N), dtype=out_dtype)
     _call(c, _lib.load().tsa_fp8_matmul, c.data_ptr(), sc.data_ptr(), T, K, w.data_ptr(), ws.data_ptr(), N, bp, bt,
           y.data_ptr(), _lib.tsa_dtype(out_dtype))
@@ -231,13 +231,166 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: t
     dt, K = _lib.tsa_dtype(x.dtype), x.shape[-1]
     w, ws, N = _fp8_weight(w, w_scales, K)
     x2 = _aligned(_rows(x, K))
-    b, bp, bt = _fp8_bias(bias, N)
+    b, bp, bt = _bias(bias, N)
     T = x2.shape[0]
     y = x2.new_empty((T, N), dtype=out_dtype)
     n = _fp8_linear_workspace_size(T, K)
     scratch = x2.new_empty(n, dtype=torch.uint8) if n else None
     _call(x2, _lib.load().tsa_fp8_linear, x2.data_ptr(), dt, T, K, w.data_ptr(), ws.data_ptr(), N, bp, bt, y.data_ptr(),
           dt if out_dtype is None else _lib.tsa_dtype(out_dtype), _lib.ptr(scratch), n)
+    return y
+
+
+# ----------------------------------------------------------------------------- int8, a scale per token and row
+def _int8_codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Quantised tokens (codes int8 [T, K], scales float32 [T]), checked."""
+    if codes.dtype != torch.int8 or codes.dim() != 2:
+        raise RuntimeError(f"int8 activations must be int8 [T, K], got {codes.dtype} {tuple(codes.shape)}")
+    if scales.shape != codes.shape[:1] or scales.dtype != torch.float32:
+        raise RuntimeError(f"activation scales must be float32 [{codes.shape[0]}], got {scales.dtype} {list(scales.shape)}")
+    return _aligned(codes), scales.contiguous()
+
+
+def _int8_weight(w: torch.Tensor, scales: torch.Tensor, K: int) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """(codes, float32 scales, N) of a weight matrix [N, K], checked."""
+    if w.dtype != torch.int8 or w.dim() != 2:
+        raise RuntimeError(f"int8 weights must be int8 [N, K], got {w.dtype} {tuple(w.shape)}")
+    N, Kw = w.shape
+    if Kw != K:
+        raise RuntimeError(f"in_features differ: activations {K}, weight {Kw}")
+    if scales.numel() != N or scales.shape[0] != N:
+        raise RuntimeError(f"weight scales must be [{N}] (or [{N}, 1]) for an [{N}, {K}] weight, got {list(scales.shape)}")
+    return _aligned(w), (scales if scales.dtype == torch.float32 else scales.float()).contiguous(), N
+
+
+def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes int8 [T, K], scales float32 [T]) of x [..., K] (bf16, fp16 or fp32): per token,
+    scale = max(max|x| / 127, 2^-126) and code = round(x / scale), ties to even. A token that holds a NaN or an
+    infinity has NaN as its scale and zeros as its codes."""
+    _lib.require_device(x, what="activation")
+    dt = _lib.tsa_dtype(x.dtype)
+    x2 = _rows(x, x.shape[-1])
+    T, K = x2.shape
+    codes = x2.new_empty((T, K), dtype=torch.int8)
+    scales = x2.new_empty(T, dtype=torch.float32)
+    _call(x2, _lib.load().tsa_int8_quantize, x2.data_ptr(), dt, T, K, codes.data_ptr(), scales.data_ptr())
+    return codes, scales
+
+
+def int8_matmul(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+                bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y [T, N] = (codes @ w^T) * scales[:, None] * w_scales (+ bias): codes [T, K] and scales [T] as
+    int8_quantize returns them, w int8 [N, K] with float32 scales [N] (or [N, 1]); exact sums. K must be a
+    multiple of 16 (at most 131056). Projections that share their input share one int8_quantize."""
+    _one_device(codes, scales, w, w_scales, bias)
+    c, sc = _int8_codes(codes, scales)
+    T, K = c.shape
+    w, ws, N = _int8_weight(w, w_scales, K)
+    b, bp, bt = _bias(bias, N)
+    y = c.new_empty((T, N), dtype=out_dtype)
+    _call(c, _lib.load().tsa_int8_matmul, c.data_ptr(), sc.data_ptr(), T, K, w.data_ptr(), ws.data_ptr(), N, bp, bt,
+          y.data_ptr(), _lib.tsa_dtype(out_dtype))
+    return y
+
+
+@functools.lru_cache(maxsize=4096)
+def _int8_linear_workspace_size(T: int, K: int) -> int:
+    n = ctypes.c_int64()
+    _lib.check(_lib.load().tsa_int8_linear_workspace_size(T, K, ctypes.byref(n)))
+    return n.value
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y [T, N] = int8_matmul(*int8_quantize(x), w, w_scales, bias) for x [..., K] in bf16, fp16 or fp32; y in
+    x's dtype unless ``out_dtype`` says otherwise. K must be a multiple of 16 (at most 131056)."""
+    _one_device(x, w, w_scales, bias)
+    dt, K = _lib.tsa_dtype(x.dtype), x.shape[-1]
+    w, ws, N = _int8_weight(w, w_scales, K)
+    x2 = _aligned(_rows(x, K))
+    b, bp, bt = _bias(bias, N)
+    T = x2.shape[0]
+    y = x2.new_empty((T, N), dtype=out_dtype)
+    n = _int8_linear_workspace_size(T, K)
+    scratch = x2.new_empty(n, dtype=torch.uint8) if n else None
+    _call(x2, _lib.load().tsa_int8_linear, x2.data_ptr(), dt, T, K, w.data_ptr(), ws.data_ptr(), N, bp, bt, y.data_ptr(),
+          dt if out_dtype is None else _lib.tsa_dtype(out_dtype), _lib.ptr(scratch), n)
+    return y
+
+
+# ----------------------------------------------------------------------------- products grouped by expert
+def _grouped_weight(w: torch.Tensor, K: int, dtype: torch.dtype) -> tuple[torch.Tensor, int, int]:
+    """(w, bytes from one expert's matrix to the next, N) of matrices [E, N, K]: each [N, K] contiguous, the experts
+    any multiple of 16 bytes apart (views of packed slots as they are), else a copy."""
+    if w.dim() != 3 or w.dtype != dtype:
+        raise RuntimeError(f"the experts' weights must be {dtype} [E, N, K], got {w.dtype} {tuple(w.shape)}")
+    E, N, Kw = w.shape
+    if Kw != K or E < 1 or N < 1:
+        raise RuntimeError(f"in_features differ: activations {K}, weights {tuple(w.shape)}")
+    es = w.element_size()
+    if w.stride(2) != 1 or w.stride(1) != K or w.stride(0) < N * K or w.stride(0) * es % 16 or w.data_ptr() % 16:
+        w = _aligned(w)
+    return w, max(w.stride(0), N * K) * es, N
+
+
+def _grouped_rows(x: torch.Tensor, offsets: torch.Tensor, rows: torch.Tensor | None, top_k: int, E: int):
+    """(offsets, rows or None, R) of a grouped product over x [T, K], checked."""
+    if offsets.dtype != torch.int32 or offsets.numel() != E + 1:
+        raise RuntimeError(f"offsets must be int32 [{E + 1}] for {E} experts, got {offsets.dtype} {list(offsets.shape)}")
+    if rows is None:
+        if top_k != 1:
+            raise RuntimeError("top_k divides rows: without them it must be 1")
+        return offsets.contiguous(), None, x.shape[0]
+    if rows.dtype != torch.int32 or rows.dim() != 1 or top_k < 1:
+        raise RuntimeError(f"rows must be an int32 vector and top_k positive, got {rows.dtype} {list(rows.shape)} and {top_k}")
+    return offsets.contiguous(), rows.contiguous(), rows.numel()
+
+
+def _grouped_bias(bias: torch.Tensor | None, E: int, N: int):
+    if bias is not None and tuple(bias.shape) != (E, N):
+        raise RuntimeError(f"bias must be [{E}, {N}], got {list(bias.shape)}")
+    return _bias(bias, E * N)
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias: torch.Tensor | None = None,
+                   rows: torch.Tensor | None = None, top_k: int = 1, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y [R, N]: y[r] = x[r] @ w[e]^T (+ bias[e]) for offsets[e] <= r < offsets[e + 1], the rows sorted by expert,
+    offsets int32 [E + 1], any number for each; rows of no expert are zeros. x [T, K] and w [E, N, K] in bf16 or fp16 (an expert's matrix
+    contiguous, the experts any multiple of 16 bytes apart), bias [E, N]; float32 sums, y in x's dtype unless
+    ``out_dtype`` says otherwise. With ``rows`` (int32 [R]), row r takes x[rows[r] // top_k]: group_by_expert's offsets and
+    perm with its top_k are the tokens of a routing. K must be a multiple of 8."""
+    _one_device(x, w, offsets, bias, rows)
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"x must be bfloat16 or float16 [T, K], got {x.dtype} {tuple(x.shape)}")
+    T, K = x.shape
+    w, stride, N = _grouped_weight(w, K, x.dtype)
+    E, x2 = w.shape[0], _aligned(x)
+    off, rows, R = _grouped_rows(x2, offsets, rows, top_k, E)
+    b, bp, bt = _grouped_bias(bias, E, N)
+    y = x2.new_empty((R, N), dtype=out_dtype or x.dtype)
+    _call(x2, _lib.load().tsa_grouped_matmul, x2.data_ptr(), _lib.tsa_dtype(x.dtype), T, K, w.data_ptr(), stride, E, N, off.data_ptr(),
+          _lib.ptr(rows), R, top_k, bp, bt, y.data_ptr(), _lib.tsa_dtype(y.dtype))
+    return y
+
+
+def int8_grouped_matmul(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, offsets: torch.Tensor,
+                        bias: torch.Tensor | None = None, rows: torch.Tensor | None = None, top_k: int = 1,
+                        out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """grouped_matmul over int8: codes [T, K] and scales [T] as int8_quantize returns them, w int8 [E, N, K] with
+    scales [E, N] (or [E, N, 1]). K must be a multiple of 16."""
+    _one_device(codes, scales, w, w_scales, offsets, bias, rows)
+    c, sc = _int8_codes(codes, scales)
+    T, K = c.shape
+    w, stride, N = _grouped_weight(w, K, torch.int8)
+    E = w.shape[0]
+    if w_scales.numel() != E * N or tuple(w_scales.shape[:2]) != (E, N):
+        raise RuntimeError(f"weight scales must be [{E}, {N}], got {list(w_scales.shape)}")
+    ws = (w_scales if w_scales.dtype == torch.float32 else w_scales.float()).contiguous()
+    off, rows, R = _grouped_rows(c, offsets, rows, top_k, E)
+    b, bp, bt = _grouped_bias(bias, E, N)
+    y = c.new_empty((R, N), dtype=out_dtype)
+    _call(c, _lib.load().tsa_int8_grouped_matmul, c.data_ptr(), sc.data_ptr(), T, K, w.data_ptr(), stride, ws.data_ptr(), E, N,
+          off.data_ptr(), _lib.ptr(rows), R, top_k, bp, bt, y.data_ptr(), _lib.tsa_dtype(out_dtype))
     return y
 
 
