@@ -45,7 +45,13 @@ typedef enum tsa_route_mode {
 
 typedef enum tsa_act { TSA_ACT_SILU = 0, TSA_ACT_SWIGLU_OAI = 1 } tsa_act;
 
-typedef enum tsa_expert_format { TSA_EXPERT_MXFP4 = 1, TSA_EXPERT_GGUF = 2, TSA_EXPERT_FP8 = 3 } tsa_expert_format;
+typedef enum tsa_expert_format {
+    TSA_EXPERT_MXFP4 = 1,
+    TSA_EXPERT_GGUF = 2,
+    TSA_EXPERT_FP8 = 3,
+    TSA_EXPERT_DENSE = 5, /* bfloat16 or float16 */
+    TSA_EXPERT_INT8 = 6
+} tsa_expert_format;
 
 /* Where one expert's tensors sit inside a packed slot (byte offsets from the slot start).
  *  MXFP4 (GPT-OSS): gate_up blocks [2I, H/32, 16] u8 at gate_off (rows interleaved:
@@ -63,6 +69,14 @@ typedef enum tsa_expert_format { TSA_EXPERT_MXFP4 = 1, TSA_EXPERT_GGUF = 2, TSA_
  *    16-byte aligned. Activations are quantised as tsa_fp8_quantize does, x before gate and up and
  *    h = act(gate, up) (float32) before down. Sums are of float32 accuracy but for down's where y has
  *    16 bits, which are tsa_fp8_matmul's.
+ *  DENSE: gate [I, H], up [I, H] and down [H, I] in the tsa_dtype of gate_type, up_type and down_type (all TSA_BF16
+ *    or all TSA_F16) at gate_off, up_off and down_off. x has the same type, and h = act(gate, up) (float32 sums) is rounded
+ *    to it before down.
+ *  INT8: the same matrices as int8 codes, with float32 scales per row at gate_scales_off (gate's [I], then up's)
+ *    and at down_scales_off ([H]). Activations are quantised as tsa_int8_quantize does, x before gate and up and h
+ *    (float32) before down; a token with a NaN or an infinity gives NaN.
+ *  DENSE and INT8: offsets and slot_bytes (below 2^31) multiples of 16, no biases (-1); pool, x and workspaces 16-byte
+ *    aligned; sums of float32 accuracy, y rounded once.
  *  act: TSA_ACT_SWIGLU_OAI = (up+1)*g*sigmoid(alpha*g), g = min(gate, limit),
  *    up = clamp(up, -limit, limit); TSA_ACT_SILU = silu(gate)*up.
  *  prefill_mfma (tiled MXFP4 prefill GEMMs): TSA_PREFILL_FP6 (0, the default) multiplies the

@@ -73,3 +73,56 @@ def grouped(x, w, offsets: list[int], bias=None, rows: list[int] | None = None, 
         else:
             y[a:b], err[a:b] = matmul16(pad(x), w[e], be)
     return y, err
+
+
+def _act(g, ge, u, ue, act: str):
+    """(h, bound of its error) of the activation on gate and up with their errors."""
+    if act == "silu":
+        sg, slope = g * torch.sigmoid(g), 1.1  # |silu'| < 1.1
+    else:
+        a, lim = 1.702, 7.0
+        g, u, slope = g.clamp(max=lim), u.clamp(-lim, lim) + 1, 1.2
+        sg = g * torch.sigmoid(a * g)
+    h = sg * u
+    # exp2 and rcp within 2 units, exp's argument rounded twice: g times 2 units more
+    return h, slope * ge * u.abs() + (sg.abs() + slope * ge) * ue + h.abs() * (8 + 4 * g.abs()) * 2 * U
+
+
+def expert8(q, s, e: dict, act: str = "silu"):
+    """(y, bound) of an int8 expert (tensors of synth.int8_layout) for quantised tokens. A code of h may be that of any
+    h / s within h's error."""
+    h, he = _act(*matmul(q, s, e["gate_proj"], e["gate_proj_scale"]), *matmul(q, s, e["up_proj"], e["up_proj_scale"]), act)
+    hq, hs = quantize(h)
+    v, top = h / hs, he.amax(1, keepdim=True) / (127 * hs) + 2 * U  # the scale's own relative error, at most
+    ve = he / hs + v.abs() * (top + 2 * U)
+    qe = torch.maximum((torch.round(v + ve) - hq).abs(), (torch.round(v - ve) - hq).abs()) + hq.abs() * top
+    y, ye = matmul(hq, hs, e["down_proj"], e["down_proj_scale"])
+    return y, ye + ((qe * hs) @ e["down_proj"].double().abs().t()) * e["down_proj_scale"].double()
+
+
+def expert16(x, e: dict, act: str = "silu"):
+    """(y, bound) of a 16-bit expert: h is rounded to the weights' type, as any number within its error may be."""
+    dt = e["down_proj"].dtype
+    h, he = _act(*matmul16(x, e["gate_proj"]), *matmul16(x, e["up_proj"]), act)
+    hr = h.to(dt).double()
+    qe = torch.maximum(((h + he).to(dt).double() - hr).abs(), ((h - he).to(dt).double() - hr).abs())
+    y, ye = matmul16(hr, e["down_proj"])
+    return y, ye + qe @ e["down_proj"].double().abs().t()
+
+
+def moe(x, idx, w, experts: list, act: str = "silu"):
+    """(y, bound) of the layer; idx < 0 (or an expert that is None) contributes nothing."""
+    int8 = next(e for e in experts if e is not None)["down_proj"].dtype == torch.int8
+    q, s = quantize(x) if int8 else (x.double(), None)
+    y = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    err, mag = torch.zeros_like(y), torch.zeros_like(y)
+    for e in torch.unique(idx).tolist():
+        if e < 0 or experts[e] is None:
+            continue
+        t, j = (idx == e).nonzero(as_tuple=True)
+        o, oe = expert8(q[t], s[t], experts[e], act) if int8 else expert16(q[t], experts[e], act)
+        wt = w[t, j].double().unsqueeze(1)
+        y.index_add_(0, t, wt * o)
+        err.index_add_(0, t, wt.abs() * oe)
+        mag.index_add_(0, t, (wt * o).abs())
+    return y, err + mag * (idx.shape[1] + 4) * 2 * U

@@ -140,8 +140,7 @@ def test_linear_views_and_no_tokens():
     wv = torch.zeros((64, 300), dtype=torch.int8, device="cuda")
     wv[:, 4:292] = w
     ref.check(ops.int8_linear(x, wv[:, 4:292], ws), want, err, "w off 16 bytes")
-    y = torch.empty(3 * 65, dtype=torch.bfloat16, device="cuda")
-    assert ops.int8_linear(x[:0], w, ws).shape == (0, 64) and y is not None
+    assert ops.int8_linear(x[:0], w, ws).shape == (0, 64)
     assert ops.int8_linear(x.view(1, 3, 288), w, ws).shape == (3, 64)
 
 

@@ -29,7 +29,7 @@ _TORCH_TO_TSA = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 # routing modes / activations / expert formats
 ROUTE_TOPK_SOFTMAX, ROUTE_SOFTMAX_TOPK, ROUTE_SOFTMAX_TOPK_RENORM = 0, 1, 2
 ACT_SILU, ACT_SWIGLU_OAI = 0, 1
-EXPERT_MXFP4, EXPERT_GGUF, EXPERT_FP8 = 1, 2, 3
+EXPERT_MXFP4, EXPERT_GGUF, EXPERT_FP8, EXPERT_DENSE, EXPERT_INT8 = 1, 2, 3, 5, 6
 PREFILL_FP6, PREFILL_BF16 = 0, 1
 
 

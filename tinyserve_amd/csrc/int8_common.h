@@ -70,22 +70,18 @@ __device__ __forceinline__ void i8_load8(const uint8_t* row, int64_t K, int c, f
     }
 }
 
-// One row quantised by the W waves that call this together (tid: the thread's number among their 64 W). A thread
-// holds its first D chunks; a longer row's others are read twice. `top`: W words of LDS that no one else uses
-// (the barrier is the workgroup's, so every wave of it has a row, or a dead one: row null).
+// One row quantised by the W waves that call these together (tid: the thread's number among their 64 W). A thread
+// holds its first D chunks from i8_row_load on; a longer row's others are read twice. `top`: W words of LDS
+// that no one else uses (the barrier is the workgroup's: every wave of it calls).
 template <int XT, bool VEC, int W, int D>
-__device__ __forceinline__ void i8_quantize_row(const uint8_t* row, int64_t K, int tid, uint8_t* codes, float* scale, uint32_t* top) {
-    float v[D][8];
-    const int chunks = row ? (int)((K + 7) / 8) : 0;
+__device__ __forceinline__ void i8_row_load(const uint8_t* row, int64_t K, int tid, float (&v)[D][8]) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-        if (row) {
-            i8_load8<XT, VEC>(row, K, tid + 64 * W * d, v[d]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[d][e] = 0.0f;
-        }
-    }
+    for (int d = 0; d < D; ++d) i8_load8<XT, VEC>(row, K, tid + 64 * W * d, v[d]);
+}
+
+template <int XT, bool VEC, int W, int D>
+__device__ __forceinline__ float i8_row_codes(const uint8_t* row, int64_t K, int tid, const float (&v)[D][8], uint8_t* codes, uint32_t* top) {
+    const int chunks = (int)((K + 7) / 8);
     uint32_t m = i8_wave_max(v);
     for (int c = tid + 64 * W * D; c < (chunks + 63) / 64 * 64; c += 64 * W) {  // whole waves
         float u[1][8];
@@ -118,7 +114,7 @@ __device__ __forceinline__ void i8_quantize_row(const uint8_t* row, int64_t K, i
         i8_load8<XT, VEC>(row, K, c, u);
         put(c, u);
     }
-    if (row && tid == 0) *scale = s;
+    return s;
 }
 
 constexpr int64_t I8_MAX_K = 131056;  // K 2^14 < 2^31: the sums fit 32 bits whatever the codes

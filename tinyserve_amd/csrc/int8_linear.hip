@@ -17,7 +17,11 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const uint8_t* __res
     const int g = (int)threadIdx.x / (64 * W);
     const int64_t t = (int64_t)blockIdx.x * (4 / W) + g;
     if (W == 1 && t >= T) return;
-    i8_quantize_row<XT, VEC, W, D>(x + t * K * ES, K, (int)threadIdx.x - 64 * W * g, codes + t * K, scales + t, top + W * g);
+    const int tid = (int)threadIdx.x - 64 * W * g;
+    float v[D][8];
+    i8_row_load<XT, VEC, W, D>(x + t * K * ES, K, tid, v);
+    const float s = i8_row_codes<XT, VEC, W, D>(x + t * K * ES, K, tid, v, codes + t * K, top + W * g);
+    if (tid == 0) scales[t] = s;
 }
 
 template <int XT, bool VEC>

@@ -18,7 +18,7 @@
 // experts top-4, 4 and 2048 tokens 74 / 71 and 605 / 568; hidden 2048, 128 experts top-8, 1, 24 and 1024 tokens
 // 15.7 / 15.3, 48.5 / 47.0 and 220 / 208.
 #include "fp8_gemm.h"
-#include "moe_group.h"
+#include "moe_grouped.h"
 
 namespace tsa {
 namespace {
@@ -46,16 +46,6 @@ struct F8Moe {
 
 constexpr int F8A_NW = 8, F8A_D = 3, F8A_XC = 1;  // gate_up: waves; K blocks in flight per wave; chunks of x held per thread
 constexpr int F8D_NW = 8, F8D_D = 3, F8D_HC = 2;  // down: the same with its units and h
-
-__device__ __forceinline__ float f8_act(const tsa_expert_layout& L, float gate, float up) {
-    if (L.act == TSA_ACT_SWIGLU_OAI) {
-        // the limits by comparisons: a minimum or maximum would give its other operand for a NaN
-        const float lim = L.swiglu_limit, g = gate > lim ? lim : gate, u = up > lim ? lim : up < -lim ? -lim : up;
-        const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * (L.swiglu_alpha * g));
-        return (u + 1.0f) * g * __builtin_amdgcn_rcpf(1.0f + e);
-    }
-    return silu_mul_fast(gate, up);
-}
 
 // One workgroup per (token, expert) pair and 8 channels: rows 0 .. 7 of the tile are the channels' gate
 // rows, 8 .. 15 their up rows, so one pair gives enough workgroups (768 at inter 768 and top-8, three
@@ -166,7 +156,7 @@ __global__ void __launch_bounds__(64 * F8A_NW) fp8_gate_up_kernel(F8Moe p) {
         float g = 0.0f, u = 0.0f;
 #pragma unroll
         for (int w = 0; w < F8A_NW; ++w) g += red[16 * w + tid], u += red[16 * w + 8 + tid];
-        p.h[(int64_t)a * I + n0 + tid] = f8_act(L, g, u);
+        p.h[(int64_t)a * I + n0 + tid] = moe_act(L, g, u);
     }
 }
 
@@ -272,8 +262,6 @@ __global__ void __launch_bounds__(64 * F8D_NW, 4) fp8_down_kernel(F8Moe p) {
     }
 }
 
-int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-
 // ---------------------------------------------------------------- many tokens
 // Four launches: (1) the assignments grouped by expert with a table of token tiles (workgroup 0), x
 // quantised (the others); (2) gate_up over the tiles: 128 channels of gate and of up per workgroup, so
@@ -329,17 +317,6 @@ __global__ void __launch_bounds__(GROUP_THREADS) fp8_prepare_kernel(F8Group p) {
     }
 }
 
-// The workgroup's (entry, tile) of n_entries x tiles: each XCD takes a run of the entries with all
-// their tiles (an expert's entries and an entry's tiles share an L2). False: none is left for it.
-__device__ __forceinline__ bool f8_work(const int* n_entries, int tiles, int& entry, int& tile) {
-    const int total = uniform(*n_entries) * tiles, lin = (int)blockIdx.x, xcd = lin & 7, q8 = total >> 3, rem = total & 7;
-    if ((lin >> 3) >= q8 + (xcd < rem ? 1 : 0)) return false;
-    const int wid = xcd * q8 + (xcd < rem ? xcd : rem) + (lin >> 3);
-    entry = wid / tiles;
-    tile = wid % tiles;
-    return true;
-}
-
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -347,7 +324,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p
     const tsa_expert_layout& L = p.L;
     const int H = (int)L.hidden, I = (int)L.inter, GH = (int)f8_blocks(H), GI = (int)f8_blocks(I);
     int entry, tile;
-    if (!f8_work(p.n_entries, GI, entry, tile)) return;
+    if (!grouped_work(p.n_entries, GI, entry, tile)) return;
     const int4 e = p.table[entry];
     const int slot = uniform(e.x), row0 = uniform(e.y), tn = uniform(e.z), c0 = tile * F8B;
     const uint8_t* base = p.pool + (int64_t)slot * L.slot_bytes;
@@ -379,7 +356,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_gate_up_kernel(F8Group p
         for (int j = 0; j < MP; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                acc[j][t][r] = f8_act(L, acc[j][t][r], acc[MP + j][t][r]);
+                acc[j][t][r] = moe_act(L, acc[j][t][r], acc[MP + j][t][r]);
                 m = max(m, __float_as_uint(acc[j][t][r]) & 0x7FFFFFFFu);
             }
         m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
@@ -413,7 +390,7 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_down_kernel(F8Group p) {
     const tsa_expert_layout& L = p.L;
     const int H = (int)L.hidden, I = (int)L.inter, GI = (int)f8_blocks(I);
     int entry, tile;
-    if (!f8_work(p.n_entries, (H + C::RN - 1) / C::RN, entry, tile)) return;
+    if (!grouped_work(p.n_entries, (H + C::RN - 1) / C::RN, entry, tile)) return;
     const int4 e = p.table[entry];
     const int slot = uniform(e.x), row0 = uniform(e.y), tn = uniform(e.z), n0 = tile * C::RN;
     const uint8_t* base = p.pool + (int64_t)slot * L.slot_bytes;
@@ -445,55 +422,10 @@ __global__ void __launch_bounds__(C::THREADS) fp8_group_down_kernel(F8Group p) {
     }
 }
 
-// y[t] = sum_j w[t, j] yk[t k + j], in order of j; a thread 8 values of a row.
-__global__ void __launch_bounds__(256) fp8_combine_kernel(F8Group p) {
-    const int H = (int)p.L.hidden, per = H / 8;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (int64_t)p.T * per) return;
-    const int t = (int)(at / per), c = (int)(at % per);
-    float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int AHEAD = 4;  // outputs on their way together
-    for (int j0 = 0; j0 < p.k; j0 += AHEAD) {
-        int sl[AHEAD];
-        float w[AHEAD], v[AHEAD][8];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int64_t a = (int64_t)t * p.k + (j0 + u < p.k ? j0 + u : j0);
-            const int e = p.idx[a];
-            w[u] = p.wts[a];
-            sl[u] = j0 + u < p.k && e >= 0 && e < p.E ? p.expert_slot[e] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {  // not resident: nothing was written there, and any row is read
-            const bool live = sl[u] >= 0 && sl[u] < p.n_slots;
-            f8_load8<TSA_F32>(p.yk + (live ? (int64_t)t * p.k + j0 + u : 0) * H, c, v[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-            for (int r = 0; r < 8; ++r) s[r] = sl[u] >= 0 && sl[u] < p.n_slots ? fmaf(w[u], v[u][r], s[r]) : s[r];
-    }
-    const int64_t o = (int64_t)t * H + 8 * c;
-    if (p.y_dtype == TSA_BF16 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + o) =
-            make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
-        return;
-    }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) store_out(p.y, p.y_dtype, o + r, s[r]);
-}
-
 using GateUp128 = F8Tile<4, 2, 4, 4, 3>;  // 128 channels x 128 tokens, 8 waves
 using GateUp64 = F8Tile<4, 2, 4, 2, 3>;   // x 64
 using Down128 = F8Tile<4, 2, 4, 4, 3>;    // 256 rows x 128 tokens
 using Down64 = F8Tile<4, 1, 2, 4, 3>;     // 128 x 64, two workgroups per CU
-
-constexpr int64_t F8_CHUNK = 131072;  // assignments at a time: bounds the workspace (1.1 GiB at hidden 2048)
-
-int64_t group_tokens(int64_t T, int k) {
-    const int64_t c = F8_CHUNK / k > 0 ? F8_CHUNK / k : 1;
-    return T < c ? T : c;
-}
 
 struct F8Places {
     int64_t counts, offsets, perm, n_entries, table, xq, xs, hq, hs, yk, bytes;
@@ -605,13 +537,13 @@ bool f8_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E)
 }
 
 int64_t f8_group_workspace_bytes(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
-    return group_places(L, group_tokens(T, k), k, E).bytes;
+    return group_places(L, group_tokens(T, k, MOE_ASSIGNMENTS), k, E).bytes;
 }
 
 int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const int32_t* expert_slot, int64_t E,
                      const int32_t* idx, const float* weights, int64_t T, int k, const void* x, int x_dtype, void* y,
                      int y_dtype, uint8_t* ws, hipStream_t st) {
-    const int64_t step = group_tokens(T, k), H = L.hidden;
+    const int64_t step = group_tokens(T, k, MOE_ASSIGNMENTS), H = L.hidden;
     const F8Places w = group_places(L, step, k, E);
     const int lds = group_lds_bytes((int)E);
     const void* fp = x_dtype == TSA_F32 ? reinterpret_cast<const void*>(&fp8_prepare_kernel<TSA_F32>)
@@ -653,9 +585,8 @@ int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_
         TSA_HIP_CHECK(hipLaunchKernel(fp, dim3((unsigned)(1 + (p.T + F8P_ROWS - 1) / F8P_ROWS)), dim3(GROUP_THREADS), args, lds, st));
         const int rc = p.tile_rows == 64 ? group_gemms<GateUp64, Down64>(p, entries, st) : group_gemms<GateUp128, Down128>(p, entries, st);
         if (rc) return rc;
-        const dim3 grid((unsigned)(((int64_t)p.T * (H / 8) + 255) / 256));
-        hipLaunchKernelGGL(fp8_combine_kernel, grid, dim3(256), 0, st, p);
-        TSA_LAUNCH_CHECK();
+        const int rc2 = launch_combine(MoeCombine{p.idx, p.wts, expert_slot, E, n_slots, p.T, k, (int)H, p.yk, p.y, y_dtype}, st);
+        if (rc2) return rc2;
     }
     return TSA_OK;
 }

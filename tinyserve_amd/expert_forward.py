@@ -10,16 +10,17 @@ The functions of tinyserve/expert_forward.py with the same names and arguments:
   slot's quantised tensors, the forward runs on this library's kernels.
 * ``_build_inline_forward(layout, act_fn)`` (:109-194): ``(packed, h) -> y`` for an
   unquantised (bf16/fp16/fp32) fused-expert slot with ``F.linear``; None for quantised
-  slots. Unquantised experts are not this library's hot path; this is plain torch on the GPU.
+  slots. These fused unquantised slots run on plain torch on the GPU; 16-bit slots of separate matrices
+  (``gate_proj`` / ``up_proj`` / ``down_proj``) have kernels (``_build_dense_inline_forward``).
 * ``_build_mxfp4_inline_forward(layout, act_fn)`` (:197-246): ``(packed, h) -> y`` for an
   MXFP4 slot, one fused decode call (the closure's ``expert_layout`` attribute is the
   kernel layout, used by the batched paths).
 * ``_build_gpu_int4_forward`` (:249-262): None, as in the reference (MXFP4 slots run on
   the MXFP4 kernels directly).
 * ``_build_cpp_layout_args(layout, act_fn)`` (:277-338): the keyword arguments of
-  ``fast_expert_forward`` for a slot layout (``{"layout": tsa_expert_layout}`` for MXFP4;
-  None where no kernel layout follows from the TensorLayout alone: GGUF needs its ggml
-  types, unquantised slots have no kernel).
+  ``fast_expert_forward`` for a slot layout (``{"layout": tsa_expert_layout}`` for MXFP4, FP8, int8 and
+  16-bit slots; None where no kernel layout follows from the TensorLayout alone: GGUF needs its ggml
+  types, fused unquantised slots run on torch).
 * ``fast_expert_forward`` is the fused top-k loop of tinyserve/csrc/expert_loop.cpp:41-123,
   one HIP call per layer with the slots and weights kept on the device.
 
@@ -37,6 +38,7 @@ import torch.nn.functional as F
 from . import _lib, ops
 from .expert_store import TensorLayout
 from .fp8 import FP8Module
+from .int8 import Int8Module
 
 # sigmoid(1.702 x) ~ GELU(x): GPT-OSS SwiGLU coefficient (tinyserve/expert_forward.py:30).
 _QUICK_GELU_COEFF = 1.702
@@ -134,13 +136,13 @@ def gguf_expert_layout(layout: TensorLayout, ggml_types: dict, proj_shapes: dict
     return L
 
 
-_FP8_MATS = ("gate_proj", "up_proj", "down_proj")
+_MATS = ("gate_proj", "up_proj", "down_proj")
 
 
 def is_fp8_layout(layout: TensorLayout) -> bool:
     """Whether a slot holds an FP8 expert: e4m3 gate_proj / up_proj / down_proj and their block scales."""
     return all(m in layout.specs and layout.specs[m][1] == torch.float8_e4m3fn and m + "_scale_inv" in layout.specs
-               for m in _FP8_MATS)
+               for m in _MATS)
 
 
 def fp8_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout:
@@ -172,13 +174,88 @@ def fp8_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None 
     return L
 
 
+def is_int8_layout(layout: TensorLayout) -> bool:
+    """Whether a slot holds an int8 expert: int8 gate_proj / up_proj / down_proj and their scales per row."""
+    return all(m in layout.specs and layout.specs[m][1] == torch.int8 and m + "_scale" in layout.specs for m in _MATS)
+
+
+def is_dense_layout(layout: TensorLayout) -> bool:
+    """Whether a slot holds a 16-bit expert as gate_proj / up_proj / down_proj and nothing else."""
+    return set(layout.specs) == set(_MATS) and all(layout.specs[m][1] in (torch.bfloat16, torch.float16) for m in _MATS)
+
+
+def _plain_layout(fmt: int, layout: TensorLayout, act_fn, slot_bytes: int | None, what: str) -> _lib.ExpertLayout:
+    """The fields that 16-bit and int8 slots of gate_proj / up_proj / down_proj share, checked."""
+    if act_fn is not None and not _is_silu(act_fn):
+        raise NotImplementedError(f"unsupported activation {act_fn!r}")
+    (I, H), off = layout.specs["gate_proj"][0], layout.offsets
+    for m, shape in (("gate_proj", (I, H)), ("up_proj", (I, H)), ("down_proj", (H, I))):
+        if tuple(layout.specs[m][0]) != shape or layout.specs[m][1] != layout.specs["gate_proj"][1]:
+            raise ValueError(f"inconsistent {what} expert shapes: {m} {layout.specs[m]}, hidden {H}, inter {I}")
+    L = _lib.ExpertLayout()
+    L.format, L.act = fmt, _lib.ACT_SILU
+    L.hidden, L.inter = H, I
+    L.slot_bytes = slot_bytes or layout.total_bytes
+    L.gate_off, L.up_off, L.down_off = off["gate_proj"], off["up_proj"], off["down_proj"]
+    L.gate_scales_off = L.down_scales_off = -1
+    L.gate_bias_off = L.down_bias_off = -1
+    L.bias_dtype = _lib.BF16
+    L.swiglu_limit, L.swiglu_alpha = _SWIGLU_LIMIT, _QUICK_GELU_COEFF
+    return L
+
+
+def int8_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout:
+    """tsa_expert_layout of an int8 slot: ``gate_proj`` / ``up_proj`` [I, H] and ``down_proj`` [H, I] as int8,
+    ``*_scale`` float32 per row, up's scales right behind gate's (the order of synth.int8_layout). act_fn None
+    or SiLU."""
+    if not is_int8_layout(layout):
+        raise ValueError(f"not an int8 expert slot: {sorted(layout.specs)}")
+    L = _plain_layout(_lib.EXPERT_INT8, layout, act_fn, slot_bytes, "int8")
+    off = layout.offsets
+    for m, n in (("gate_proj", L.inter), ("up_proj", L.inter), ("down_proj", L.hidden)):
+        shape, dtype = layout.specs[m + "_scale"]
+        if tuple(shape) not in ((n,), (n, 1)) or dtype != torch.float32:
+            raise ValueError(f"inconsistent int8 expert shapes: {m}_scale {shape} {dtype}, expected float32 [{n}]")
+    if off["up_proj_scale"] != off["gate_proj_scale"] + layout.sizes["gate_proj_scale"]:
+        raise ValueError("up_proj_scale must follow gate_proj_scale in the slot")
+    L.gate_scales_off, L.down_scales_off = off["gate_proj_scale"], off["down_proj_scale"]
+    return L
+
+
+def dense_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout:
+    """tsa_expert_layout of a bfloat16 or float16 slot: ``gate_proj`` / ``up_proj`` [I, H] and ``down_proj`` [H, I],
+    act_fn None or SiLU; or, with act_fn SiLU, the fused ``gate_up_proj`` [2 I, H] (gate's rows, then up's) and
+    ``down_proj``. (act_fn None stands for the clamped SwiGLU on interleaved rows there, which has no kernel.)"""
+    specs = layout.specs
+    if set(specs) == {"gate_up_proj", "down_proj"} and _is_silu(act_fn):
+        (two_i, H), dt = specs["gate_up_proj"] if len(specs["gate_up_proj"][0]) == 2 else ((0, 0), None)
+        if two_i % 2 or dt not in (torch.bfloat16, torch.float16) or tuple(specs["down_proj"][0]) != (H, two_i // 2):
+            raise ValueError(f"not a 16-bit expert slot of [out, in] matrices: {specs}")
+        halves = TensorLayout({"gate_proj": ((two_i // 2, H), dt), "up_proj": ((two_i // 2, H), dt), "down_proj": specs["down_proj"]})
+        L = _plain_layout(_lib.EXPERT_DENSE, halves, act_fn, slot_bytes or layout.total_bytes, "16-bit")
+        L.gate_off = layout.offsets["gate_up_proj"]
+        L.up_off, L.down_off = L.gate_off + halves.sizes["gate_proj"], layout.offsets["down_proj"]
+    elif is_dense_layout(layout):
+        dt = specs["gate_proj"][1]
+        L = _plain_layout(_lib.EXPERT_DENSE, layout, act_fn, slot_bytes, "16-bit")
+    else:
+        raise ValueError(f"not a 16-bit expert slot: {specs}")
+    L.gate_type = L.up_type = L.down_type = _lib.tsa_dtype(dt)
+    return L
+
+
 def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | None = None,
                         proj_shapes: dict | None = None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
-    """The kernel-side layout of a packed expert, or None for unquantised layouts."""
+    """The kernel-side layout of a packed expert, or None for unquantised layouts of fused matrices
+    (dense_expert_layout takes some of them)."""
     if "gate_up_proj_scales" in layout.specs:
         return mxfp4_expert_layout(layout, act_fn, slot_bytes)
     if is_fp8_layout(layout):
         return fp8_expert_layout(layout, act_fn, slot_bytes)
+    if is_int8_layout(layout):
+        return int8_expert_layout(layout, act_fn, slot_bytes)
+    if is_dense_layout(layout):
+        return dense_expert_layout(layout, act_fn, slot_bytes)
     if ggml_types is not None and {"gate", "up", "down"} <= set(layout.specs):
         return gguf_expert_layout(layout, ggml_types, proj_shapes, slot_bytes)
     return None
@@ -308,6 +385,25 @@ class FP8ExpertModule(FP8Module):
         return ops.fp8_linear(F.silu(g) * u, self.down_proj, self.down_proj_scale_inv, out_dtype=h.dtype)
 
 
+class Int8ExpertModule(Int8Module):
+    """An int8 expert whose parameters are the slot's tensors (``gate_proj``, ``up_proj``, ``down_proj`` and their
+    ``_scale``), for forward_from_packed / swap_weights_and_forward; the forward is the fused kernels' layer in
+    three int8 linears: gate and up in float32, silu(gate) * up quantised again for down."""
+
+    def __init__(self, layout: TensorLayout, device=None):
+        super().__init__()
+        if not is_int8_layout(layout):
+            raise ValueError(f"not an int8 expert slot: {sorted(layout.specs)}")
+        for name, (shape, dtype) in layout.specs.items():
+            self.register_parameter(name, nn.Parameter(torch.zeros(shape, dtype=dtype, device=device),
+                                                       requires_grad=False))
+
+    def forward(self, h: torch.Tensor) -> torch.Tensor:
+        g = ops.int8_linear(h, self.gate_proj, self.gate_proj_scale, out_dtype=torch.float32)
+        u = ops.int8_linear(h, self.up_proj, self.up_proj_scale, out_dtype=torch.float32)
+        return ops.int8_linear(F.silu(g) * u, self.down_proj, self.down_proj_scale, out_dtype=h.dtype)
+
+
 # ----------------------------------------------------------------------------- inline builders
 def _build_inline_forward(layout: TensorLayout, act_fn):
     """``(packed, h) -> y`` for an unquantised fused-expert slot (``gate_up_proj`` and
@@ -362,10 +458,14 @@ def _build_gpu_int4_forward(layout, act_fn):
 
 def _build_cpp_layout_args(layout: TensorLayout, act_fn):
     """Keyword arguments of fast_expert_forward for slots of this layout: the kernel layout
-    of an MXFP4 or FP8 slot; None where the TensorLayout alone fixes no kernel layout (GGUF slots
-    need their ggml types, see gguf_expert_layout; unquantised slots have no kernel)."""
+    of an MXFP4, FP8, int8 or 16-bit slot; None where the TensorLayout alone fixes no kernel layout (GGUF
+    slots need their ggml types, see gguf_expert_layout; fused unquantised slots run on torch)."""
     if is_fp8_layout(layout):
         return {"layout": fp8_expert_layout(layout, act_fn)}
+    if is_int8_layout(layout):
+        return {"layout": int8_expert_layout(layout, act_fn)}
+    if is_dense_layout(layout):
+        return {"layout": dense_expert_layout(layout, act_fn)}
     if "gate_up_proj_scales" not in layout.specs:
         return None
     return {"layout": mxfp4_expert_layout(layout, act_fn)}
@@ -381,6 +481,13 @@ def _build_mxfp4_inline_forward(layout: TensorLayout, act_fn):
 def _build_fp8_inline_forward(layout: TensorLayout, act_fn):
     """The same for an FP8 slot."""
     return _layout_forward(fp8_expert_layout(layout, act_fn)) if is_fp8_layout(layout) else None
+
+
+def _build_dense_inline_forward(layout: TensorLayout, act_fn):
+    """The same for a 16-bit or int8 slot of gate_proj / up_proj / down_proj."""
+    if is_int8_layout(layout):
+        return _layout_forward(int8_expert_layout(layout, act_fn))
+    return _layout_forward(dense_expert_layout(layout, act_fn)) if is_dense_layout(layout) else None
 
 
 def _layout_forward(L: _lib.ExpertLayout):

@@ -32,8 +32,9 @@ import torch.nn as nn
 
 from . import ops
 from .expert_cache import ExpertCache
-from .expert_forward import (_build_cpp_layout_args, _build_fp8_inline_forward, _build_gpu_int4_forward, _build_inline_forward,
-                             _build_mxfp4_inline_forward, _precompute_param_refs, mxfp4_expert_layout)
+from .expert_forward import (_build_cpp_layout_args, _build_dense_inline_forward, _build_fp8_inline_forward,
+                             _build_gpu_int4_forward, _build_inline_forward, _build_mxfp4_inline_forward,
+                             _precompute_param_refs, mxfp4_expert_layout)
 
 
 class ExpertPipeline:
@@ -81,6 +82,7 @@ class ExpertPipeline:
             self._inline_fwd = (_build_inline_forward(store.layout, self._act_fn)
                                 or _build_mxfp4_inline_forward(self.cache_layout, self._act_fn)
                                 or _build_fp8_inline_forward(self.cache_layout, self._act_fn)
+                                or _build_dense_inline_forward(self.cache_layout, self._act_fn)
                                 or _build_gpu_int4_forward(store.layout, self._act_fn))
             self._cpp_layout_args = _build_cpp_layout_args(self.cache_layout, self._act_fn)
         self._kernel_layouts: dict[int, object] = {}

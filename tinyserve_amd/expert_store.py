@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import itertools
 import math
+import re
 
 import torch
 
@@ -69,20 +70,51 @@ def mxfp4_tiled_specs(specs: dict) -> dict:
     return out
 
 
-def _stack_fp8(tensors: dict[str, torch.Tensor], layer: int) -> dict[str, torch.Tensor]:
-    """A layer's FP8 experts, ``<e>.<matrix>.weight`` and ``.weight_scale_inv``, as one tensor per name
-    with the experts first, in slot order (the matrices, then their scales as float32)."""
+# per-expert checkpoints: the codes' type, the suffix of the scales in the checkpoint and in the slot
+_SPLIT_FORMATS = {
+    "FP8": (torch.float8_e4m3fn, "weight_scale_inv", "_scale_inv"),
+    "int8": (torch.int8, "weight_scale", "_scale"),
+    "16-bit": (None, None, None),
+}
+
+
+def _split_format(names, first: dict[str, torch.Tensor]) -> str | None:
+    """The format of a layer that keeps one tensor per expert (``<e>.<matrix>.weight`` and its scales), or None."""
+    if any(re.fullmatch(r"\d+\.\w+\.weight_scale_inv", n) for n in names):
+        return "FP8"
+    weights = [n for n in names if re.fullmatch(r"\d+\.(gate|up|down)_proj\.weight", n)]
+    if any(first[n].dtype == torch.int8 for n in weights):
+        return "int8"
+    if weights and len(weights) == len(names) and all(first[n].dtype in (torch.bfloat16, torch.float16) for n in weights):
+        return "16-bit"
+    return None
+
+
+def _stack_experts(tensors: dict[str, torch.Tensor], layer: int, fmt: str) -> dict[str, torch.Tensor]:
+    """A layer's FP8, int8 or 16-bit experts, ``<e>.<matrix>.weight`` and its scales, as one tensor per name
+    with the experts first, in slot order (the matrices, then their scales as float32; int8's as vectors)."""
+    dtype, scale, part = _SPLIT_FORMATS[fmt]
     n = 1 + max((int(k.split(".")[0]) for k in tensors if k.split(".")[0].isdigit()), default=-1)
     out: dict[str, torch.Tensor] = {}
-    for suffix, part in (("weight", ""), ("weight_scale_inv", "_scale_inv")):
+    for suffix, name in (("weight", ""), (scale, part)):
+        if suffix is None:
+            continue
         for mat in ("gate_proj", "up_proj", "down_proj"):
             keys = [f"{e}.{mat}.{suffix}" for e in range(n)]
             missing = [k for k in keys if k not in tensors]
             if missing:
-                raise ValueError(f"layer {layer}: FP8 expert tensors missing: {missing[:4]}")
-            out[mat + part] = torch.stack([tensors.pop(k).float() if part else tensors.pop(k) for k in keys])
-            if not part and out[mat].dtype != torch.float8_e4m3fn:
-                raise ValueError(f"layer {layer}: {mat} is {out[mat].dtype}, not float8_e4m3fn")
+                raise ValueError(f"layer {layer}: {fmt} expert tensors missing: {missing[:4]}")
+            got = [tensors.pop(k) for k in keys]
+            if name:
+                got = [t.float() for t in got]
+                if fmt == "int8":
+                    rows = out[mat].shape[1]
+                    if any(tuple(t.shape) not in ((rows,), (rows, 1)) for t in got):
+                        raise ValueError(f"layer {layer}: {mat}.{suffix} must be [{rows}, 1] (a scale for each row), got {list(got[0].shape)}")
+                    got = [t.reshape(-1) for t in got]
+            out[mat + name] = torch.stack(got)
+            if not name and out[mat].dtype != (dtype or out["gate_proj"].dtype):
+                raise ValueError(f"layer {layer}: {mat} is {out[mat].dtype}, not {str(dtype or out['gate_proj'].dtype).removeprefix('torch.')}")
     if tensors:
         raise ValueError(f"layer {layer}: unexpected expert tensors {sorted(tensors)[:4]}")
     return out
@@ -128,12 +160,11 @@ class ExpertStore:
         / ``gate_up_proj_bias`` / ``down_proj`` ...), and the slot keeps the checkpoint's key
         order. ``tiled``: MXFP4 matrices are stored in the 16-row MFMA tile order of the fast
         decode instead (mx_tiles.tile_mxfp4; their scale tensors become the tile-scale areas).
-        FP8 checkpoints keep one tensor per expert: ``<e>.gate_proj.weight`` / ``up_proj`` / ``down_proj``
-        (e4m3) and their ``weight_scale_inv``; the slot is synth.fp8_layout's. Returns (store,
-        num_experts)."""
+        FP8, int8 and 16-bit checkpoints keep one tensor per expert: ``<e>.gate_proj.weight`` / ``up_proj`` / ``down_proj``,
+        e4m3 with their ``weight_scale_inv``, int8 with their ``weight_scale`` ([out, 1]), or bfloat16 / float16; the slot
+        is synth.fp8_layout's, int8_layout's or dense_layout's. Returns (store, num_experts)."""
         import json
         import os
-        import re
 
         from safetensors import safe_open
 
@@ -159,18 +190,18 @@ class ExpertStore:
         layers = sorted(layer_tensors) if layer_indices is None else [li for li in layer_indices if li in layer_tensors]
         if not layers:
             raise ValueError(f"No expert tensors found in {model_dir} (pattern *.layers.<i>.{prefix}*)")
-        fp8 = any(re.fullmatch(r"\d+\.\w+\.weight_scale_inv", n) for n in layer_tensors[layers[0]])
-        if fp8:
+        split = _split_format(list(layer_tensors[layers[0]]), layer_tensors[layers[0]])
+        if split:
             if tiled:
-                raise ValueError("tiled slots need MXFP4 experts; this checkpoint holds FP8 ones")
-            layer_tensors = {li: _stack_fp8(layer_tensors[li], li) for li in layers}
+                raise ValueError(f"tiled slots need MXFP4 experts; this checkpoint holds {split} ones")
+            layer_tensors = {li: _stack_experts(layer_tensors[li], li, split) for li in layers}
         first = layer_tensors[layers[0]]
         num_experts = int(next(iter(first.values())).shape[0])
         specs = {n: (tuple(t.shape[1:]), t.dtype) for n, t in first.items()}
         shapes = {n: (tuple(t.shape), t.dtype) for n, t in first.items()}
         if tiled:
             specs = mxfp4_tiled_specs(specs)
-        layout = TensorLayout(specs, align=16 if fp8 else 1)
+        layout = TensorLayout(specs, align=16 if split else 1)
         data = torch.empty((len(layers), num_experts, layout.total_bytes), dtype=torch.uint8,
                            pin_memory=torch.cuda.is_available())
         host = data.numpy()
@@ -216,9 +247,14 @@ class ExpertStore:
         return self._data[layer_idx].to(device)
 
     def expert_layout(self, act_fn=None):
-        """The kernels' tsa_expert_layout of these slots (MXFP4 and FP8 checkpoints)."""
-        from .expert_forward import fp8_expert_layout, is_fp8_layout, mxfp4_expert_layout
+        """The kernels' tsa_expert_layout of these slots."""
+        from .expert_forward import (dense_expert_layout, fp8_expert_layout, int8_expert_layout, is_fp8_layout, is_int8_layout,
+                                     mxfp4_expert_layout)
 
         if is_fp8_layout(self.layout):
             return fp8_expert_layout(self.layout, act_fn, self.expert_bytes)
+        if is_int8_layout(self.layout):
+            return int8_expert_layout(self.layout, act_fn, self.expert_bytes)
+        if "gate_up_proj_scales" not in self.layout.specs:
+            return dense_expert_layout(self.layout, act_fn, self.expert_bytes)
         return mxfp4_expert_layout(self.layout, act_fn, self.expert_bytes, tiled=self.tiled)

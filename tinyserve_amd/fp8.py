@@ -18,13 +18,15 @@ from . import ops
 logger = logging.getLogger(__name__)
 
 
-class FP8Module(nn.Module):
-    """A module whose e4m3 parameters and block scales (``*_scale_inv``) keep their types when the model around
-    it is cast (``.to(dtype)``, ``.half()``, ``.type(dtype)``): they are a format, not values of some precision."""
+class FormatModule(nn.Module):
+    """A module some of whose parameters (``_is_format``: codes and their scales) keep their types when the model
+    around it is cast (``.to(dtype)``, ``.half()``, ``.type(dtype)``): they are a format, not values of some precision."""
+
+    def _is_format(self, name: str, p: torch.Tensor) -> bool:
+        raise NotImplementedError
 
     def _apply(self, fn, recurse=True):
-        fixed = {id(p) for n, p in self._parameters.items()
-                 if p is not None and (p.dtype == torch.float8_e4m3fn or n.endswith("_scale_inv"))}
+        fixed = {id(p) for n, p in self._parameters.items() if p is not None and self._is_format(n, p)}
 
         def keep(t):
             if id(t) not in fixed:
@@ -34,6 +36,13 @@ class FP8Module(nn.Module):
             return (out if out.dtype == raw.dtype else raw.to(out.device)).view(t.dtype)
 
         return super()._apply(keep, recurse)
+
+
+class FP8Module(FormatModule):
+    """FormatModule for e4m3 parameters and block scales (``*_scale_inv``)."""
+
+    def _is_format(self, name: str, p: torch.Tensor) -> bool:
+        return p.dtype == torch.float8_e4m3fn or name.endswith("_scale_inv")
 
 
 class FP8Linear(FP8Module):
@@ -63,11 +72,10 @@ class FP8Linear(FP8Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
-def replace_linear_with_fp8(model: nn.Module, weights: dict[str, tuple[torch.Tensor, torch.Tensor]],
-                            device: torch.device | str = "cuda") -> int:
-    """Replace ``nn.Linear`` modules named in ``weights`` (path -> (weight, weight_scale_inv)) by
-    ``FP8Linear``, keeping their biases; returns the number replaced. Paths that do not resolve to an
-    ``nn.Linear`` are skipped; meta-device biases are dropped."""
+def replace_linears(model: nn.Module, weights: dict[str, tuple[torch.Tensor, torch.Tensor]], make) -> int:
+    """Replace ``nn.Linear`` modules named in ``weights`` (path -> (weight, scales)) by ``make(weight, scales, bias)``,
+    keeping their biases; returns the number replaced. Paths that do not resolve to an ``nn.Linear`` are skipped;
+    meta-device biases are dropped."""
     replaced = 0
     for name, (weight, scales) in weights.items():
         path, _, attr = name.rpartition(".")
@@ -79,7 +87,15 @@ def replace_linear_with_fp8(model: nn.Module, weights: dict[str, tuple[torch.Ten
         if not isinstance(old, nn.Linear):
             continue
         bias = old.bias if old.bias is not None and old.bias.device.type != "meta" else None
-        setattr(parent, attr, FP8Linear(weight, scales, bias, device))
+        setattr(parent, attr, make(weight, scales, bias))
         replaced += 1
+    return replaced
+
+
+def replace_linear_with_fp8(model: nn.Module, weights: dict[str, tuple[torch.Tensor, torch.Tensor]],
+                            device: torch.device | str = "cuda") -> int:
+    """Replace ``nn.Linear`` modules named in ``weights`` (path -> (weight, weight_scale_inv)) by
+    ``FP8Linear`` (replace_linears)."""
+    replaced = replace_linears(model, weights, lambda w, s, b: FP8Linear(w, s, b, device))
     logger.info("FP8Linear now backs %d linear layer(s)", replaced)
     return replaced

@@ -242,6 +242,9 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: t
 
 
 # ----------------------------------------------------------------------------- int8, a scale per token and row
+INT8_MAX_K = 131056  # values a row may have: the sums fit 32 bits
+
+
 def _int8_codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Quantised tokens (codes int8 [T, K], scales float32 [T]), checked."""
     if codes.dtype != torch.int8 or codes.dim() != 2:
@@ -444,9 +447,9 @@ def _n_slots(pool: torch.Tensor, layout: _lib.ExpertLayout) -> int:
 
 
 def _moe_rows(layout: _lib.ExpertLayout, x: torch.Tensor) -> torch.Tensor:
-    """x as contiguous rows of ``hidden`` values (from a multiple of 16 bytes on for FP8 experts)."""
+    """x as contiguous rows of ``hidden`` values (from a multiple of 16 bytes on for FP8, 16-bit and int8 experts)."""
     x2 = _rows(x, layout.hidden)
-    return _aligned(x2) if layout.format == _lib.EXPERT_FP8 else x2
+    return _aligned(x2) if layout.format in (_lib.EXPERT_FP8, _lib.EXPERT_DENSE, _lib.EXPERT_INT8) else x2
 
 
 def _moe_out(out: torch.Tensor | None, x2: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

@@ -257,3 +257,45 @@ def make_fp8_expert(rng: np.random.Generator, hidden: int, inter: int, sigma: fl
     for name, (r, c) in (("gate_proj", (inter, hidden)), ("up_proj", (inter, hidden)), ("down_proj", (hidden, inter))):
         e[name], e[name + "_scale_inv"] = make_fp8(rng, r, c, sigma)
     return e
+
+
+# ----------------------------------------------------------------------------- 16-bit and int8 experts
+def dense_layout(hidden: int, inter: int, dtype: torch.dtype = torch.bfloat16) -> TensorLayout:
+    """A 16-bit expert's slot: gate, up and down, filled up to a multiple of 16 bytes."""
+    return TensorLayout({"gate_proj": ((inter, hidden), dtype), "up_proj": ((inter, hidden), dtype),
+                         "down_proj": ((hidden, inter), dtype)}, align=16)
+
+
+def int8_layout(hidden: int, inter: int) -> TensorLayout:
+    """An int8 expert's slot: the matrices' codes, then their float32 scales per row, filled up to a multiple
+    of 16 bytes."""
+    return TensorLayout({
+        "gate_proj": ((inter, hidden), torch.int8),
+        "up_proj": ((inter, hidden), torch.int8),
+        "down_proj": ((hidden, inter), torch.int8),
+        "gate_proj_scale": ((inter,), torch.float32),
+        "up_proj_scale": ((inter,), torch.float32),
+        "down_proj_scale": ((hidden,), torch.float32),
+    }, align=16)
+
+
+def make_int8(rng: np.random.Generator, rows: int, cols: int, sigma: float = 0.03) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of an N(0, sigma) matrix [rows, cols], the largest value of each row at 127."""
+    w = rng.normal(0.0, sigma, (rows, cols)).astype(np.float32)
+    s = np.abs(w).max(1) / np.float32(127)
+    return torch.from_numpy(np.rint(w / s[:, None]).clip(-127, 127).astype(np.int8)), torch.from_numpy(s)
+
+
+def make_int8_expert(rng: np.random.Generator, hidden: int, inter: int, sigma: float = 0.03) -> dict[str, torch.Tensor]:
+    """The tensors of int8_layout."""
+    e = {}
+    for name, (r, c) in (("gate_proj", (inter, hidden)), ("up_proj", (inter, hidden)), ("down_proj", (hidden, inter))):
+        e[name], e[name + "_scale"] = make_int8(rng, r, c, sigma)
+    return e
+
+
+def make_dense_expert(rng: np.random.Generator, hidden: int, inter: int, dtype: torch.dtype = torch.bfloat16,
+                      sigma: float = 0.03) -> dict[str, torch.Tensor]:
+    """The tensors of dense_layout."""
+    shapes = (("gate_proj", (inter, hidden)), ("up_proj", (inter, hidden)), ("down_proj", (hidden, inter)))
+    return {name: torch.from_numpy(rng.normal(0.0, sigma, shape).astype(np.float32)).to(dtype) for name, shape in shapes}
