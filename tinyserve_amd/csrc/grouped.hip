@@ -3,9 +3,8 @@
 //     y[r, n] = sum_k x[rows[r] / top_k, k] w[e, n, k]  (+ bias[e, n]);
 // int8 operands are scaled as the plain product's are. Rows of no expert are zeros.
 //
-// One launch, nothing read back: the grid holds as many workgroups as any offsets can need, and each finds its
-// tile of rows by a prefix sum over the groups (a wave, four groups a lane; about 0.5 us, where a launch ahead
-// that writes a table takes 2 and more).
+// One launch, nothing read back: each workgroup finds its tiles by a prefix sum over the groups (a wave, four groups
+// a lane).
 #include "int8_common.h"
 #include "mm_epilogue.h"
 
@@ -36,115 +35,114 @@ __device__ __forceinline__ int wave_incl_sum(int v) {
     return v;
 }
 
-struct GroupedTile {
-    int expert;  // -1: rows of none
-    int row0, rows, tile;
-};
+// A workgroup's tiles (mm_pair's order; an entry: up to TM rows of a group). The rows ahead of the first group and
+// behind the last are groups of their own, of no expert. Offsets that do not ascend, or leave [0, R], give groups cut
+// to it: every row that is touched is one of the R.
+template <class C, class E>
+struct GroupedWork {
+    static constexpr int TM = C::TM;
+    const Grouped& p;
+    int entries;
+    int b[5], n[4], sum, incl;  // this lane's four groups (of the first 256): bounds, entries, their sums
+    MmRuns runs;
+    int expert, n0, row0, tn, next_expert, next_n0, next_row0, next_tn;
 
-// The tile of this workgroup: of all (rows of TM of a group, tile of N) pairs in order, each XCD takes a run (the
-// row tiles of an expert and the tiles of a row tile share an L2). The rows ahead of the first group and behind
-// the last are groups of their own, of no expert. Offsets that do not ascend, or leave [0, R], give groups cut to
-// it: every row that is touched is one of the R. False: nothing is left for this workgroup.
-template <int TM>
-__device__ __forceinline__ bool grouped_tile(const Grouped& p, GroupedTile& o) {
-    const int lane = (int)threadIdx.x & 63, G = p.E + 2;
-    auto bound = [&](int g) {  // where group g starts: 0, offsets[0 .. E], R
+    __device__ __forceinline__ int bound(int g) const {  // where group g starts: 0, offsets[0 .. E], R
         const int v = p.offsets[g < 1 ? 0 : g - 1 > p.E ? p.E : g - 1];
         return g < 1 ? 0 : g > p.E + 1 ? p.R : v < 0 ? 0 : v > p.R ? p.R : v;
-    };
-    int b[5], n[4], sum;
-    auto load = [&](int g0) {
+    }
+    __device__ __forceinline__ void load(int g0) {
+        const int lane = (int)threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < 5; ++j) b[j] = bound(g0 + 4 * lane + j);
         sum = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            n[j] = g0 + 4 * lane + j < G && b[j + 1] > b[j] ? (b[j + 1] - b[j] + TM - 1) / TM : 0;
+            n[j] = g0 + 4 * lane + j < p.E + 2 && b[j + 1] > b[j] ? (b[j + 1] - b[j] + TM - 1) / TM : 0;
             sum += n[j];
         }
-    };
-    int total = 0, incl = 0;
-    for (int g0 = 0; g0 < G; g0 += 256) {
-        load(g0);
         incl = wave_incl_sum(sum);
-        total += __builtin_amdgcn_readlane(incl, 63);
     }
-    const int all = total * p.tiles_n, lin = (int)blockIdx.x, xcd = lin & 7, q8 = all >> 3, rem = all & 7;
-    if ((lin >> 3) >= q8 + (xcd < rem ? 1 : 0)) return false;
-    const int wid = xcd * q8 + (xcd < rem ? xcd : rem) + (lin >> 3);
-    int entry = wid / p.tiles_n;
-    o.tile = wid % p.tiles_n;
-    for (int g0 = 0;; g0 += 256) {
-        if (G > 256) {
+    __device__ __forceinline__ int count() {
+        entries = 0;
+        for (int g0 = 0; g0 < p.E + 2; g0 += 256) {
             load(g0);
-            incl = wave_incl_sum(sum);
-            const int here = __builtin_amdgcn_readlane(incl, 63);
-            if (entry >= here) {
-                entry -= here;
-                continue;
-            }
+            entries += __builtin_amdgcn_readlane(incl, 63);
         }
-        int left = entry - (incl - sum), g = -1, r0 = 0, end = 0;  // in this lane's groups
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (g < 0 && left < n[j]) {
-                g = g0 + 4 * lane + j;
-                r0 = b[j] + TM * left;
-                end = b[j + 1];
-            }
-            left -= n[j];
-        }
-        const int l = __ffsll((unsigned long long)__ballot(incl > entry)) - 1;
-        g = __builtin_amdgcn_readlane(g, l);
-        o.row0 = __builtin_amdgcn_readlane(r0, l);
-        end = __builtin_amdgcn_readlane(end, l);
-        o.rows = end - o.row0 < TM ? end - o.row0 : TM;
-        o.expert = g >= 1 && g <= p.E ? g - 1 : -1;
-        return true;
+        return entries * p.tiles_n;
     }
-}
+    __device__ __forceinline__ explicit GroupedWork(const Grouped& p) : p(p), runs(count()) {}
+    __device__ __forceinline__ bool next() {
+        while (runs.next()) {
+            int entry, tile;
+            mm_pair(runs.at, entries, p.tiles_n, entry, tile);
+            next_n0 = tile * C::RN;
+            for (int g0 = 0;; g0 += 256) {
+                if (p.E + 2 > 256) {
+                    load(g0);
+                    const int here = __builtin_amdgcn_readlane(incl, 63);
+                    if (entry >= here) {
+                        entry -= here;
+                        continue;
+                    }
+                }
+                int left = entry - (incl - sum), g = -1, r0 = 0, end = 0;  // in this lane's groups
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (g < 0 && left < n[j]) {
+                        g = g0 + 4 * ((int)threadIdx.x & 63) + j;
+                        r0 = b[j] + TM * left;
+                        end = b[j + 1];
+                    }
+                    left -= n[j];
+                }
+                const int l = __ffsll((unsigned long long)__ballot(incl > entry)) - 1;
+                g = __builtin_amdgcn_readlane(g, l);
+                next_row0 = __builtin_amdgcn_readlane(r0, l);
+                end = __builtin_amdgcn_readlane(end, l);
+                next_tn = end - next_row0 < TM ? end - next_row0 : TM;
+                next_expert = g >= 1 && g <= p.E ? g - 1 : -1;
+                break;
+            }
+            if (next_expert >= 0) return true;
+            const int cols = p.N - next_n0 < C::RN ? p.N - next_n0 : C::RN;
+            for (int r = 0; r < next_tn; ++r)
+                for (int c = threadIdx.x; c < cols; c += C::THREADS)
+                    store_out(p.out.y, p.out.y_dtype, (int64_t)(next_row0 + r) * p.out.ldy + next_n0 + c, 0.0f);
+        }
+        return false;
+    }
+    __device__ __forceinline__ int picked(int row) const {  // row of x, -1 for one that is not there
+        const int a = p.rows[row];
+        return a >= 0 && a / p.top_k < p.x_rows ? a / p.top_k : -1;
+    }
+    __device__ __forceinline__ int token(int r) const { return p.rows ? picked(next_row0 + r) : r; }
+    __device__ __forceinline__ MmOperands<1> operands() const {
+        const uint8_t* w = p.w + next_expert * p.w_stride + (int64_t)next_n0 * p.KB;
+        const uint8_t* x = p.rows ? p.x : p.x + (int64_t)next_row0 * p.KB;
+        return MmOperands<1>{{w}, p.N - next_n0, x, (uint32_t)(p.rows ? p.x_rows : next_tn) * (uint32_t)p.KB, next_tn};
+    }
+    __device__ __forceinline__ void take() { expert = next_expert, n0 = next_n0, row0 = next_row0, tn = next_tn; }
+    __device__ __forceinline__ bool store(const typename E::acc (&acc)[C::MR][C::MT], uint8_t* out) const {
+        MmOut o = p.out;
+        if (o.bias) o.bias = static_cast<const uint8_t*>(o.bias) + (int64_t)expert * p.N * (o.bias_dtype == TSA_F32 ? 4 : 2);
+        auto scale = [&](int r) {
+            const int t = p.rows ? picked(row0 + r) : row0 + r;
+            return t >= 0 ? p.xs[t] : 0.0f;
+        };
+        return mm_store<C>(acc, o, out, n0, p.N, tn, [&](int r) { return (int64_t)(row0 + r); }, scale, p.ws + (int64_t)expert * p.N);
+    }
+};
 
 template <class C, class E>
 __global__ void __launch_bounds__(C::THREADS) grouped_kernel(Grouped p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    GroupedTile g;
-    if (!grouped_tile<C::TM>(p, g)) return;
-    const int n0 = g.tile * C::RN, row0 = g.row0, tn = g.rows;
-    if (g.expert < 0) {
-        const int cols = p.N - n0 < C::RN ? p.N - n0 : C::RN;
-        for (int r = 0; r < tn; ++r)
-            for (int c = threadIdx.x; c < cols; c += C::THREADS) store_out(p.out.y, p.out.y_dtype, (int64_t)(row0 + r) * p.out.ldy + n0 + c, 0.0f);
-        return;
-    }
-    auto token = [&](int r) {  // row of x, -1 for one that is not there
-        const int a = p.rows[row0 + r];
-        return a >= 0 && a / p.top_k < p.x_rows ? a / p.top_k : -1;
-    };
-    MmOperands<1> o;
-    o.w[0] = p.w + g.expert * p.w_stride + (int64_t)n0 * p.KB;
-    o.w_rows = p.N - n0;
-    o.KB = (uint32_t)p.KB;
-    typename E::acc acc[C::MR][C::MT];
-    if (p.rows) {
-        o.x = p.x;
-        o.x_records = (uint32_t)p.x_rows * (uint32_t)p.KB;
-    } else {
-        o.x = p.x + (int64_t)row0 * p.KB;
-        o.x_records = (uint32_t)tn * (uint32_t)p.KB;
-    }
-    mm_tile<C, E, 1>(o, smem, tn, [&](int r) { return p.rows ? token(r) : r; }, acc);
-    MmOut out = p.out;
-    if (out.bias) out.bias = static_cast<const uint8_t*>(out.bias) + (int64_t)g.expert * p.N * (out.bias_dtype == TSA_F32 ? 4 : 2);
-    auto scale = [&](int r) {
-        if (!p.rows) return p.xs[row0 + r];
-        const int t = token(r);
-        return t >= 0 ? p.xs[t] : 0.0f;
-    };
-    mm_store<C>(acc, out, n0, p.N, tn, [&](int r) { return (int64_t)(row0 + r); }, scale, p.ws + (int64_t)g.expert * p.N);
+    GroupedWork<C, E> work(p);
+    mm_run<C, E, 1, true>(work, (uint32_t)p.KB, smem);
 }
 
 template <class C, class E>
-hipError_t launch_grouped(const Grouped& p, hipStream_t st) {
+hipError_t launch_grouped(const Grouped& p, int per, hipStream_t st) {
     const void* fn = reinterpret_cast<const void*>(&grouped_kernel<C, E>);
     const hipError_t e = ensure_dynamic_lds(fn, C::LDS);
     if (e != hipSuccess) return e;
@@ -153,8 +151,7 @@ hipError_t launch_grouped(const Grouped& p, hipStream_t st) {
     void* args[] = {&q};
     // a group of n rows has at most n / TM + 1 tiles, and no more than n
     const int64_t groups = (int64_t)p.E + 2 < p.R ? p.E + 2 : p.R, tiles = p.R / C::TM + groups;
-    const int64_t grid = (tiles * q.tiles_n + 7) / 8 * 8;
-    return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(C::THREADS), args, C::LDS, st);
+    return hipLaunchKernel(fn, dim3(mm_grid(tiles * q.tiles_n, per)), dim3(C::THREADS), args, C::LDS, st);
 }
 
 using Grp128 = MmTile<4, 2, 4, 4, 3>;  // 256 rows x 128 tokens
@@ -165,10 +162,10 @@ using Grp16 = MmTile<4, 1, 1, 1, 4>;   // 64 x 16
 template <class E>
 hipError_t pick_grouped(const Grouped& p, hipStream_t st) {
     const int64_t R = p.R, n = p.E;
-    if (R > 48 * n) return launch_grouped<Grp128, E>(p, st);
-    if (R > 20 * n) return launch_grouped<Grp64, E>(p, st);
-    if (R > 8 * n) return launch_grouped<Grp32, E>(p, st);
-    return launch_grouped<Grp16, E>(p, st);
+    if (R > 48 * n) return launch_grouped<Grp128, E>(p, 1, st);
+    if (R > 20 * n) return launch_grouped<Grp64, E>(p, 2, st);
+    if (R > 8 * n) return launch_grouped<Grp32, E>(p, 1, st);
+    return launch_grouped<Grp16, E>(p, 2, st);
 }
 
 constexpr int64_t GROUPED_MAX_E = 65536;

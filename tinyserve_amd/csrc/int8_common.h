@@ -11,16 +11,52 @@
 namespace tsa {
 namespace {
 
-// The largest of the wave's values (magnitudes as bits: their integer order is the order of the values, an
-// infinity above all numbers, a NaN above it).
-template <int N>
-__device__ __forceinline__ uint32_t i8_wave_max(const float (&v)[N][8]) {
-    uint32_t m = 0;
+// 8 values as they lie in memory.
+template <int XT>
+struct I8Raw {
+    u32x4 w[XT == TSA_F32 ? 2 : 1];
+};
+
+// Chunk c (8 values) of a row of K values; past the row zeros. VEC: 16-byte aligned rows of whole chunks.
+template <int XT, bool VEC>
+__device__ __forceinline__ I8Raw<XT> i8_load(const uint8_t* row, int64_t K, int c) {
+    I8Raw<XT> v = {};
+    const int64_t k = (int64_t)8 * c;
+    if constexpr (VEC) {
+        if (k < K) {
+            const u32x4* p = reinterpret_cast<const u32x4*>(row);
+            if constexpr (XT == TSA_F32) v.w[0] = p[2 * c], v.w[1] = p[2 * c + 1];
+            else v.w[0] = p[c];
+        }
+    } else {
 #pragma unroll
-    for (int c = 0; c < N; ++c)
+        for (int e = 0; e < 8; ++e)
+            if (k + e < K) {
+                if constexpr (XT == TSA_F32) v.w[e >> 2][e & 3] = reinterpret_cast<const uint32_t*>(row)[k + e];
+                else v.w[0][e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[k + e] << (16 * (e & 1));
+            }
+    }
+    return v;
+}
+
+// The largest magnitude, as bits of the type (their integer order is the order of the values, an infinity above all
+// numbers, a NaN above it).
+template <int XT>
+__device__ __forceinline__ uint32_t i8_max(const I8Raw<XT>& v, uint32_t m) {
+    if constexpr (XT == TSA_F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[c][e]) & 0x7FFFFFFFu);
-    return wave_max_u32(m);
+        for (int e = 0; e < 8; ++e) m = max(m, v.w[e >> 2][e & 3] & 0x7FFFFFFFu);
+    } else {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) m = max(m, max(v.w[0][d] & 0x7FFFu, v.w[0][d] >> 16 & 0x7FFFu));
+    }
+    return m;
+}
+
+// Such bits as a float32's.
+template <int XT>
+__device__ __forceinline__ uint32_t i8_max_f32(uint32_t m) {
+    return XT == TSA_F32 ? m : XT == TSA_BF16 ? m << 16 : __float_as_uint(f16_bits_to_f32(m));
 }
 
 __device__ __forceinline__ float i8_scale(uint32_t max_bits) {
@@ -30,13 +66,19 @@ __device__ __forceinline__ float i8_scale(uint32_t max_bits) {
 }
 
 // The codes of 8 values of a token with scale s. The quotient by Markstein's correction, as the FP8 codes have
-// it (f8_codes8), which divides where bits of the remainder could underflow; EXACT (fp32 inputs) divides. |q| <=
+// it (f8_codes8), which divides where bits of the remainder could underflow; fp32 inputs divide. |q| <=
 // 127 (1 + 2^-23), so adding 1.5 2^23 rounds it to an integer, ties to even, in the sum's low bits.
-template <bool EXACT>
-__device__ __forceinline__ uint2 i8_codes8(const float (&v)[8], float s) {
-    float q[8];
+template <int XT>
+__device__ __forceinline__ uint2 i8_codes8(const I8Raw<XT>& raw, float s) {
     if (!(s == s)) return make_uint2(0u, 0u);
-    if (EXACT || !(s > F8_MIN_CORRECTED)) {
+    float v[8], q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (XT == TSA_F32) v[e] = __uint_as_float(raw.w[e >> 2][e & 3]);
+        else v[e] = XT == TSA_BF16 ? __uint_as_float(e & 1 ? raw.w[0][e >> 1] & 0xFFFF0000u : raw.w[0][e >> 1] << 16)
+                                   : f16_bits_to_f32(raw.w[0][e >> 1] >> (16 * (e & 1)));
+    }
+    if (XT == TSA_F32 || !(s > F8_MIN_CORRECTED)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] = v[e] / s;
     } else {
@@ -56,64 +98,47 @@ __device__ __forceinline__ uint2 i8_codes8(const float (&v)[8], float s) {
     return make_uint2(pack(b[0], b[1], b[2], b[3]), pack(b[4], b[5], b[6], b[7]));
 }
 
-// Chunk c (8 values) of a row of K values; past the row zeros. VEC: 16-byte aligned rows of whole chunks.
-template <int XT, bool VEC>
-__device__ __forceinline__ void i8_load8(const uint8_t* row, int64_t K, int c, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if constexpr (VEC) {
-        if ((int64_t)8 * c < K) f8_load8<XT>(row, c, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if ((int64_t)8 * c + e < K) v[e] = load_act(row, XT, (int64_t)8 * c + e);
-    }
-}
-
 // One row quantised by the W waves that call these together (tid: the thread's number among their 64 W). A thread
 // holds its first D chunks from i8_row_load on; a longer row's others are read twice. `top`: W words of LDS
 // that no one else uses (the barrier is the workgroup's: every wave of it calls).
 template <int XT, bool VEC, int W, int D>
-__device__ __forceinline__ void i8_row_load(const uint8_t* row, int64_t K, int tid, float (&v)[D][8]) {
+__device__ __forceinline__ void i8_row_load(const uint8_t* row, int64_t K, int tid, I8Raw<XT> (&v)[D]) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) i8_load8<XT, VEC>(row, K, tid + 64 * W * d, v[d]);
+    for (int d = 0; d < D; ++d) v[d] = i8_load<XT, VEC>(row, K, tid + 64 * W * d);
+}
+
+template <int XT, bool VEC>
+__device__ __forceinline__ void i8_put(const I8Raw<XT>& v, float s, uint8_t* codes, int64_t K, int c) {
+    const uint2 o = i8_codes8<XT>(v, s);
+    uint8_t* dst = codes + (int64_t)8 * c;
+    if constexpr (VEC) {
+        *reinterpret_cast<uint2*>(dst) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if ((int64_t)8 * c + e < K) dst[e] = (uint8_t)((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
+    }
 }
 
 template <int XT, bool VEC, int W, int D>
-__device__ __forceinline__ float i8_row_codes(const uint8_t* row, int64_t K, int tid, const float (&v)[D][8], uint8_t* codes, uint32_t* top) {
+__device__ __forceinline__ float i8_row_codes(const uint8_t* row, int64_t K, int tid, const I8Raw<XT> (&v)[D], uint8_t* codes, uint32_t* top) {
     const int chunks = (int)((K + 7) / 8);
-    uint32_t m = i8_wave_max(v);
-    for (int c = tid + 64 * W * D; c < (chunks + 63) / 64 * 64; c += 64 * W) {  // whole waves
-        float u[1][8];
-        i8_load8<XT, VEC>(row, K, c, u[0]);
-        m = max(m, i8_wave_max(u));
-    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int d = 0; d < D; ++d) m = i8_max<XT>(v[d], m);
+    for (int c = tid + 64 * W * D; c < chunks; c += 64 * W) m = i8_max<XT>(i8_load<XT, VEC>(row, K, c), m);
+    m = wave_max_u32(m);
     if constexpr (W > 1) {
         if ((tid & 63) == 0) top[tid >> 6] = m;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) m = max(m, top[w]);
     }
-    const float s = i8_scale(m);
-    auto put = [&](int c, const float (&u)[8]) {
-        const uint2 o = i8_codes8<XT == TSA_F32>(u, s);
-        uint8_t* dst = codes + (int64_t)8 * c;
-        if constexpr (VEC) {
-            *reinterpret_cast<uint2*>(dst) = o;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if ((int64_t)8 * c + e < K) dst[e] = (uint8_t)((e < 4 ? o.x : o.y) >> (8 * (e & 3)));
-        }
-    };
+    const float s = i8_scale(i8_max_f32<XT>(m));
 #pragma unroll
     for (int d = 0; d < D; ++d)
-        if (tid + 64 * W * d < chunks) put(tid + 64 * W * d, v[d]);
-    for (int c = tid + 64 * W * D; c < chunks; c += 64 * W) {
-        float u[8];
-        i8_load8<XT, VEC>(row, K, c, u);
-        put(c, u);
-    }
+        if (tid + 64 * W * d < chunks) i8_put<XT, VEC>(v[d], s, codes, K, tid + 64 * W * d);
+    for (int c = tid + 64 * W * D; c < chunks; c += 64 * W) i8_put<XT, VEC>(i8_load<XT, VEC>(row, K, c), s, codes, K, c);
     return s;
 }
 

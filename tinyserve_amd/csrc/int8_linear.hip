@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const uint8_t* __res
     const int64_t t = (int64_t)blockIdx.x * (4 / W) + g;
     if (W == 1 && t >= T) return;
     const int tid = (int)threadIdx.x - 64 * W * g;
-    float v[D][8];
+    I8Raw<XT> v[D];
     i8_row_load<XT, VEC, W, D>(x + t * K * ES, K, tid, v);
     const float s = i8_row_codes<XT, VEC, W, D>(x + t * K * ES, K, tid, v, codes + t * K, top + W * g);
     if (tid == 0) scales[t] = s;
@@ -49,14 +49,14 @@ struct I8Rows {
     int K, tiles_n, rows;  // rows: tokens of the largest tile
 };
 
-constexpr int I8R_NW = 8, I8R_D = 3;  // waves; steps of 128 columns a wave has in flight
+constexpr int I8R_NW = 8, I8R_D = 4;  // waves; steps of 128 columns a wave has in flight
 
 // Workgroup = 16 weight rows x 16 MT tokens; its waves take the steps of 128 columns in turn and their sums
 // meet in LDS. The weights come straight into the A operand's registers (every byte is read by one lane of
 // the workgroup), the tokens' codes from memory, or (XT: their dtype, up to 16 tokens) quantised here
 // into LDS while the weights are on their way.
-template <int XT, int MT>
-__global__ void __launch_bounds__(64 * I8R_NW) int8_rows_kernel(I8Rows p) {
+template <int XT, int MT, int HELD>
+__global__ void __launch_bounds__(64 * I8R_NW, 4) int8_rows_kernel(I8Rows p) {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int NT = 64 * I8R_NW;
     static_assert(XT < 0 || MT == 1, "one token tile is quantised here");
@@ -88,47 +88,41 @@ __global__ void __launch_bounds__(64 * I8R_NW) int8_rows_kernel(I8Rows p) {
         }
     };
     uint8_t* xc = smem;
-    uint32_t* top = reinterpret_cast<uint32_t*>(smem + p.rows * ld);  // [token]: the largest magnitude, then the scale's bits
+    float* xl = reinterpret_cast<float*>(smem + p.rows * ld);  // [token]: the scales
     if constexpr (XT >= 0) {
-        // pieces of 512 values, a wave each; the first ones are held from the search of the maximum on
-        const int per = (K + 511) / 512, pieces = per * tn;
-        constexpr int HELD = 2;
-        float v[HELD][8];
+        // 8 / `many` waves a token, pieces of 512 values in turn; the first HELD are held from the search of the maximum on
+        const int many = tn > 4 ? 8 : tn > 2 ? 4 : tn, per = I8R_NW / many, sub = wave % per, pieces = (K + 511) / 512;
+        for (int r0 = 0; r0 < tn; r0 += many) {  // workgroup-uniform; one turn where waves share a token
+            const int r = r0 + wave / per;
+            const uint8_t* row = xrow + (int64_t)(r < tn ? r : 0) * K * ES;
+            const int64_t len = r < tn ? K : 0;
+            I8Raw<XT> v[HELD];
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            const int u = wave + I8R_NW * h, r = u / per, c = u % per * 64 + lane;
-            i8_load8<XT, true>(xrow + (int64_t)(u < pieces ? r : 0) * K * ES, u < pieces ? K : 0, c, v[h]);
-        }
-        load(0);
-        if (tid < 16) top[tid] = 0;
-        __syncthreads();
+            for (int h = 0; h < HELD; ++h) v[h] = i8_load<XT, true>(row, len, 64 * (sub + per * h) + lane);
+            if (r0 == 0) load(0);
+            uint32_t m = 0;
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {
-            const int u = wave + I8R_NW * h;
-            float one[1][8];
+            for (int h = 0; h < HELD; ++h) m = i8_max<XT>(v[h], m);
+            for (int u = sub + per * HELD; u < pieces; u += per) m = i8_max<XT>(i8_load<XT, true>(row, len, 64 * u + lane), m);
+            m = wave_max_u32(m);
+            if (per > 1) {
+                uint32_t* top = reinterpret_cast<uint32_t*>(xl + 16);
+                if (lane == 0) top[wave] = m;
+                __syncthreads();
+                for (int w = 0; w < per; ++w) m = max(m, top[wave - sub + w]);
+            }
+            if (r >= tn) continue;
+            const float s = i8_scale(i8_max_f32<XT>(m));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) one[0][e] = v[h][e];
-            const uint32_t m = i8_wave_max(one);
-            if (u < pieces && lane == 0) atomicMax(&top[u / per], m);
-        }
-        for (int u = wave + I8R_NW * HELD; u < pieces; u += I8R_NW) {
-            float one[1][8];
-            i8_load8<XT, true>(xrow + (int64_t)(u / per) * K * ES, K, u % per * 64 + lane, one[0]);
-            const uint32_t m = i8_wave_max(one);
-            if (lane == 0) atomicMax(&top[u / per], m);
-        }
-        __syncthreads();
-        auto put = [&](int u, const float (&a)[8]) {
-            const int r = u / per, c = u % per * 64 + lane;
-            if (8 * c < steps * MMB) *reinterpret_cast<uint2*>(xc + r * ld + 8 * c) = i8_codes8<XT == TSA_F32>(a, i8_scale(top[r]));
-        };
-#pragma unroll
-        for (int h = 0; h < HELD; ++h)
-            if (wave + I8R_NW * h < pieces) put(wave + I8R_NW * h, v[h]);
-        for (int u = wave + I8R_NW * HELD; u < pieces; u += I8R_NW) {
-            float a[8];
-            i8_load8<XT, true>(xrow + (int64_t)(u / per) * K * ES, K, u % per * 64 + lane, a);
-            put(u, a);
+            for (int h = 0; h < HELD; ++h) {
+                const int c = 64 * (sub + per * h) + lane;
+                if (8 * c < steps * MMB) *reinterpret_cast<uint2*>(xc + r * ld + 8 * c) = i8_codes8<XT>(v[h], s);
+            }
+            for (int u = sub + per * HELD; u < pieces; u += per) {
+                const int c = 64 * u + lane;
+                if (8 * c < steps * MMB) *reinterpret_cast<uint2*>(xc + r * ld + 8 * c) = i8_codes8<XT>(i8_load<XT, true>(row, len, c), s);
+            }
+            if (lane == 0 && sub == 0) xl[r] = s;
         }
         __syncthreads();
     } else {
@@ -159,7 +153,7 @@ __global__ void __launch_bounds__(64 * I8R_NW) int8_rows_kernel(I8Rows p) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int t = (tid + NT * m) >> 4;  // of output tid + NT m, below
-        if constexpr (XT >= 0) sc[m] = t < tn ? i8_scale(top[t]) : 0.0f;
+        if constexpr (XT >= 0) sc[m] = t < tn ? xl[t] : 0.0f;
         else sc[m] = t < tn ? p.xs[t0 + t] : 0.0f;
     }
     __syncthreads();
@@ -182,14 +176,14 @@ __global__ void __launch_bounds__(64 * I8R_NW) int8_rows_kernel(I8Rows p) {
 }
 
 int i8r_lds(int xt, int mt, int64_t K, int rows) {
-    const int red = I8R_NW * 256 * mt * 4, x = xt >= 0 ? rows * (int)((K + MMB - 1) / MMB * MMB + 16) + 64 : 0;
+    const int red = I8R_NW * 256 * mt * 4, x = xt >= 0 ? rows * (int)((K + MMB - 1) / MMB * MMB + 16) + 128 : 0;
     return x > red ? x : red;
 }
 
-template <int XT, int MT>
+template <int XT, int MT, int HELD>
 hipError_t launch_rows(const I8Rows& p, hipStream_t st) {
     const int lds = i8r_lds(XT, MT, p.K, p.rows);
-    const void* fn = reinterpret_cast<const void*>(&int8_rows_kernel<XT, MT>);
+    const void* fn = reinterpret_cast<const void*>(&int8_rows_kernel<XT, MT, HELD>);
     const hipError_t e = ensure_dynamic_lds(fn, lds);
     if (e != hipSuccess) return e;
     // a launch ends at 2^32 threads, 2^23 of these workgroups: more rows than that go in several
@@ -209,6 +203,13 @@ hipError_t launch_rows(const I8Rows& p, hipStream_t st) {
     return hipSuccess;
 }
 
+// Quantised inside: two pieces a wave held for the fewest tokens, else eight (of float32 values four; more are read twice).
+template <int XT>
+hipError_t launch_linear(const I8Rows& p, hipStream_t st) {
+    const int per = I8R_NW / (p.T > 4 ? 8 : p.T > 2 ? 4 : (int)p.T), pieces = (p.K + 511) / 512;
+    return pieces <= 2 * per ? launch_rows<XT, 1, 2>(p, st) : launch_rows<XT, 1, XT == TSA_F32 ? 4 : 8>(p, st);
+}
+
 // ---------------------------------------------------------------- many tokens
 struct I8Gemm {
     const uint8_t* w;
@@ -216,79 +217,91 @@ struct I8Gemm {
     const uint8_t* x;
     const float* xs;
     MmOut out;
-    int T, N, K, tiles_t;
+    int T, N, K, tiles_n, tiles_t;
+};
+
+// The product's tiles in bands of 8 row tiles, token tile by token tile (about square pieces of the product at a time
+// share an XCD's L2).
+template <class C>
+struct I8Work {
+    const I8Gemm& p;
+    MmRuns runs;
+    int n0, t0, tn, next_n0, next_t0, next_tn;
+    __device__ __forceinline__ explicit I8Work(const I8Gemm& p) : p(p), runs(p.tiles_n * p.tiles_t) {}
+    __device__ __forceinline__ bool next() {
+        if (!runs.next()) return false;
+        constexpr int BAND = 8;
+        const int band = runs.at / (BAND * p.tiles_t), in = runs.at - band * BAND * p.tiles_t;
+        const int deep = p.tiles_n - BAND * band < BAND ? p.tiles_n - BAND * band : BAND;  // row tiles of the band
+        next_n0 = (BAND * band + in % deep) * C::RN;
+        next_t0 = in / deep * C::TM;
+        next_tn = p.T - next_t0 < C::TM ? p.T - next_t0 : C::TM;
+        return true;
+    }
+    __device__ __forceinline__ MmOperands<1> operands() const {
+        return MmOperands<1>{{p.w + (int64_t)next_n0 * p.K}, p.N - next_n0, p.x + (int64_t)next_t0 * p.K, (uint32_t)next_tn * (uint32_t)p.K, next_tn};
+    }
+    __device__ __forceinline__ void take() { n0 = next_n0, t0 = next_t0, tn = next_tn; }
+    __device__ __forceinline__ bool store(const v4i (&acc)[C::MR][C::MT], uint8_t* out) const {
+        return mm_store<C>(acc, p.out, out, n0, p.N, tn, [&](int r) { return (int64_t)(t0 + r); }, [&](int r) { return p.xs[t0 + r]; }, p.ws);
+    }
 };
 
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) int8_gemm_kernel(I8Gemm p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    // Workgroups are dealt round the 8 XCDs by linear id: renumbered so that each XCD takes a run, and
-    // within it bands of 8 row tiles, token tile by token tile (about square pieces of the product at
-    // a time share one L2).
-    const int total = (int)gridDim.x, wid = xcd_run((int)blockIdx.x, total);
-    constexpr int BAND = 8;
-    const int rows = total / p.tiles_t, band = wid / (BAND * p.tiles_t), in = wid - band * BAND * p.tiles_t;
-    const int deep = rows - BAND * band < BAND ? rows - BAND * band : BAND;  // row tiles of the band
-    const int n0 = (BAND * band + in % deep) * C::RN, t0 = in / deep * C::TM;
-    const int tn = p.T - t0 < C::TM ? p.T - t0 : C::TM;
-    MmOperands<1> o;
-    o.w[0] = p.w + (int64_t)n0 * p.K;
-    o.w_rows = p.N - n0;
-    o.x = p.x + (int64_t)t0 * p.K;
-    o.x_records = (uint32_t)tn * (uint32_t)p.K;
-    o.KB = (uint32_t)p.K;
-    v4i acc[C::MR][C::MT];
-    mm_tile<C, MmI8, 1>(o, smem, tn, [](int r) { return r; }, acc);
-    mm_store<C>(acc, p.out, n0, p.N, tn, [&](int r) { return (int64_t)(t0 + r); },
-                [&](int r) { return p.xs[t0 + r]; }, p.ws);
+    I8Work<C> work(p);
+    mm_run<C, MmI8, 1, false>(work, (uint32_t)p.K, smem);
 }
 
 template <class C>
-hipError_t launch_gemm(const I8Gemm& p, hipStream_t st) {
+hipError_t launch_gemm(const I8Gemm& p, int per, hipStream_t st) {
     const void* fn = reinterpret_cast<const void*>(&int8_gemm_kernel<C>);
     const hipError_t e = ensure_dynamic_lds(fn, C::LDS);
     if (e != hipSuccess) return e;
     I8Gemm q = p;
+    q.tiles_n = (p.N + C::RN - 1) / C::RN;
     q.tiles_t = (p.T + C::TM - 1) / C::TM;
     void* args[] = {&q};
-    const int64_t grid = (int64_t)((p.N + C::RN - 1) / C::RN) * q.tiles_t;
-    return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(C::THREADS), args, C::LDS, st);
+    return hipLaunchKernel(fn, dim3(mm_grid((int64_t)q.tiles_n * q.tiles_t, per)), dim3(C::THREADS), args, C::LDS, st);
 }
 
-using TileA = MmTile<2, 4, 8, 4, 2>;  // 256 rows x 256 tokens
+using TileA = MmTile<4, 2, 4, 8, 2>;  // 256 rows x 256 tokens
 using TileB = MmTile<4, 2, 4, 4, 3>;  // 256 x 128
 using TileC = MmTile<2, 2, 4, 4, 2>;  // 128 x 128
 using TileD = MmTile<4, 1, 2, 4, 3>;  // 128 x 64
 using TileE = MmTile<4, 1, 1, 2, 4>;  // 64 x 32
 
-// The tile (A .. E as 0 .. 4) with the least rounds x round time, a round being `per` workgroups on
-// every CU; -1 if every tile needs more workgroups than a launch takes (2^32 threads).
+// The tile (A .. E as 0 .. 4) with the least rounds x round time, a round being `per` workgroups on every CU; -1 if
+// every tile gives 2^30 of them or more.
+struct GemmTile { int rows, tok, per, cost; };
+constexpr GemmTile gemm_tiles[5] = {{TileA::RN, TileA::TM, 1, 45},
+                                    {TileB::RN, TileB::TM, 1, 26},
+                                    {TileC::RN, TileC::TM, 2, 32},
+                                    {TileD::RN, TileD::TM, 2, 20},
+                                    {TileE::RN, TileE::TM, 3, 13}};
 int gemm_tile(int64_t T, int64_t N) {
-    struct Tile { int rows, tok, threads, per, cost; };
-    constexpr Tile tiles[5] = {{TileA::RN, TileA::TM, TileA::THREADS, 1, 45},
-                               {TileB::RN, TileB::TM, TileB::THREADS, 1, 26},
-                               {TileC::RN, TileC::TM, TileC::THREADS, 2, 32},
-                               {TileD::RN, TileD::TM, TileD::THREADS, 2, 20},
-                               {TileE::RN, TileE::TM, TileE::THREADS, 3, 13}};
     const int64_t cus = num_cus() > 0 ? num_cus() : 256;
     int best = -1;
     int64_t least = INT64_MAX;
     for (int i = 0; i < 5; ++i) {
-        const int64_t wgs = (N + tiles[i].rows - 1) / tiles[i].rows * ((T + tiles[i].tok - 1) / tiles[i].tok);
-        if (wgs * tiles[i].threads >= (int64_t)1 << 32) continue;
-        const int64_t cost = (wgs + cus * tiles[i].per - 1) / (cus * tiles[i].per) * tiles[i].cost;
+        const GemmTile& t = gemm_tiles[i];
+        const int64_t tiles = (N + t.rows - 1) / t.rows * ((T + t.tok - 1) / t.tok);
+        if (tiles >= (int64_t)1 << 30) continue;
+        const int64_t cost = (tiles + cus * t.per - 1) / (cus * t.per) * t.cost;
         if (cost < least) least = cost, best = i;
     }
     return best;
 }
 
 hipError_t pick_gemm(const I8Gemm& p, hipStream_t st) {
-    switch (gemm_tile(p.T, p.N)) {
-        case 0: return launch_gemm<TileA>(p, st);
-        case 1: return launch_gemm<TileB>(p, st);
-        case 2: return launch_gemm<TileC>(p, st);
-        case 3: return launch_gemm<TileD>(p, st);
-        default: return launch_gemm<TileE>(p, st);
+    const int i = gemm_tile(p.T, p.N), per = gemm_tiles[i].per;
+    switch (i) {
+        case 0: return launch_gemm<TileA>(p, per, st);
+        case 1: return launch_gemm<TileB>(p, per, st);
+        case 2: return launch_gemm<TileC>(p, per, st);
+        case 3: return launch_gemm<TileD>(p, per, st);
+        default: return launch_gemm<TileE>(p, per, st);
     }
 }
 
@@ -371,11 +384,16 @@ extern "C" int tsa_int8_matmul(const void* codes, const float* scales, int64_t T
         return TSA_OK;
     }
     const I8Rows p = rows_params(codes, scales, T, K, w, w_scales, N, out);
-    TSA_HIP_CHECK(T <= 16 ? (launch_rows<-1, 1>(p, as_stream(stream))) : (launch_rows<-1, 2>(p, as_stream(stream))));
+    TSA_HIP_CHECK(T <= 16 ? (launch_rows<-1, 1, 0>(p, as_stream(stream))) : (launch_rows<-1, 2, 0>(p, as_stream(stream))));
     return TSA_OK;
 }
 
-static bool linear_in_one(int64_t T, int64_t K) { return T <= 16 && i8r_lds(0, 1, K, (int)T) <= 128 * 1024; }
+// Whether few enough tokens are quantised inside the product's launch: the second launch costs a call that is made by
+// itself 3.3 us of host time (9.7 to 10 us, whatever the sizes), while every group of 8 tokens here adds a load latency and
+// its arithmetic to every workgroup. us of one launch / two: calls one by one, 2880 x 2880, 2048 x 4096 and 5760 x 2880, 8 tokens
+// 6.3, 7.2 and 8.0 / 9.7, 12 tokens 7.0, 8.0 and 9.6 / 9.7, 16 tokens 8.0, 9.3 and 10.9 / 9.8; inside a graph, 8 tokens 7.0, 8.0 and
+// 8.8 / 7.1, 8.7 and 8.9, 12 tokens 7.8, 8.9 and 10.5 / 7.3, 9.1 and 9.1.
+static bool linear_in_one(int64_t T, int64_t K) { return T <= 12 && i8r_lds(0, 1, K, (int)T) <= 128 * 1024; }
 static int64_t linear_ws(int64_t T, int64_t K) { return linear_in_one(T, K) ? 0 : (T * K + 255) / 256 * 256 + T * 4; }
 
 extern "C" int tsa_int8_linear_workspace_size(int64_t T, int64_t K, int64_t* bytes) {
@@ -398,8 +416,8 @@ extern "C" int tsa_int8_linear(const void* x, int x_dtype, int64_t T, int64_t K,
     hipStream_t st = as_stream(stream);
     if (linear_in_one(T, K)) {
         const I8Rows p = rows_params(x, nullptr, T, K, w, w_scales, N, mm_out(y, y_dtype, N, bias, bias_dtype));
-        TSA_HIP_CHECK(x_dtype == TSA_F32 ? (launch_rows<TSA_F32, 1>(p, st))
-                      : x_dtype == TSA_F16 ? (launch_rows<TSA_F16, 1>(p, st)) : (launch_rows<TSA_BF16, 1>(p, st)));
+        TSA_HIP_CHECK(x_dtype == TSA_F32 ? launch_linear<TSA_F32>(p, st)
+                      : x_dtype == TSA_F16 ? launch_linear<TSA_F16>(p, st) : launch_linear<TSA_BF16>(p, st));
         return TSA_OK;
     }
     TSA_REQUIRE(workspace && workspace_bytes >= linear_ws(T, K), TSA_ERR_WORKSPACE,

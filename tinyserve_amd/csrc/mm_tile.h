@@ -1,5 +1,5 @@
-// The tile of the products of int8 and 16-bit matrices over many tokens: RN weight rows x TM tokens of a
-// workgroup of WR x WT waves, each MR x MT tiles of 16 x 16.
+// Products of int8 and 16-bit matrices over many tokens: tiles of RN weight rows x TM tokens, each by a workgroup
+// of WR x WT waves with MR x MT tiles of 16 x 16.
 //
 // y[n, t] = sum_k w[n, k] x[t, k], on v_mfma_i32_16x16x64_i8 or v_mfma_f32_16x16x32_{bf16,f16}: all of
 // them take 16 bytes a lane of either operand, so the tile counts in bytes. Lane 16 q + i holds bytes 16 q ..
@@ -12,6 +12,9 @@
 // reads at once then fall on distinct banks. The barrier sits between a step's two products: by then the
 // second half's operands are in registers, so the stage is free for the copies of step s + S, which go out
 // among the second half's products, as do the LDS reads of step s + 1.
+//
+// A workgroup works through tiles one after the other, and their steps are one stream: the last S steps of a tile
+// issue the copies of the next tile's first, and the results go out while those land.
 #pragma once
 
 #include "lds_copy.h"
@@ -56,8 +59,10 @@ struct MmTile {
     static constexpr int NW = WR * WT, THREADS = 64 * NW, RN = 16 * WR * MR, TM = 16 * WT * MT;
     static constexpr int NXW = RN / 8 / NW, NXT = (TM + 8 * NW - 1) / (8 * NW);  // copies of 8 rows, a wave's
     static constexpr int PER = NXW + NXT;                                        // those of a step
-    static constexpr int STAGE = (RN + 8 * NW * NXT) * MMB, LDS = S * STAGE;
-    static_assert(RN % (8 * NW) == 0 && (S - 1) * PER < 63 && S >= 2, "tile");
+    static constexpr int STAGE = (RN + 8 * NW * NXT) * MMB;
+    static constexpr int OUT = 16 * MR * 32;  // a wave's place for 16 tokens' results of 16 bits
+    static constexpr int LDS = S * STAGE + NW * OUT;
+    static_assert(RN % (8 * NW) == 0 && (S - 1) * PER + MR * MT < 63 && S >= 2 && LDS <= 160 * 1024, "tile");
 };
 
 // What a tile multiplies. Weight row r of the tile (r < RN) is row r of w[r / (RN / PARTS)] counted
@@ -67,27 +72,38 @@ struct MmOperands {
     const uint8_t* w[PARTS];  // first row of the tile
     int w_rows;               // rows there are from it on (those past RN / PARTS are not read)
     const uint8_t* x;
-    uint32_t x_records;       // its bytes, below 2^31
-    uint32_t KB;              // bytes of a row of either, a multiple of 16
+    uint32_t x_records;       // its bytes, at most 2^31
+    int tokens;
 };
 
+// This wave's copies have landed but for the newest N, and its LDS reads are done; then the barrier. `stores`: another
+// STORES of the newest operations are stores that nothing here waits for (reads and writes are counted together, in
+// the order of their issue).
+template <int N, int STORES>
+__device__ __forceinline__ void mm_wait(bool stores) {
+    if (stores) wait_copies_barrier<N + STORES>();
+    else wait_copies_barrier<N>();
+}
+
+// Works through `work`'s tiles. KB: bytes of a row of either operand, a multiple of 16.
+//   bool work.next(): the next tile becomes work's pending one (uniform); false: there is none
+//   MmOperands<PARTS> work.operands(), int work.token(r): of the pending tile; the row of x of its token r (-1: zeros);
+//     GATHER false: token r is row r
+//   void work.take(): the pending tile becomes the current one
+//   bool work.store(acc, out): the current tile's results; `out`: this wave's place in LDS. True: at least MR MT / 2
+//     stores were the last that was done.
 // acc[m][t]: rows 4 q .. 4 q + 3 of tile m, token 16 t + i, for lane 16 q + i of the wave. Tile m is
-// the wave's m-th: of its MR, the first MR / PARTS belong to part 0. `token(r)`: row of x of the
-// tile's token r, -1 from `tokens` on (and for a row of zeros).
-template <class C, class E, int PARTS, class Token>
-__device__ __forceinline__ void mm_tile(const MmOperands<PARTS>& p, uint8_t* smem, int tokens, Token token,
-                                        typename E::acc (&acc)[C::MR][C::MT]) {
-    constexpr int MR = C::MR, MT = C::MT, S = C::S, HALF = C::RN / PARTS, MP = MR / PARTS;
+// the wave's m-th: of its MR, the first MR / PARTS belong to part 0.
+template <class C, class E, int PARTS, bool GATHER, class Work>
+__device__ __forceinline__ void mm_run(Work& work, uint32_t KB, uint8_t* smem) {
+    constexpr int MR = C::MR, MT = C::MT, S = C::S, HALF = C::RN / PARTS, MP = MR / PARTS, STORES = MR * MT / 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
     const int wr = wave % C::WR, wt = wave / C::WR;
-    const uint32_t KB = p.KB, lds0 = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-    const int steps = (int)((KB + MMB - 1) / MMB);
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+    const int all = (int)((KB + MMB - 1) / MMB), steps = all > S ? all : S;  // short rows: steps of zeros
 
     // copy j of this wave fills rows 8 (NX wave + j) + lane / 8, slot lane % 8
-    buf_v4i rw[PARTS];
-#pragma unroll
-    for (int h = 0; h < PARTS; ++h) rw[h] = buf_desc(p.w[h], (uint32_t)(p.w_rows < HALF ? p.w_rows : HALF) * KB);
-    const buf_v4i rx = buf_desc(p.x, p.x_records);
+    buf_v4i rw[PARTS], rx;
     uint32_t wo[C::NXW], xo[C::NXT];
     auto chunk = [&](int n) { return (uint32_t)((lane & 7) ^ ((4 * n + (lane >> 4)) & 7)); };  // of copy n's rows
 #pragma unroll
@@ -97,94 +113,162 @@ __device__ __forceinline__ void mm_tile(const MmOperands<PARTS>& p, uint8_t* sme
     }
 #pragma unroll
     for (int j = 0; j < C::NXT; ++j) {
-        const int n = C::NXT * wave + j, r = 8 * n + (lane >> 3), row = r < tokens ? token(r) : -1;
-        xo[j] = row < 0 ? 0x80000000u : (uint32_t)row * KB + 16u * chunk(n);
+        const int n = C::NXT * wave + j;
+        xo[j] = (uint32_t)(8 * n + (lane >> 3)) * KB + 16u * chunk(n);  // past x's records: zeros
     }
     uint32_t at[2];  // this lane's column in copies of even and odd number
 #pragma unroll
     for (int n = 0; n < 2; ++n) at[n] = 16u * chunk(n);
+    int tokens = 0, pending = 0;  // of the tile whose products run, and of the one whose copies go out
+    // the copies' tile becomes work's pending one (none: buffers without bytes)
+    auto setup = [&](bool there) {
+        if (!there) {
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) rw[h] = buf_desc(smem, 0);
+            rx = buf_desc(smem, 0);
+            return;
+        }
+        const MmOperands<PARTS> p = work.operands();
+        pending = p.tokens;
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) rw[h] = buf_desc(p.w[h], (uint32_t)(p.w_rows < HALF ? p.w_rows : HALF) * KB);
+        rx = buf_desc(p.x, p.x_records);
+        if constexpr (GATHER) {
+#pragma unroll
+            for (int j = 0; j < C::NXT; ++j) {
+                const int n = C::NXT * wave + j, r = 8 * n + (lane >> 3), row = r < p.tokens ? work.token(r) : -1;
+                xo[j] = row < 0 ? 0x80000000u : (uint32_t)row * KB + 16u * chunk(n);
+            }
+        }
+    };
     // copy j (of PER) of step s. Columns past K and steps past the last read zeros, so every step issues as
     // many. (The scalar offset stays inside the buffers: the range check may subtract it from their size.)
     auto issue = [&](int j, int s, int stage) {
         const uint32_t col = (uint32_t)MMB * (uint32_t)s, base = lds0 + (uint32_t)stage * C::STAGE;
-        const uint32_t soff = s < steps ? col : 0u;
+        const uint32_t soff = s < all ? col : 0u;
         const int n = j < C::NXW ? C::NXW * wave + j : C::NXT * wave + j - C::NXW;
         const bool in = col + (n & 1 ? at[1] : at[0]) < KB;
         if (j < C::NXW) lds_copy16(rw[PARTS == 1 ? 0 : 8 * n / HALF], in ? wo[j] : 0x80000000u, soff, base + 1024u * (uint32_t)n);
         else lds_copy16(rx, in ? xo[j - C::NXW] : 0x80000000u, soff, base + (uint32_t)C::RN * MMB + 1024u * (uint32_t)n);
     };
 
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[m][t] = typename E::acc{0, 0, 0, 0};
-
     const int frag = i * MMB + 16 * (q ^ (i >> 1));  // chunk q of row i of a tile; chunk q + 4 is 64 off by xor
-    auto read_a = [&](const uint8_t* wl, int m, int h) {
-        return *reinterpret_cast<const u32x4*>(wl + (m / MP * HALF + (wr * MP + m % MP) * 16) * MMB + (frag ^ (64 * h)));
+    u32x4 A[2][MR], Bv[2][MT];
+    typename E::acc acc[MR][MT];
+    auto fetch = [&](const uint8_t* wl, int m, int h) {  // what row tile m's turn brings of the next half
+        A[h][m] = *reinterpret_cast<const u32x4*>(wl + (m / MP * HALF + (wr * MP + m % MP) * 16) * MMB + (frag ^ (64 * h)));
+#pragma unroll
+        for (int t = m * MT / MR; t < (m + 1) * MT / MR; ++t)
+            Bv[h][t] = *reinterpret_cast<const u32x4*>(wl + (C::RN + (wt * MT + t) * 16) * MMB + (frag ^ (64 * h)));
     };
-    auto read_b = [&](const uint8_t* wl, int t, int h) {
-        return *reinterpret_cast<const u32x4*>(wl + (C::RN + (wt * MT + t) * 16) * MMB + (frag ^ (64 * h)));
-    };
+
+    bool more = work.next();
+    if (!more) return;
+    setup(true);
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int j = 0; j < C::PER; ++j) issue(j, s, s);
-
-    // The steps, for a wave whose first LIVE tiles of tokens hold any.
-    auto steps_of = [&](auto live) {
-        constexpr int LIVE = decltype(live)::value;
-        u32x4 A[2][MR], Bv[2][MT];
-        auto fetch = [&](const uint8_t* wl, int m, int h) {  // what row tile m's turn brings of the next half
-            if (LIVE == 0) return;
-            A[h][m] = read_a(wl, m, h);
+    wait_copies_barrier<(S - 1) * C::PER>();
+    int stage = 0;
+    bool stored = false;  // the tile before left its stores behind
+    do {
+        work.take();
+        tokens = pending;
+        // (read again after a tile's results: held through them, the operands would take too many registers)
 #pragma unroll
-            for (int t = m * LIVE / MR; t < (m + 1) * LIVE / MR; ++t) Bv[h][t] = read_b(wl, t, h);
-        };
+        for (int m = 0; m < MR; ++m) fetch(smem + stage * C::STAGE, m, 0);
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[m][t] = typename E::acc{0, 0, 0, 0};
+        // token tiles that hold none (a short last tile of a prompt, an expert with few) are left out, by halves
+        constexpr int H0 = (MT + 1) / 2;
+        const int live = (tokens - 16 * MT * wt + 15) / 16;
         auto products = [&](int m, int h) {
+            if (live > 0) {
 #pragma unroll
-            for (int t = 0; t < LIVE; ++t) acc[m][t] = E::mfma(A[h][m], Bv[h][t], acc[m][t]);
+                for (int t = 0; t < H0; ++t) acc[m][t] = E::mfma(A[h][m], Bv[h][t], acc[m][t]);
+            }
+            if (live > H0) {
+#pragma unroll
+                for (int t = H0; t < MT; ++t) acc[m][t] = E::mfma(A[h][m], Bv[h][t], acc[m][t]);
+            }
         };
-        wait_copies_barrier<(S - 1) * C::PER>();
-#pragma unroll
-        for (int m = 0; m < MR; ++m) fetch(smem, m, 0);
-        int stage = 0;
-        for (int s = 0; s < steps; ++s) {
-            const uint8_t* wl = smem + stage * C::STAGE;
-#pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                fetch(wl, m, 1);
-                products(m, 0);
-                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {  // the steps whose copies are this tile's, then those of the next
+            if (part) {
+                more = work.next();
+                setup(more);
             }
-            // every wave has read this stage, and step s + 1 has landed
-            wait_copies_barrier<(S - 2) * C::PER>();
-            const int next = stage + 1 == S ? 0 : stage + 1;
-            const uint8_t* wn = smem + next * C::STAGE;
+            const int s1 = part ? steps : steps - S, ahead = part ? S - steps : S;
+#pragma unroll 1
+            for (int s = part ? steps - S : 0; s < s1; ++s) {
+                const uint8_t* wl = smem + stage * C::STAGE;
 #pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                fetch(wn, m, 0);
-                products(m, 1);
+                for (int m = 0; m < MR; ++m) {
+                    fetch(wl, m, 1);
+                    products(m, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // every wave has read this stage, and the next step has landed
+                mm_wait<(S - 2) * C::PER, STORES>(stored && s < S - 1);
+                const int next = stage + 1 == S ? 0 : stage + 1;
+                const uint8_t* wn = smem + next * C::STAGE;
 #pragma unroll
-                for (int j = m * C::PER / MR; j < (m + 1) * C::PER / MR; ++j) issue(j, s + S, stage);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int m = 0; m < MR; ++m) {
+                    fetch(wn, m, 0);
+                    products(m, 1);
+#pragma unroll
+                    for (int j = m * C::PER / MR; j < (m + 1) * C::PER / MR; ++j) issue(j, s + ahead, stage);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                stage = next;
             }
-            stage = next;
         }
-    };
-    // tiles without tokens (a short last tile of a prompt, an expert with few) are left out
-    const int live = (tokens - 16 * MT * wt + 15) / 16;
-    if (live > (MT + 1) / 2) steps_of(std::integral_constant<int, MT>{});
-    else if (MT > 2 && live > (MT + 3) / 4) steps_of(std::integral_constant<int, (MT + 1) / 2>{});
-    else if (live > 0) steps_of(std::integral_constant<int, (MT > 2 ? (MT + 3) / 4 : (MT + 1) / 2)>{});
-    else steps_of(std::integral_constant<int, 0>{});
-    wait_copies_barrier<0>();  // LDS is free
+        if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may land after the workgroup's end
+        stored = work.store(acc, smem + S * C::STAGE + wave * C::OUT);
+    } while (more);
 }
 
 // The linear id's place when each of the 8 XCDs (dealt round by id) takes a run: a bijection of [0, total).
 __device__ __forceinline__ int xcd_run(int lin, int total) {
     const int xcd = lin & 7, rem = total & 7;
     return xcd * (total >> 3) + (xcd < rem ? xcd : rem) + (lin >> 3);
+}
+
+// The places of [0, total) that a workgroup of a grid of whole rounds of XCDs works through: each XCD takes a run, its
+// workgroups the places of it in turn.
+struct MmRuns {
+    int at, end, step;
+    __device__ __forceinline__ explicit MmRuns(int total) {
+        const int lin = (int)blockIdx.x, xcd = lin & 7, rem = total & 7, first = xcd * (total >> 3) + (xcd < rem ? xcd : rem);
+        step = (int)gridDim.x >> 3;
+        end = first + (total >> 3) + (xcd < rem ? 1 : 0);
+        at = first + (lin >> 3) - step;
+    }
+    __device__ __forceinline__ bool next() {
+        at += step;
+        return at < end;
+    }
+};
+
+// Item `at` of the (entry, row tile) pairs of a grouped product: in bands of 2 row tiles, entry by entry. Each XCD's run is
+// then a few row tiles of every expert: a matrix's rows are read by one XCD, which shares them among its entries in
+// L2, and experts with few tokens (a stream of weights) and with many (products) are spread over all XCDs alike.
+// (8192 rows of 32 uneven experts, 5760 x 2880: 386 us with runs of whole experts in bands of 8, 366 so; bands of 1 and 4
+// measure the same.)
+__device__ __forceinline__ void mm_pair(int at, int entries, int tiles, int& entry, int& tile) {
+    constexpr int BAND = 2;
+    const int band = at / (BAND * entries), in = at - band * BAND * entries, deep = tiles - BAND * band < BAND ? tiles - BAND * band : BAND;
+    entry = in / deep;
+    tile = BAND * band + in % deep;
+}
+
+// Workgroups for `tiles` tiles where `per` of them run on a CU at a time: whole rounds of XCDs.
+inline unsigned mm_grid(int64_t tiles, int per) {
+    const int64_t most = (int64_t)(num_cus() >= 8 ? num_cus() : 256) * per;
+    return (unsigned)(((tiles < most ? tiles : most) + 7) / 8 * 8);
 }
 
 }  // namespace

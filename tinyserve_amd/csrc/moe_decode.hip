@@ -228,6 +228,11 @@ int f8_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, 
 bool dense_format(const tsa_expert_layout& L);
 int dense_validate(const tsa_expert_layout& L);
 bool dense_routes(int64_t T, int64_t E, int k);
+int64_t dense_decode_ws_bytes(const tsa_expert_layout& L, int64_t T, int k);
+bool dense_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E);
+int dense_routed_batch(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const void* logits, int logits_dtype, int mode,
+                       const int32_t* expert_slot, int64_t E, int32_t* idx_out, float* w_out, int64_t T, int k, const void* x, int x_dtype,
+                       void* y, int y_dtype, uint8_t* ws, int64_t ws_bytes, hipStream_t st);
 int dense_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const int32_t* slots, const float* wts,
                  const void* logits, int logits_dtype, int mode, const int32_t* expert_slot, int64_t E, int32_t* idx_out,
                  float* w_out, int64_t T, int k, const void* x, int x_dtype, void* y, int y_dtype, uint8_t* ws,
@@ -243,7 +248,9 @@ static int64_t h_region(const tsa_expert_layout& L, int64_t T, int k) {
     return v1 > fu ? (v1 > ti ? v1 : ti) : (fu > ti ? fu : ti);
 }
 static int64_t ws_bytes(const tsa_expert_layout& L, int64_t T, int k) {
-    return MXT_SYNC_BYTES + h_region(L, T, k) + 3 * ((T * k * 4 + 255) / 256 * 256);
+    const int64_t any = MXT_SYNC_BYTES + h_region(L, T, k) + 3 * ((T * k * 4 + 255) / 256 * 256);
+    const int64_t dense = dense_format(L) ? MXT_SYNC_BYTES + dense_decode_ws_bytes(L, T, k) : 0;
+    return any > dense ? any : dense;
 }
 
 namespace {
@@ -506,6 +513,9 @@ static int decode_routed(const tsa_expert_layout* layout, const void* pool, int6
     if ((L.mx_tiled || (T <= 64 && mxt_checkpoint_ok(L, pl, x, x_dtype, k))) && E <= 256)
         return tiled_decode(L, pl, n_slots, nullptr, nullptr, logits, logits_dtype, mode, expert_slot, E, idx_out,
                             w_out, T, k, x, x_dtype, y, y_dtype, sync, ws, wsb, st);
+    if (dense_group_supported(L, T, k, E))
+        return dense_routed_batch(L, pl, n_slots, logits, logits_dtype, mode, expert_slot, E, idx_out, w_out, T, k, x, x_dtype, y, y_dtype,
+                                  ws, wsb, st);
     if (!L.mx_tiled && T * k > 65535) {  // the row-per-assignment paths: token chunks, routed one by one
         const int64_t tc = 65535 / k;
         for (int64_t t0 = 0; t0 < T; t0 += tc) {

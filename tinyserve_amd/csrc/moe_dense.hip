@@ -5,7 +5,7 @@
 // once.
 //
 // Few tokens: two launches ordered by the stream. gate_up: one workgroup per (token, expert) pair and 8 channels; down:
-// one per token and 8 outputs, over all the token's experts, so every output has one writer. Each is a stream of
+// one per token and 4 outputs, over all the token's experts, so every output has one writer. Each is a stream of
 // weights into the A operands of matrix instructions (one or two columns of B in use).
 #include "int8_common.h"
 #include "mm_epilogue.h"
@@ -18,9 +18,6 @@ namespace {
 
 template <class E>
 constexpr bool is_int8 = std::is_same<E, MmI8>::value;
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(int v) { return (float)v; }
 
 struct DenseMoe {
     tsa_expert_layout L;
@@ -44,7 +41,9 @@ struct DenseMoe {
 };
 
 constexpr int DMA_NW = 8, DMA_D = 4;  // gate_up: waves; steps of 128 bytes in flight per wave
-constexpr int DMD_NW = 8, DMD_D = 4;  // down
+constexpr int DMD_NW = 8;             // down
+template <class E>
+constexpr int dmd_d = is_int8<E> ? 2 : 3;  // (one more: spills, and down takes 2 to 3 times as long)
 
 // The slot of assignment a (token t, its jj-th), selected by every wave; the token's first workgroup writes all the
 // selections for the down launch.
@@ -88,7 +87,8 @@ __global__ void __launch_bounds__(64 * DMA_NW) dense_gate_up_kernel(DenseMoe p) 
     const int a = blockIdx.y, t = a / k, jj = a % k, n0 = (int)blockIdx.x * 8;
     constexpr int XS = is_int8<E> ? (XT == TSA_F32 ? 4 : 2) : E::ES;
     const uint8_t* xrow = static_cast<const uint8_t*>(p.x) + (int64_t)t * H * XS;
-    float xv[1][8];
+    constexpr int XR = is_int8<E> ? XT : TSA_BF16;
+    I8Raw<XR> xv[1];
     if constexpr (is_int8<E>) i8_row_load<XT, true, DMA_NW, 1>(xrow, H, tid, xv);
     const int64_t slot = dense_slot(p, a, t, jj, lane, wave);
     if (slot < 0 || slot >= p.n_slots) return;  // every wave of the workgroup: the pair's h is never read
@@ -151,16 +151,17 @@ __global__ void __launch_bounds__(64 * DMA_NW) dense_gate_up_kernel(DenseMoe p) 
 
 __device__ const uint32_t dense_zeros[4] = {0, 0, 0, 0};  // what lanes past a matrix read
 
-// One workgroup per token and 8 outputs, over all the token's experts: rows 0 .. 7 of a tile are the outputs' rows of
-// an even expert, 8 .. 15 those of the next, which meet columns 0 and 1 (their h); a unit is a step of 128 bytes of
-// such a pair, and the waves take the units in turn. int8: the experts' h are quantised in LDS.
+// One workgroup per token and 4 outputs, over all the token's experts: rows 4 e .. 4 e + 3 of a tile are the outputs' rows
+// of the e-th of four experts, which meet column e (its h); a unit is a step of 128 bytes of such four, and the waves take
+// the units in turn. (Two experts and 8 outputs, half as many workgroups: XX.) int8: the experts' h are quantised in LDS.
 template <class E>
-__global__ void __launch_bounds__(64 * DMD_NW) dense_down_kernel(DenseMoe p) {
+__global__ void __launch_bounds__(64 * DMD_NW, 4) dense_down_kernel(DenseMoe p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), q = lane >> 4, i = lane & 15;
     const tsa_expert_layout& L = p.L;
     const int H = (int)L.hidden, I = (int)L.inter, k = p.k, KB = I * E::ES, G = (KB + MMB - 1) / MMB;
-    const int t = blockIdx.y, n0 = (int)blockIdx.x * 8;
+    const int t = blockIdx.y, n0 = (int)blockIdx.x * 4;
+    constexpr int D = dmd_d<E>;
     __shared__ __align__(16) float red[DMD_NW * 16];
     __shared__ float hs[64];
     // lane j: the token's j-th slot (-1: none) and weight
@@ -171,79 +172,87 @@ __global__ void __launch_bounds__(64 * DMD_NW) dense_down_kernel(DenseMoe p) {
         my_w = p.wts[(int64_t)t * k + lane];
     }
     my_slot = my_slot < p.n_slots ? my_slot : -1;
+    my_w = my_slot >= 0 ? my_w : 0.0f;  // the weight of an expert that is not here may be anything
     const uint8_t* hrows = static_cast<const uint8_t*>(p.h) + (int64_t)t * k * I * (is_int8<E> ? 4 : 2);
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int c0 = 0; c0 < k; c0 += p.chunk) {  // workgroup-uniform
-        const int nc = k - c0 < p.chunk ? k - c0 : p.chunk, units = (nc + 1) / 2 * G;
-        u32x4 A[DMD_D][2], Bv[DMD_D][2];
-        v4f sc[DMD_D];
+        const int nc = k - c0 < p.chunk ? k - c0 : p.chunk, units = (nc + 3) / 4 * G;
+        u32x4 A[D][2], Bv[D][2];
+        v4f ws[D];
+        float sc[D];
         auto load = [&](int u0) {
 #pragma unroll
-            for (int d = 0; d < DMD_D; ++d) {
-                const int u = u0 + DMD_NW * d, pair = u / G, b = u % G;
+            for (int d = 0; d < D; ++d) {
+                const int u = u0 + DMD_NW * d, four = u / G, b = u - four * G;
                 if (u >= units) break;
-                const int ja = 2 * pair + (i >> 3), js = 2 * pair + (q >> 1), jb = 2 * pair + (i & 1);
+                const int ja = 4 * four + (i >> 2), js = 4 * four + q, jb = 4 * four + (i & 3);  // of the lane's row of A, its sums, its column
                 // every lane takes part in the shuffles: one that is off has 0 (a slot) read from it
                 const int la = __shfl(my_slot, (c0 + ja) & 63, 64), ls = __shfl(my_slot, (c0 + js) & 63, 64);
-                const int lb = __shfl(my_slot, (c0 + jb) & 63, 64);
                 const float w = __shfl(my_w, (c0 + js) & 63, 64);
-                const int sa = ja < nc ? la : -1, ss = js < nc ? ls : -1, sb = i < 2 && jb < nc ? lb : -1;
+                const int sa = ja < nc ? la : -1, ss = js < nc ? ls : -1;
                 const int o = MMB * b + 16 * q;
                 const void* z = dense_zeros;
+                sc[d] = js < nc ? w : 0.0f;
                 if constexpr (!is_int8<E>) {
-                    const uint8_t* hr = hrows + (int64_t)(c0 + jb) * KB + o;  // a dead expert's was never written
-                    Bv[d][0] = *static_cast<const u32x4*>(sb >= 0 && o < KB ? hr : z);
-                    Bv[d][1] = *static_cast<const u32x4*>(sb >= 0 && o + 64 < KB ? hr + 64 : z);
-                    const float ws = ss >= 0 ? w : 0.0f;  // a dead expert's weight may be anything
-                    sc[d] = v4f{ws, ws, ws, ws};
+                    const int lb = __shfl(my_slot, (c0 + jb) & 63, 64);
+                    const bool live = i < 4 && jb < nc && lb >= 0;  // the h of an expert that is not here was never written
+                    const uint8_t* hr = hrows + (int64_t)(c0 + jb) * KB + o;
+                    Bv[d][0] = *static_cast<const u32x4*>(live && o < KB ? hr : z);
+                    Bv[d][1] = *static_cast<const u32x4*>(live && o + 64 < KB ? hr + 64 : z);
                 } else {
-                    const uint8_t* sp = p.pool + (int64_t)ss * L.slot_bytes + L.down_scales_off + 4 * (n0 + 4 * (q & 1));
-                    const v4f ws = *static_cast<const v4f*>(ss >= 0 ? static_cast<const void*>(sp) : z);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[d][e] = ss >= 0 ? w * ws[e] : 0.0f;
+                    const uint8_t* sp = p.pool + (int64_t)ss * L.slot_bytes + L.down_scales_off + 4 * n0;
+                    ws[d] = *static_cast<const v4f*>(ss >= 0 ? static_cast<const void*>(sp) : z);
                 }
-                const uint8_t* at = p.pool + (int64_t)sa * L.slot_bytes + L.down_off + (int64_t)(n0 + (i & 7)) * KB + o;
+                const uint8_t* at = p.pool + (int64_t)sa * L.slot_bytes + L.down_off + (int64_t)(n0 + (i & 3)) * KB + o;
                 A[d][0] = *static_cast<const u32x4*>(sa >= 0 && o < KB ? at : z);
                 A[d][1] = *static_cast<const u32x4*>(sa >= 0 && o + 64 < KB ? at + 64 : z);
             }
         };
-        load(wave);
         if constexpr (is_int8<E>) {
+            // a wave an expert: the first one's values are loaded ahead of the weights. (Codes of an expert that is not
+            // here meet weights of zero.)
+            constexpr int HELD = 2;
+            auto live = [&](int j) { return j < nc && __builtin_amdgcn_readlane(my_slot, (c0 + j) & 63) >= 0; };
+            const int mine = __shfl(my_slot, (c0 + lane) & 63, 64);  // lane j's: the chunk's j-th
+            const uint8_t* hr = hrows + (int64_t)(c0 + wave) * I * 4;
+            const bool first = live(wave);
+            I8Raw<TSA_F32> v[HELD];
+            i8_row_load<TSA_F32, true, 1, HELD>(hr, first ? I : 0, lane, v);
+            load(wave);
             if (c0) __syncthreads();  // the chunk before is used up
-            for (int j = wave; j < nc; j += DMD_NW) {  // a wave an expert
-                const int slot = __builtin_amdgcn_readlane(my_slot, c0 + j);
-                uint8_t* codes = smem + j * G * MMB;
-                if (slot < 0) {  // what is there is multiplied by weights of zero
-                    for (int c = lane; c < G * MMB / 16; c += 64) *reinterpret_cast<u32x4*>(codes + 16 * c) = u32x4{0, 0, 0, 0};
-                    if (lane == 0) hs[j] = 0.0f;
-                    continue;
-                }
-                constexpr int D = 6;
-                const uint8_t* hr = hrows + (int64_t)(c0 + j) * I * 4;
-                float v[D][8];
-                i8_row_load<TSA_F32, true, 1, D>(hr, I, lane, v);
-                const float s = i8_row_codes<TSA_F32, true, 1, D>(hr, I, lane, v, codes, nullptr);
+            if (first) {
+                const float s = i8_row_codes<TSA_F32, true, 1, HELD>(hr, I, lane, v, smem + wave * G * MMB, nullptr);
+                if (lane == 0) hs[wave] = s;
+            }
+            for (int j = wave + DMD_NW; j < nc; j += DMD_NW) {
+                if (!live(j)) continue;
+                const uint8_t* row = hrows + (int64_t)(c0 + j) * I * 4;
+                i8_row_load<TSA_F32, true, 1, HELD>(row, I, lane, v);
+                const float s = i8_row_codes<TSA_F32, true, 1, HELD>(row, I, lane, v, smem + j * G * MMB, nullptr);
                 if (lane == 0) hs[j] = s;
             }
+            if (wave == 0 && lane < nc && mine < 0) hs[lane] = 0.0f;
             __syncthreads();
+        } else {
+            load(wave);
         }
-        for (int u0 = wave; u0 < units; u0 += DMD_NW * DMD_D) {
+        for (int u0 = wave; u0 < units; u0 += DMD_NW * D) {
             if (u0 != wave) load(u0);
 #pragma unroll
-            for (int d = 0; d < DMD_D; ++d) {
+            for (int d = 0; d < D; ++d) {
                 const int u = u0 + DMD_NW * d;
                 if (u >= units) break;
-                v4f s = sc[d];
+                v4f s = {sc[d], sc[d], sc[d], sc[d]};
                 if constexpr (is_int8<E>) {
-                    const int pair = u / G, b = u % G, j = 2 * pair + i, js = 2 * pair + (q >> 1);
+                    const int four = u / G, b = u - four * G, j = 4 * four + i, js = 4 * four + q;
                     Bv[d][0] = Bv[d][1] = u32x4{0, 0, 0, 0};
-                    if (i < 2 && j < nc) {
+                    if (i < 4 && j < nc) {
                         Bv[d][0] = *reinterpret_cast<const u32x4*>(smem + MMB * (j * G + b) + 16 * q);
                         Bv[d][1] = *reinterpret_cast<const u32x4*>(smem + MMB * (j * G + b) + 64 + 16 * q);
                     }
-                    const float f = js < nc ? hs[js] : 0.0f;
+                    const float f = js < nc ? sc[d] * hs[js] : 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[e] = sc[d][e] * f;
+                    for (int e = 0; e < 4; ++e) s[e] = f * ws[d][e];
                 }
                 typename E::acc part = {0, 0, 0, 0};
                 part = E::mfma(A[d][0], Bv[d][0], part);
@@ -253,12 +262,12 @@ __global__ void __launch_bounds__(64 * DMD_NW) dense_down_kernel(DenseMoe p) {
             }
         }
     }
-    if (i == (q >> 1)) *reinterpret_cast<v4f*>(red + wave * 16 + 4 * q) = acc;  // an expert's rows in its own column
+    if (i == q) *reinterpret_cast<v4f*>(red + wave * 16 + 4 * q) = acc;  // an expert's rows in its own column
     __syncthreads();
-    if (tid < 8) {
+    if (tid < 4) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < DMD_NW; ++w) v += red[16 * w + tid] + red[16 * w + 8 + tid];
+        for (int w = 0; w < DMD_NW * 4; ++w) v += red[4 * w + tid];
         store_out(p.y, p.y_dtype, (int64_t)t * H + n0 + tid, v);
     }
 }
@@ -303,99 +312,130 @@ __global__ void __launch_bounds__(GROUP_THREADS) dense_prepare_kernel(DenseGroup
         if (t >= p.T) return;
         constexpr int ES = XT == TSA_F32 ? 4 : 2, D = 6;
         const uint8_t* row = static_cast<const uint8_t*>(p.x) + (int64_t)t * H * ES;
-        float v[D][8];
+        I8Raw<XT> v[D];
         i8_row_load<XT, true, 1, D>(row, H, lane, v);
         const float s = i8_row_codes<XT, true, 1, D>(row, H, lane, v, const_cast<uint8_t*>(p.xq) + (int64_t)t * H, nullptr);
         if (lane == 0) p.xs[t] = s;
     }
 }
 
+// A workgroup's tiles (mm_pair's order) of the table's entries.
+template <class C>
+struct DenseWork {
+    const DenseGroup& p;
+    const int entries, tiles;  // row tiles of an entry
+    MmRuns runs;
+    int slot, row0, tn, tile, next_slot, next_row0, next_tn, next_tile;
+    __device__ __forceinline__ DenseWork(const DenseGroup& p, int tiles) : p(p), entries(uniform(*p.n_entries)), tiles(tiles), runs(entries * tiles) {}
+    __device__ __forceinline__ bool next() {
+        if (!runs.next()) return false;
+        int entry;
+        mm_pair(runs.at, entries, tiles, entry, next_tile);
+        const int4 e = p.table[entry];
+        next_slot = uniform(e.x), next_row0 = uniform(e.y), next_tn = uniform(e.z);
+        return true;
+    }
+    __device__ __forceinline__ void take() { slot = next_slot, row0 = next_row0, tn = next_tn, tile = next_tile; }
+};
+
+template <class C, class E>
+struct DenseUp : DenseWork<C> {
+    using B = DenseWork<C>;
+    static constexpr int CH = C::RN / 2, MP = C::MR / 2, MT = C::MT;  // channels of a tile
+    __device__ __forceinline__ explicit DenseUp(const DenseGroup& p) : B(p, ((int)p.L.inter + CH - 1) / CH) {}
+    __device__ __forceinline__ int picked(int row) const { return B::p.perm[row] / B::p.k; }
+    __device__ __forceinline__ int token(int r) const { return picked(B::next_row0 + r); }
+    __device__ __forceinline__ MmOperands<2> operands() const {
+        const tsa_expert_layout& L = B::p.L;
+        const int KB = (int)L.hidden * E::ES, c0 = B::next_tile * CH;
+        const uint8_t* base = B::p.pool + (int64_t)B::next_slot * L.slot_bytes;
+        return MmOperands<2>{{base + L.gate_off + (int64_t)c0 * KB, base + L.up_off + (int64_t)c0 * KB}, (int)L.inter - c0, B::p.xq,
+                             (uint32_t)B::p.T * (uint32_t)KB, B::next_tn};
+    }
+    __device__ __forceinline__ bool store(const typename E::acc (&acc)[C::MR][MT], uint8_t* out) const {
+        const DenseGroup& p = B::p;
+        const tsa_expert_layout& L = p.L;
+        const int I = (int)L.inter, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
+        const int t0 = wave / C::WR * MT * 16, cw = B::tile * CH + wave % C::WR * MP * 16;
+        v4f sg[MP], su[MP];
+        float sx[MT];
+        if constexpr (is_int8<E>) {
+            const float* s = reinterpret_cast<const float*>(p.pool + (int64_t)B::slot * L.slot_bytes + L.gate_scales_off);
+#pragma unroll
+            for (int m = 0; m < MP; ++m) {  // I % 32 == 0: all four or none
+                const int c = cw + 16 * m + 4 * q;
+                sg[m] = *reinterpret_cast<const v4f*>(s + (c < I ? c : 0));
+                su[m] = *reinterpret_cast<const v4f*>(s + I + (c < I ? c : 0));
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) sx[t] = t0 + 16 * t + i < B::tn ? p.xs[picked(B::row0 + t0 + 16 * t + i)] : 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            if (t0 + 16 * t >= B::tn) continue;  // uniform
+            v4f h[MP];
+#pragma unroll
+            for (int m = 0; m < MP; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float g = to_f32(acc[m][t][r]), u = to_f32(acc[MP + m][t][r]);
+                    h[m][r] = is_int8<E> ? moe_act(L, g * (sx[t] * sg[m][r]), u * (sx[t] * su[m][r])) : moe_act(L, g, u);
+                }
+            if constexpr (is_int8<E>) {
+                const int tk = t0 + 16 * t + i;
+                float* dst = static_cast<float*>(p.h) + (int64_t)(B::row0 + tk) * I;
+#pragma unroll
+                for (int m = 0; m < MP; ++m) {
+                    const int c = cw + 16 * m + 4 * q;
+                    if (tk < B::tn && c < I) *reinterpret_cast<v4f*>(dst + c) = h[m];
+                }
+            } else {
+                uint2 v[MP];
+#pragma unroll
+                for (int m = 0; m < MP; ++m) v[m] = mm_pack4<std::is_same<E, MmBf16>::value ? TSA_BF16 : TSA_F16>(h[m]);
+                mm_rows16<MP, false>(v, out, [&](int r, int c) -> void* {
+                    const int tk = t0 + 16 * t + r, n = cw + 8 * c;
+                    return tk < B::tn && n < I ? static_cast<uint16_t*>(p.h) + (int64_t)(B::row0 + tk) * I + n : nullptr;
+                });
+            }
+        }
+        return false;
+    }
+};
+
+template <class C, class E>
+struct DenseDown : DenseWork<C> {
+    using B = DenseWork<C>;
+    __device__ __forceinline__ explicit DenseDown(const DenseGroup& p) : B(p, ((int)p.L.hidden + C::RN - 1) / C::RN) {}
+    __device__ __forceinline__ int token(int r) const { return r; }
+    __device__ __forceinline__ MmOperands<1> operands() const {
+        const tsa_expert_layout& L = B::p.L;
+        const int KB = (int)L.inter * E::ES, n0 = B::next_tile * C::RN;
+        return MmOperands<1>{{B::p.pool + (int64_t)B::next_slot * L.slot_bytes + L.down_off + (int64_t)n0 * KB}, (int)L.hidden - n0,
+                             B::p.hq + (int64_t)B::next_row0 * KB, (uint32_t)B::next_tn * (uint32_t)KB, B::next_tn};
+    }
+    __device__ __forceinline__ bool store(const typename E::acc (&acc)[C::MR][C::MT], uint8_t* out) const {
+        const DenseGroup& p = B::p;
+        const int H = (int)p.L.hidden;
+        const MmOut o = MmOut{p.yk, TSA_F32, H, nullptr, 0, 1};  // H % 32 == 0: rows of whole 16-byte pieces
+        return mm_store<C>(acc, o, out, B::tile * C::RN, H, B::tn, [&](int r) { return (int64_t)p.perm[B::row0 + r]; },
+                           [&](int r) { return p.hs[B::row0 + r]; },
+                           reinterpret_cast<const float*>(p.pool + (int64_t)B::slot * p.L.slot_bytes + p.L.down_scales_off));
+    }
+};
+
 template <class C, class E>
 __global__ void __launch_bounds__(C::THREADS) dense_group_gate_up_kernel(DenseGroup p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    const tsa_expert_layout& L = p.L;
-    const int H = (int)L.hidden, I = (int)L.inter, KB = H * E::ES;
-    constexpr int CH = C::RN / 2, MP = C::MR / 2;  // channels of a workgroup
-    int entry, tile;
-    if (!grouped_work(p.n_entries, (I + CH - 1) / CH, entry, tile)) return;
-    const int4 e = p.table[entry];
-    const int slot = uniform(e.x), row0 = uniform(e.y), tn = uniform(e.z), c0 = tile * CH;
-    const uint8_t* base = p.pool + (int64_t)slot * L.slot_bytes;
-    MmOperands<2> o;
-    o.w[0] = base + L.gate_off + (int64_t)c0 * KB;
-    o.w[1] = base + L.up_off + (int64_t)c0 * KB;
-    o.w_rows = I - c0;
-    o.x = p.xq;
-    o.x_records = (uint32_t)p.T * (uint32_t)KB;
-    o.KB = (uint32_t)KB;
-    typename E::acc acc[C::MR][C::MT];
-    auto token = [&](int r) { return p.perm[row0 + r] / p.k; };
-    mm_tile<C, E, 2>(o, smem, tn, token, acc);
-
-    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
-    const int wr = wave % C::WR, wt = wave / C::WR;
-    v4f sg[MP], su[MP];
-    if constexpr (is_int8<E>) {
-        const float* s = reinterpret_cast<const float*>(base + L.gate_scales_off);
-#pragma unroll
-        for (int m = 0; m < MP; ++m) {
-            const int c = c0 + (wr * MP + m) * 16 + 4 * q;
-            sg[m] = *reinterpret_cast<const v4f*>(s + (c < I ? c : 0));
-            su[m] = *reinterpret_cast<const v4f*>(s + I + (c < I ? c : 0));
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < C::MT; ++t) {
-        const int tk = 16 * (C::MT * wt + t) + i;
-        if (tk >= tn) continue;
-        float sx = 1.0f;
-        if constexpr (is_int8<E>) sx = p.xs[token(tk)];
-#pragma unroll
-        for (int m = 0; m < MP; ++m) {
-            const int c = c0 + (wr * MP + m) * 16 + 4 * q;  // I % 32 == 0: all four or none
-            if (c >= I) continue;
-            v4f h;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float g = to_f32(acc[m][t][r]), u = to_f32(acc[MP + m][t][r]);
-                h[r] = is_int8<E> ? moe_act(L, g * (sx * sg[m][r]), u * (sx * su[m][r])) : moe_act(L, g, u);
-            }
-            const int64_t at = (int64_t)(row0 + tk) * I + c;
-            if constexpr (is_int8<E>) {
-                *reinterpret_cast<v4f*>(static_cast<float*>(p.h) + at) = h;
-            } else {
-                uint16_t* dst = static_cast<uint16_t*>(p.h) + at;
-                if constexpr (std::is_same<E, MmBf16>::value)
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3]));
-                else
-                    *reinterpret_cast<uint2*>(dst) = make_uint2((uint32_t)f32_to_f16_bits(h[0]) | (uint32_t)f32_to_f16_bits(h[1]) << 16,
-                                                                (uint32_t)f32_to_f16_bits(h[2]) | (uint32_t)f32_to_f16_bits(h[3]) << 16);
-            }
-        }
-    }
+    DenseUp<C, E> work(p);
+    mm_run<C, E, 2, true>(work, (uint32_t)p.L.hidden * E::ES, smem);
 }
 
 template <class C, class E>
 __global__ void __launch_bounds__(C::THREADS) dense_group_down_kernel(DenseGroup p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    const tsa_expert_layout& L = p.L;
-    const int H = (int)L.hidden, KB = (int)L.inter * E::ES;
-    int entry, tile;
-    if (!grouped_work(p.n_entries, (H + C::RN - 1) / C::RN, entry, tile)) return;
-    const int4 e = p.table[entry];
-    const int slot = uniform(e.x), row0 = uniform(e.y), tn = uniform(e.z), n0 = tile * C::RN;
-    const uint8_t* base = p.pool + (int64_t)slot * L.slot_bytes;
-    MmOperands<1> o;
-    o.w[0] = base + L.down_off + (int64_t)n0 * KB;
-    o.w_rows = H - n0;
-    o.x = p.hq + (int64_t)row0 * KB;
-    o.x_records = (uint32_t)tn * (uint32_t)KB;
-    o.KB = (uint32_t)KB;
-    typename E::acc acc[C::MR][C::MT];
-    mm_tile<C, E, 1>(o, smem, tn, [](int r) { return r; }, acc);
-    const MmOut out = MmOut{p.yk, TSA_F32, H, nullptr, 0, 1};  // H % 32 == 0: rows of whole 16-byte pieces
-    mm_store<C>(acc, out, n0, H, tn, [&](int r) { return (int64_t)p.perm[row0 + r]; }, [&](int r) { return p.hs[row0 + r]; },
-                reinterpret_cast<const float*>(base + L.down_scales_off));
+    DenseDown<C, E> work(p);
+    mm_run<C, E, 1, false>(work, (uint32_t)p.L.inter * E::ES, smem);
 }
 
 struct DensePlaces {
@@ -416,7 +456,7 @@ DensePlaces dense_places(const tsa_expert_layout& L, int64_t T, int k, int64_t E
     w.offsets = take((E + 1) * 4);
     w.perm = take(n * 4);
     w.n_entries = take(4);
-    w.table = take((n / 16 + E) * 16);
+    w.table = take((n / 64 + E) * 16);
     w.xq = take(i8 ? T * H : 0);
     w.xs = take(i8 ? T * 4 : 0);
     w.h = take(n * I * (i8 ? 4 : 2));
@@ -434,7 +474,7 @@ int64_t dense_tokens(const tsa_expert_layout& L, int64_t T, int k) {
 }
 
 template <class E, class GU, class DN>
-int dense_gemms(const DenseGroup& p, int64_t entries, hipStream_t st) {
+int dense_gemms(const DenseGroup& p, int64_t entries, int per, hipStream_t st) {
     DenseGroup q = p;
     void* args[] = {&q};
     const void* fg = reinterpret_cast<const void*>(&dense_group_gate_up_kernel<GU, E>);
@@ -443,40 +483,36 @@ int dense_gemms(const DenseGroup& p, int64_t entries, hipStream_t st) {
     TSA_HIP_CHECK(ensure_dynamic_lds(fd, DN::LDS));
     static_assert(GU::TM == DN::TM, "one table of token tiles");
     const int64_t tg = (p.L.inter + GU::RN / 2 - 1) / (GU::RN / 2), td = (p.L.hidden + DN::RN - 1) / DN::RN;
-    auto grid = [](int64_t n) { return dim3((unsigned)((n + 7) / 8 * 8)); };  // whole rounds of XCDs
-    TSA_HIP_CHECK(hipLaunchKernel(fg, grid(entries * tg), dim3(GU::THREADS), args, GU::LDS, st));
+    TSA_HIP_CHECK(hipLaunchKernel(fg, dim3(mm_grid(entries * tg, per)), dim3(GU::THREADS), args, GU::LDS, st));
     if (is_int8<E>) {  // every sorted row, also those of experts that are not here (never read)
         const int rc = i8_quantize(p.h, TSA_F32, (int64_t)p.T * p.k, p.L.inter, const_cast<uint8_t*>(p.hq), const_cast<float*>(p.hs), st);
         if (rc) return rc;
     }
-    TSA_HIP_CHECK(hipLaunchKernel(fd, grid(entries * td), dim3(DN::THREADS), args, DN::LDS, st));
+    TSA_HIP_CHECK(hipLaunchKernel(fd, dim3(mm_grid(entries * td, per)), dim3(DN::THREADS), args, DN::LDS, st));
     return TSA_OK;
 }
 
 using Up128 = MmTile<4, 2, 4, 4, 3>;   // 128 channels x 128 tokens, 8 waves
 using Up64 = MmTile<4, 1, 2, 4, 3>;    // 64 x 64
-using Up16 = MmTile<4, 1, 2, 1, 3>;    // 64 x 16
 using Down128 = MmTile<4, 2, 4, 4, 3>; // 256 rows x 128 tokens
 using Down64 = MmTile<4, 1, 2, 4, 3>;  // 128 x 64
-using Down16 = MmTile<4, 1, 2, 1, 3>;  // 128 x 16
 
 template <class E>
 int dense_gemms(const DenseGroup& p, hipStream_t st) {
     const int64_t n = (int64_t)p.T * p.k, entries = n / p.tile_rows + (p.E < n ? p.E : n);
-    switch (p.tile_rows) {
-        case 16: return dense_gemms<E, Up16, Down16>(p, entries, st);
-        case 64: return dense_gemms<E, Up64, Down64>(p, entries, st);
-        default: return dense_gemms<E, Up128, Down128>(p, entries, st);
-    }
+    return p.tile_rows == 64 ? dense_gemms<E, Up64, Down64>(p, entries, 2, st) : dense_gemms<E, Up128, Down128>(p, entries, 1, st);
 }
 
 }  // namespace
 
 bool dense_format(const tsa_expert_layout& L) { return L.format == TSA_EXPERT_DENSE || L.format == TSA_EXPERT_INT8; }
 
-// h [T k, I] fp32, then the routed selection.
+// Pairs: h [T k, I] fp32, then the routed selection. Routed calls of more tokens: the selection, then what the grouped
+// kernels need (for any number of experts).
 int64_t dense_decode_ws_bytes(const tsa_expert_layout& L, int64_t T, int k) {
-    return align256(T * k * L.inter * 4) + 2 * align256(T * k * 4);
+    const int64_t pairs = align256(T * k * L.inter * 4), table = 2 * align256(T * k * 4);
+    const int64_t grouped = T > DENSE_PAIR_TOKENS ? dense_places(L, dense_tokens(L, T, k), k, MAX_GROUP_E).bytes : 0;
+    return table + (pairs > grouped ? pairs : grouped);
 }
 
 // Calls whose routing runs inside the gate_up kernel.
@@ -523,7 +559,7 @@ int dense_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slot
     p.y_dtype = y_dtype;
     const int GH = (int)((L.hidden + MMB - 1) / MMB), GI = (int)((L.inter + MMB - 1) / MMB), row = GI * MMB;
     p.chunk = !i8 || k * row <= 60 * 1024 ? k : 60 * 1024 / row;  // at least 3 rows of 16384
-    p.chunk = p.chunk < k ? p.chunk / 2 * 2 : p.chunk;            // whole pairs
+    p.chunk = p.chunk < k && p.chunk >= 4 ? p.chunk / 4 * 4 : p.chunk;  // whole fours
     const int lds_a = i8 ? GH * MMB : 0, lds_b = i8 ? p.chunk * row : 0;
     const void* fa = !i8 ? (L.gate_type == TSA_BF16 ? reinterpret_cast<const void*>(&dense_gate_up_kernel<MmBf16, TSA_BF16>)
                                                     : reinterpret_cast<const void*>(&dense_gate_up_kernel<MmF16, TSA_F16>))
@@ -541,11 +577,13 @@ int dense_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slot
     const void* fb = i8 ? reinterpret_cast<const void*>(&dense_down_kernel<MmI8>)
                      : L.gate_type == TSA_BF16 ? reinterpret_cast<const void*>(&dense_down_kernel<MmBf16>)
                                                : reinterpret_cast<const void*>(&dense_down_kernel<MmF16>);
-    TSA_HIP_CHECK(hipLaunchKernel(fb, dim3((unsigned)(L.hidden / 8), (unsigned)T), dim3(64 * DMD_NW), args_b, lds_b, st));
+    TSA_HIP_CHECK(hipLaunchKernel(fb, dim3((unsigned)(L.hidden / 4), (unsigned)T), dim3(64 * DMD_NW), args_b, lds_b, st));
     return TSA_OK;
 }
 
-// Calls that the grouped kernels take.
+// Calls that the grouped kernels take (us of a layer grouped / as pairs, without the routing: hidden 2048, 128 experts top-8,
+// 2 / 3 / 4 / 8 tokens, bf16 39 / 43 / 47 / 56 and 34 / 46 / 58 / 105, int8 33 / 35 / 38 / 44 and 24 / 32 / 40 / 72; hidden 2880,
+// 32 experts top-4, 2 / 3 / 4 tokens, bf16 82 / 87 / 91 and 74 / 102 / 130, int8 62 / 62 / 65 and 57 / 76 / 96).
 bool dense_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
     return dense_format(L) && T > DENSE_PAIR_TOKENS && E <= MAX_GROUP_E && k <= 64;
 }
@@ -591,7 +629,12 @@ int dense_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t
         p.hs = reinterpret_cast<float*>(ws + w.hs);
         p.yk = reinterpret_cast<float*>(ws + w.yk);
         const int64_t n = (int64_t)p.T * k;
-        p.tile_rows = n <= 12 * E ? 16 : n <= 48 * E ? 64 : 128;
+        // us of a layer in tiles of 64 / 128 tokens, hidden 2048, 128 experts top-8, 24 / 200 / 700 / 1024 / 2048 tokens:
+        // bf16 82 / 151 / 238 / 286 / 426 and 88 / 158 / 239 / 273 / 376, int8 56 / 97 / 158 / 190 / 288 and 61 / 103 / 159 /
+        // 188 / 265; hidden 2880, 32 experts top-4, 100 / 200 / 400 / 2048 tokens: bf16 270 / 311 / 355 / 760 and 291 / 322 /
+        // 342 / 600, int8 170 / 207 / 244 / 541 and 188 / 216 / 237 / 435. (Tiles of 16: bf16 2 to 5% faster for 24 and 48
+        // tokens over 128 experts, else slower.)
+        p.tile_rows = n <= 48 * E ? 64 : 128;
         void* args[] = {&p};
         const unsigned wgs = i8 ? (unsigned)(1 + (p.T + GROUP_WAVES - 1) / GROUP_WAVES) : 1u;
         TSA_HIP_CHECK(hipLaunchKernel(fp, dim3(wgs), dim3(GROUP_THREADS), args, lds, st));
@@ -602,6 +645,20 @@ int dense_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t
         if (rc) return rc;
     }
     return TSA_OK;
+}
+
+// Routed calls of more tokens than the pairs take: top-k, then as a prompt.
+int dense_routed_batch(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const void* logits, int logits_dtype, int mode,
+                       const int32_t* expert_slot, int64_t E, int32_t* idx_out, float* w_out, int64_t T, int k, const void* x, int x_dtype,
+                       void* y, int y_dtype, uint8_t* ws, int64_t ws_bytes, hipStream_t st) {
+    TSA_REQUIRE(ws_bytes >= dense_decode_ws_bytes(L, T, k), TSA_ERR_WORKSPACE, "workspace too small for the decode");
+    int rc = check_dense(L, pool, x, x_dtype, ws);
+    if (rc) return rc;
+    int32_t* idx = idx_out ? idx_out : reinterpret_cast<int32_t*>(ws);
+    float* w = w_out ? w_out : reinterpret_cast<float*>(ws + align256(T * k * 4));
+    rc = tsa_route_topk(logits, logits_dtype, T, E, k, mode, idx, w, st);
+    if (rc) return rc;
+    return dense_group_prefill(L, pool, n_slots, expert_slot, E, idx, w, T, k, x, x_dtype, y, y_dtype, ws + 2 * align256(T * k * 4), st);
 }
 
 // Requirements beyond the common ones of validate_layout, with the status they fail with.
