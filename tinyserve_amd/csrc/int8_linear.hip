@@ -270,28 +270,41 @@ using TileA = MmTile<4, 2, 4, 8, 2>;  // 256 rows x 256 tokens
 using TileB = MmTile<4, 2, 4, 4, 3>;  // 256 x 128
 using TileC = MmTile<2, 2, 4, 4, 2>;  // 128 x 128
 using TileD = MmTile<4, 1, 2, 4, 3>;  // 128 x 64
-using TileE = MmTile<4, 1, 1, 2, 4>;  // 64 x 32
 
-// The tile (A .. E as 0 .. 4) with the least rounds x round time, a round being `per` workgroups on every CU; -1 if
-// every tile gives 2^30 of them or more.
-struct GemmTile { int rows, tok, per, cost; };
-constexpr GemmTile gemm_tiles[5] = {{TileA::RN, TileA::TM, 1, 45},
-                                    {TileB::RN, TileB::TM, 1, 26},
-                                    {TileC::RN, TileC::TM, 2, 32},
-                                    {TileD::RN, TileD::TM, 2, 20},
-                                    {TileE::RN, TileE::TM, 3, 13}};
-int gemm_tile(int64_t T, int64_t N) {
+// The tile (A .. D as 0 .. 3) with the least time, where a CU that works on 1 .. `per` tiles at once takes cost[0 .. per - 1]
+// for them, and on more in rounds; -1 if every tile gives 2^30 of them or more. (us of a product of K 2880 to 4096. Over the shapes of N 512
+// to 8192 and 33 to 8192 tokens that were measured: within 6% of the best tile but for a few of fewer than 100 tokens.)
+struct GemmTile { int rows, tok, per, cost[2]; };
+constexpr GemmTile gemm_tiles[4] = {{TileA::RN, TileA::TM, 1, {43}},
+                                    {TileB::RN, TileB::TM, 1, {25}},
+                                    {TileC::RN, TileC::TM, 2, {21, 28}},
+                                    {TileD::RN, TileD::TM, 2, {14, 20}}};
+
+// The tile, and its time.
+int gemm_tile(int64_t T, int64_t N, int64_t* time = nullptr) {
     const int64_t cus = num_cus() > 0 ? num_cus() : 256;
     int best = -1;
     int64_t least = INT64_MAX;
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const GemmTile& t = gemm_tiles[i];
-        const int64_t tiles = (N + t.rows - 1) / t.rows * ((T + t.tok - 1) / t.tok);
+        const int64_t tiles = (N + t.rows - 1) / t.rows * ((T + t.tok - 1) / t.tok), on = (tiles + cus - 1) / cus;
         if (tiles >= (int64_t)1 << 30) continue;
-        const int64_t cost = (tiles + cus * t.per - 1) / (cus * t.per) * t.cost;
+        const int64_t cost = on / t.per * t.cost[t.per - 1] + (on % t.per ? t.cost[on % t.per - 1] : 0);
         if (cost < least) least = cost, best = i;
     }
+    if (time) *time = least;
     return best;
+}
+
+// Whether the row kernel takes a product: up to 32 tokens, and more while its rounds of 16 rows x 32 tokens on every CU take
+// less than the tiles. us of the row kernel / the tiles, weights from memory: 2880 x 2880, 64 / 128 / 192 tokens 8.3 / 16.8, 10.9 /
+// 17.0 and 15.4 / 15.4; 2048 x 4096, 128 / 192 / 256 14.1 / 21.8, 19.3 / 21.8 and 24.4 / 21.9; 5760 x 2880, 64 / 96 / 128 10.9 / 17.0,
+// 15.5 / 15.6 and 17.8 / 15.5; 512 x 2048, 512 tokens 8.3 / 12.9.
+bool rows_kernel(int64_t T, int64_t N) {
+    if (T <= 32) return true;
+    const int64_t cus = num_cus() > 0 ? num_cus() : 256, on = ((N + 15) / 16 * ((T + 31) / 32) + cus - 1) / cus;
+    int64_t time;
+    return gemm_tile(T, N, &time) >= 0 && 3 + 3 * on <= time;
 }
 
 hipError_t pick_gemm(const I8Gemm& p, hipStream_t st) {
@@ -300,8 +313,7 @@ hipError_t pick_gemm(const I8Gemm& p, hipStream_t st) {
         case 0: return launch_gemm<TileA>(p, per, st);
         case 1: return launch_gemm<TileB>(p, per, st);
         case 2: return launch_gemm<TileC>(p, per, st);
-        case 3: return launch_gemm<TileD>(p, per, st);
-        default: return launch_gemm<TileE>(p, per, st);
+        default: return launch_gemm<TileD>(p, per, st);
     }
 }
 
@@ -370,7 +382,7 @@ extern "C" int tsa_int8_matmul(const void* codes, const float* scales, int64_t T
     TSA_REQUIRE(codes && scales && w && w_scales && y, TSA_ERR_INVALID_ARG, "null pointer");
     TSA_REQUIRE(aligned16(codes) && aligned16(w), TSA_ERR_INVALID_ARG, "the codes must be 16-byte aligned");
     const MmOut out = mm_out(y, y_dtype, N, bias, bias_dtype);
-    if (T > 32) {
+    if (!rows_kernel(T, N)) {
         I8Gemm p{};
         p.w = static_cast<const uint8_t*>(w);
         p.ws = w_scales;
