@@ -507,11 +507,23 @@ int dense_gemms(const DenseGroup& p, hipStream_t st) {
 
 bool dense_format(const tsa_expert_layout& L) { return L.format == TSA_EXPERT_DENSE || L.format == TSA_EXPERT_INT8; }
 
+// Tokens up to which a call runs as pairs: two, and more while they are few and their experts' weights, read once for each
+// pair, few bytes; the grouped kernels read each expert once, in five or six launches. us of a layer grouped / as pairs, without the
+// routing: hidden 2048, 128 experts top-8, 2 / 3 / 4 / 8 tokens, bf16 (9.4 MB an expert) 39 / 43 / 47 / 56 and 34 / 46 / 58 / 105, int8 33 /
+// 35 / 38 / 44 and 24 / 32 / 40 / 72; hidden 2880, 32 experts top-4, 2 / 3 / 4 tokens, bf16 (50 MB) 82 / 87 / 91 and 74 / 102 / 130, int8 62 /
+// 62 / 65 and 57 / 76 / 96; hidden 1440, 20 experts top-3, int8 (3.2 MB), 6 / 8 tokens 28 / 28 and 27 / 33; hidden 1024, 16 experts top-2, bf16
+// (3.1 MB), 12 / 16 tokens 26 / 26 and 27 / 34; hidden 256, 64 experts top-4 (0.25 MB), 16 / 24 tokens 18 / 18 and 12 / 15.
+int64_t dense_pair_tokens(const tsa_expert_layout& L, int k) {
+    const int64_t expert = 3 * L.hidden * L.inter * (L.format == TSA_EXPERT_INT8 ? 1 : 2), bytes = ((int64_t)72 << 20) / (k * expert), few = 64 / k;
+    const int64_t most = bytes < few ? bytes : few;
+    return most > 2 ? most : 2;
+}
+
 // Pairs: h [T k, I] fp32, then the routed selection. Routed calls of more tokens: the selection, then what the grouped
 // kernels need (for any number of experts).
 int64_t dense_decode_ws_bytes(const tsa_expert_layout& L, int64_t T, int k) {
     const int64_t pairs = align256(T * k * L.inter * 4), table = 2 * align256(T * k * 4);
-    const int64_t grouped = T > DENSE_PAIR_TOKENS ? dense_places(L, dense_tokens(L, T, k), k, MAX_GROUP_E).bytes : 0;
+    const int64_t grouped = T > dense_pair_tokens(L, k) ? dense_places(L, dense_tokens(L, T, k), k, MAX_GROUP_E).bytes : 0;
     return table + (pairs > grouped ? pairs : grouped);
 }
 
@@ -519,7 +531,7 @@ int64_t dense_decode_ws_bytes(const tsa_expert_layout& L, int64_t T, int k) {
 bool dense_routes(int64_t T, int64_t E, int k) { return E <= 256 && k <= FUSED_MAXK && T * k <= 65535; }
 
 // What a call needs beyond its layout.
-static int check_dense(const tsa_expert_layout& L, const void* pool, const void* x, int x_dtype, const void* ws) {
+int check_dense(const tsa_expert_layout& L, const void* pool, const void* x, int x_dtype, const void* ws) {
     TSA_REQUIRE(((reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(ws)) & 15) == 0,
                 TSA_ERR_INVALID_ARG, "16-bit and int8 experts: pool, x and workspace must be 16-byte aligned");
     TSA_REQUIRE(L.format == TSA_EXPERT_INT8 || x_dtype == L.gate_type, TSA_ERR_INVALID_ARG,
@@ -581,11 +593,9 @@ int dense_decode(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slot
     return TSA_OK;
 }
 
-// Calls that the grouped kernels take (us of a layer grouped / as pairs, without the routing: hidden 2048, 128 experts top-8,
-// 2 / 3 / 4 / 8 tokens, bf16 39 / 43 / 47 / 56 and 34 / 46 / 58 / 105, int8 33 / 35 / 38 / 44 and 24 / 32 / 40 / 72; hidden 2880,
-// 32 experts top-4, 2 / 3 / 4 tokens, bf16 82 / 87 / 91 and 74 / 102 / 130, int8 62 / 62 / 65 and 57 / 76 / 96).
+// Calls that the grouped kernels take.
 bool dense_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {
-    return dense_format(L) && T > DENSE_PAIR_TOKENS && E <= MAX_GROUP_E && k <= 64;
+    return dense_format(L) && T > dense_pair_tokens(L, k) && E <= MAX_GROUP_E && k <= 64;
 }
 
 int64_t dense_group_workspace_bytes(const tsa_expert_layout& L, int64_t T, int k, int64_t E) {

@@ -11,7 +11,6 @@ constexpr int GROUP_WAVES = GROUP_THREADS / 64;
 constexpr int MAX_GROUP_E = 1024;
 constexpr int GROUP_AHEAD = 8;  // id batches loaded ahead per wave
 constexpr int F8_PAIR_TOKENS = 4;  // FP8 experts: calls of more tokens are grouped
-constexpr int DENSE_PAIR_TOKENS = 2;  // 16-bit and int8 experts: the same
 
 // Optional tile table (the grouped GGUF GEMMs' work list): per resident expert in id order,
 // entries of up to `rows` sorted rows {slot, first sorted row, rows, 0}; n_entries[0] = their

@@ -22,6 +22,9 @@ int f8_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_
                      const int32_t* idx, const float* weights, int64_t T, int k, const void* x, int x_dtype, void* y,
                      int y_dtype, uint8_t* ws, hipStream_t stream);
 
+bool dense_format(const tsa_expert_layout& L);
+int check_dense(const tsa_expert_layout& L, const void* pool, const void* x, int x_dtype, const void* ws);
+int64_t dense_pair_tokens(const tsa_expert_layout& L, int k);
 bool dense_group_supported(const tsa_expert_layout& L, int64_t T, int k, int64_t E);
 int64_t dense_group_workspace_bytes(const tsa_expert_layout& L, int64_t T, int k, int64_t E);
 int dense_group_prefill(const tsa_expert_layout& L, const uint8_t* pool, int64_t n_slots, const int32_t* expert_slot, int64_t E,
@@ -95,7 +98,7 @@ static int64_t prefill_ws(const tsa_expert_layout& L, int64_t T, int k, int64_t 
     // FP8, 16-bit and int8 pools are grouped whatever x's type, but for the few tokens that *_group_supported leaves (no
     // fewer bytes for more tokens: a workspace serves every call of its size and below)
     const bool f8 = f8_group_supported(L, T, k, E), dense = dense_group_supported(L, T, k, E);
-    const int64_t c = chunked_ws(L, f8 ? F8_PAIR_TOKENS : dense ? DENSE_PAIR_TOKENS : T, k);
+    const int64_t c = chunked_ws(L, f8 ? F8_PAIR_TOKENS : dense ? dense_pair_tokens(L, k) : T, k);
     int64_t g = 0;
     if (L.format == TSA_EXPERT_MXFP4 && L.mx_tiled) g = pf_mxt_workspace_bytes(L, T, k, E);
     if (gf_supported(L, TSA_BF16, T, k)) g = gf_workspace_bytes(L, T, k, E);
@@ -149,11 +152,15 @@ extern "C" int tsa_moe_prefill(const tsa_expert_layout* layout, const void* pool
         return f8_group_prefill(*layout, static_cast<const uint8_t*>(pool), n_slots, expert_slot, E, idx, weights, T, k, x, x_dtype,
                                 y, y_dtype, static_cast<uint8_t*>(workspace), as_stream(stream));
     }
-    if (dense_group_supported(*layout, T, k, E)) {
+    if (dense_format(*layout)) {
         TSA_REQUIRE(pool && x && y, TSA_ERR_INVALID_ARG, "null pointer");
         TSA_REQUIRE(valid_dtype(x_dtype) && valid_dtype(y_dtype), TSA_ERR_INVALID_ARG, "bad dtype (x %d, y %d)", x_dtype, y_dtype);
-        return dense_group_prefill(*layout, static_cast<const uint8_t*>(pool), n_slots, expert_slot, E, idx, weights, T, k, x,
-                                   x_dtype, y, y_dtype, static_cast<uint8_t*>(workspace), as_stream(stream));
+        TSA_REQUIRE(k <= 64, TSA_ERR_INVALID_ARG, "k %d exceeds 64", k);
+        rc = check_dense(*layout, pool, x, x_dtype, workspace);
+        if (rc) return rc;
+        if (dense_group_supported(*layout, T, k, E))
+            return dense_group_prefill(*layout, static_cast<const uint8_t*>(pool), n_slots, expert_slot, E, idx, weights, T, k, x,
+                                       x_dtype, y, y_dtype, static_cast<uint8_t*>(workspace), as_stream(stream));
     }
     int32_t* slots = static_cast<int32_t*>(workspace);
     const int64_t off = ((T * k * 4 + 255) / 256) * 256;
