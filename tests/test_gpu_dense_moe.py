@@ -295,3 +295,61 @@ def test_pipeline_and_hook(tmp_path, kind, T):
         ref.check(pipe.execute_layer_experts_batched(x, li, idx, w), *ref.moe(x, idx, w, ex), "batched")
         items = [BatchItem(x[i : i + 1], idx[i], w[i], i) for i in range(T)]
         ref.check(torch.cat(pipe.execute_batched_experts(items, li)), *ref.moe(x, idx, w, ex), "batcher")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,I,E,k,T", [(256, 320, 12, 4, 16), (256, 320, 12, 4, 17), (1024, 1024, 9, 2, 6), (1024, 1024, 9, 2, 7),
+                                       (1024, 1024, 9, 2, 12), (1024, 1024, 9, 2, 13), (2048, 768, 10, 8, 2), (2048, 768, 10, 8, 3),
+                                       (64, 32, 70, 64, 2), (64, 32, 70, 64, 3), (64, 32, 3, 1, 64), (64, 32, 3, 1, 65)])
+def test_last_tokens_as_pairs(kind, H, I, E, k, T):
+    """Either side of the most tokens that run as pairs, routed and given; the buffers that a capture would hold."""
+    L, pool, experts = layer(kind, H, I, E)
+    x, lg = tokens(kind, T, H, E, k)
+    slot = torch.arange(E, dtype=torch.int32, device="cuda")
+    y, idx, w = ops.moe_decode_routed(L, pool, slot, lg, x, k, return_routing=True, workspace=ops.moe_decode_workspace(L, T, k, "cuda"))
+    want = ref.moe(x, idx, w, experts)
+    ref.check(y, *want, "routed")
+    ref.check(ops.moe_decode(L, pool, idx, w, x), *want, "given")
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), *want, "prefill")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_prompt_in_pieces(kind):
+    """More assignments than are worked on at a time."""
+    H, I, E, k, T = 64, 32, 6, 4, 70_001
+    L, pool, experts = layer(kind, H, I, E)
+    x, lg = tokens(kind, T, H, E, k)
+    idx, w = ops.route_topk(lg, k)
+    slot = torch.arange(E, dtype=torch.int32, device="cuda")
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), *ref.moe(x, idx, w, experts))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_far_slots(kind):
+    """Slots past 2^32 bytes of the pool."""
+    H, I, E, k = 256, 96, 6, 3
+    L, small, experts = layer(kind, H, I, E)
+    L.slot_bytes = 2**30 - 16
+    pool = torch.zeros((E, 2**30 - 16), dtype=torch.uint8, device="cuda")
+    pool[:, : small.shape[1]] = small
+    slot = torch.arange(E, dtype=torch.int32, device="cuda")
+    for T in (1, 2, 50):
+        x, lg = tokens(kind, T, H, E, k)
+        y, idx, w = ops.moe_decode_routed(L, pool, slot, lg, x, k, return_routing=True)
+        want = ref.moe(x, idx, w, experts)
+        ref.check(y, *want, "routed")
+        ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), *want, "prefill")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [2, 60])
+def test_same_expert_twice(kind, T):
+    """A selection that names an expert more than once adds it as often."""
+    L, pool, experts = layer(kind, 256, 96, 4)
+    x, _ = tokens(kind, T, 256, 4, 3)
+    idx = torch.tensor([[1, 1, 3], [2, 2, 2]], dtype=torch.int32, device="cuda").repeat(T // 2, 1)
+    w = torch.rand((T, 3), device="cuda", generator=gen(5))
+    slot = torch.arange(4, dtype=torch.int32, device="cuda")
+    want = ref.moe(x, idx, w, experts)
+    ref.check(ops.moe_decode(L, pool, idx, w, x), *want, "decode")
+    ref.check(ops.moe_prefill(L, pool, slot, idx, w, x), *want, "prefill")

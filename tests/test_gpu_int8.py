@@ -259,3 +259,146 @@ def test_grouped_nothing():
     off = torch.zeros(4, dtype=torch.int32, device="cuda")
     assert ops.grouped_matmul(x[:0], w, off, b).shape == (0, 72)
     assert ops.grouped_matmul(x[:0], w, off, b, rows=off[:0]).shape == (0, 72)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("E", [5, 300, 1000])
+def test_grouped_offsets_that_do_not_ascend(kind, E):
+    """Offsets are raised to the largest before them and cut to the rows there are: each row is in one group."""
+    x, w, ws, b, _, rows = grouped_case(kind, E, 48, 64, 90, 2)
+    off = torch.randint(-50, 300, (E + 1,), device="cuda", generator=gen(E)).int()
+    off[0] = 7
+    top = off.clamp(0, 180).cummax(0).values.tolist()
+    ref.check(run_grouped(x, w, ws, off.tolist(), b, rows, 2), *want_grouped(x, w, ws, top, b, rows, 2))
+    worst = torch.arange(E, -1, -1, device="cuda").int() * 2**20
+    ref.check(run_grouped(x, w, ws, worst.tolist(), b, rows, 2), *want_grouped(x, w, ws, worst.clamp(0, 180).cummax(0).values.tolist(), b, rows, 2))
+
+
+# ----------------------------------------------------------------------------- where rules change, and far ends
+@pytest.mark.parametrize("T", [11, 12, 13, 14, 95, 96, 97, 128, 160, 161, 192, 193, 224, 225, 256, 257, 320])
+@pytest.mark.parametrize("K,N", [(2048, 512), (704, 2880), (720, 4096), (256, 5760)])
+def test_linear_where_kernels_change(T, K, N):
+    """Around the last token count that is quantised inside the product, and that the row kernel takes."""
+    x, w, ws, b = linear_case(T, K, N, torch.bfloat16, torch.float32)
+    want, err = ref.matmul(*ref.quantize(x), w, ws, b)
+    ref.check(ops.int8_linear(x, w, ws, b), want, err)
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 12])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", [8192, 8208, 10912, 10928, 32768, 131056])
+def test_linear_long_rows(T, K, dtype):
+    """Rows longer than what a wave holds, and than what LDS holds (quantised by a launch of their own)."""
+    x, w, ws, b = linear_case(T, K, 40, dtype, None)
+    want, err = ref.matmul(*ref.quantize(x), w, ws, b)
+    ref.check(ops.int8_linear(x, w, ws, b), want, err)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("per", [1, 4, 5, 48, 49])
+def test_grouped_where_tiles_change(kind, per):
+    """Rows per expert on average at the ends of the tiles' ranges."""
+    x, w, ws, b, off, rows = grouped_case(kind, 7, 200, 144, 7 * per, 1)
+    for R in (7 * per - 1, 7 * per):
+        o = [min(v, R) for v in off]
+        ref.check(run_grouped(x, w, ws, o, b, rows[:R].contiguous()), *want_grouped(x, w, ws, o, b, rows[:R]))
+
+
+def test_many_tokens():
+    """More tokens than a launch has threads for, results past 2^32 bytes."""
+    T, K, N = 2**26 + 17, 16, 40
+    x = torch.randn((2**20, K), device="cuda", generator=gen(1)).bfloat16().repeat(65, 1)[:T]
+    x[-40:] *= 3
+    w, ws = ref.weights8(gen(2), N, K)
+    codes, scales = ops.int8_quantize(x)
+    y = ops.int8_matmul(codes, scales, w, ws)
+    for at in (0, 2**25 - 20, 2**31 // 80 - 100, 2**32 // 80 - 100, 2**26 - 100):
+        part = slice(at, min(T, at + 200))
+        check_codes(x[part], codes[part], scales[part])
+        ref.check(y[part], *ref.matmul(*ref.quantize(x[part]), w, ws), f"from {at}")
+    assert torch.equal(y[2**20 : 2**21], y[: 2**20])
+    again = ops.int8_linear(x, w, ws)
+    assert all(torch.equal(a, b) for a, b in zip(again.split(2**24), y.split(2**24)))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_grouped_far_offsets(kind):
+    """Experts whose matrices lie past 2^32 bytes, results that do."""
+    es, K, N = (1, 65536, 1024) if kind == "int8" else (2, 32768, 1024)
+    E = 70  # of 64 MiB
+    w = torch.zeros((E, N, K), dtype=torch.int8 if es == 1 else torch.bfloat16, device="cuda")
+    ws = torch.full((E, N), 2.0**-7, device="cuda") if es == 1 else None
+    for e in (0, 31, 32, 63, 64, 69):
+        r = torch.randint(-127, 128, (N, 128), device="cuda", generator=gen(e))
+        w[e, :, ::K // 128] = r.to(w.dtype)
+    x = acts(gen(3), 30, K)
+    sizes = {0: 5, 31: 3, 32: 4, 63: 6, 64: 5, 69: 7}
+    off = [0]
+    for e in range(E):
+        off.append(off[-1] + sizes.get(e, 0))
+    ref.check(run_grouped(x, w, ws, off), *want_grouped(x, w, ws, off))
+    del w
+    R, N, K = 1_100_000, 2048, 16
+    x = acts(gen(4), 4096, K).repeat(R // 4096 + 1, 1)[:R]
+    w, ws = ref.weights8(gen(5), 2, N, K) if es == 1 else (0.1 * torch.randn((2, N, K), device="cuda", generator=gen(5)).bfloat16(), None)
+    y = run_grouped(x, w, ws, [0, 600_000, R - 50])
+    for at in (0, 2**31 // 4096 - 50, 600_000 - 100, 2**32 // 4096 - 50, R - 200):
+        n = min(200, R - at)
+        cut = [min(n, max(0, o - at)) for o in (0, 600_000, R - 50)]
+        ref.check(y[at : at + n], *want_grouped(x[at : at + n], w, None if ws is None else ws, cut), f"from {at}")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_grouped_x_at_its_limit(kind):
+    """Rows picked from an x of nearly 2^31 bytes."""
+    K = 2048 if kind == "int8" else 1024
+    rows_x = 2**20 - 1
+    x = acts(gen(6), 1023, K).repeat(1025, 1)[:rows_x]
+    w, ws = ref.weights8(gen(7), 2, 48, K) if kind == "int8" else (0.1 * torch.randn((2, 48, K), device="cuda", generator=gen(7)).bfloat16(), None)
+    rows = torch.tensor([0, rows_x - 1, 2**19, 2**19 - 1, rows_x, rows_x - 2, 3, rows_x - 1], dtype=torch.int32, device="cuda")
+    y = run_grouped(x, w, ws, [0, 5, 8], None, rows)
+    small = torch.where(rows < rows_x, torch.arange(8, device="cuda").int(), torch.tensor(8, device="cuda", dtype=torch.int32))
+    ref.check(y, *want_grouped(x[rows.long().clamp(max=rows_x - 1)], w, ws, [0, 5, 8], None, small))
+
+
+def test_captured_and_on_a_stream():
+    """Captured calls replayed on new inputs, eager ones between; and the same on a stream of the caller's."""
+    w, ws = ref.weights8(gen(1), 200, 288)
+    wg, wgs = ref.weights8(gen(2), 4, 80, 288)
+    w16 = (0.05 * torch.randn((4, 80, 288), device="cuda", generator=gen(3))).bfloat16()
+    xs = [acts(gen(4), T, 288) for T in (1, 12, 40, 300)]
+    off = torch.tensor([0, 100, 100, 180, 290], dtype=torch.int32, device="cuda")
+
+    def step():
+        out = [ops.int8_linear(x, w, ws) for x in xs]
+        codes, scales = ops.int8_quantize(xs[3])
+        out += [ops.int8_matmul(codes, scales, w, ws), ops.int8_grouped_matmul(codes, scales, wg, wgs, off), ops.grouped_matmul(xs[3], w16, off)]
+        return out
+
+    def check(outs):
+        for x, y in zip(xs, outs):
+            ref.check(y, *ref.matmul(*ref.quantize(x), w, ws))
+        assert torch.equal(outs[4], outs[3])
+        o = off.tolist()
+        ref.check(outs[5], *ref.grouped(ref.quantize(xs[3]), wg, o, int8=wgs))
+        ref.check(outs[6], *ref.grouped(xs[3], w16, o))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        for x in xs:
+            x.copy_(acts(gen(100 + seed + len(x)), *x.shape))
+        graph.replay()
+        got = [y.clone() for y in outs]
+        check(got)
+        assert all(torch.equal(a, b) for a, b in zip(step(), got))
+        torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = step()
+    torch.cuda.current_stream().wait_stream(side)
+    check(outs)

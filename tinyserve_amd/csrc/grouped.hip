@@ -24,7 +24,8 @@ struct Grouped {
     MmOut out;  // its bias: [E, N]
 };
 
-// Inclusive prefix sum over the wave's lanes (DPP: row shifts, then the rows' last lanes passed on).
+// Over the wave's lanes (DPP: row shifts, then the rows' last lanes passed on): the sum up to this lane, and the largest
+// of the lanes before it (0 for none; of numbers that are not negative).
 __device__ __forceinline__ int wave_incl_sum(int v) {
     v += dpp_i<0x111, 0xF, 0xF>(v, 0);
     v += dpp_i<0x112, 0xF, 0xF>(v, 0);
@@ -34,10 +35,19 @@ __device__ __forceinline__ int wave_incl_sum(int v) {
     v += dpp_i<0x143, 0xC, 0xF>(v, 0);
     return v;
 }
+__device__ __forceinline__ int wave_excl_max(int v) {
+    v = max(v, dpp_i<0x111, 0xF, 0xF>(v, 0));
+    v = max(v, dpp_i<0x112, 0xF, 0xF>(v, 0));
+    v = max(v, dpp_i<0x114, 0xF, 0xF>(v, 0));
+    v = max(v, dpp_i<0x118, 0xF, 0xF>(v, 0));
+    v = max(v, dpp_i<0x142, 0xA, 0xF>(v, 0));
+    v = max(v, dpp_i<0x143, 0xC, 0xF>(v, 0));
+    return __shfl_up(v, 1, 64) * ((threadIdx.x & 63) != 0);
+}
 
 // A workgroup's tiles (mm_pair's order; an entry: up to TM rows of a group). The rows ahead of the first group and
-// behind the last are groups of their own, of no expert. Offsets that do not ascend, or leave [0, R], give groups cut
-// to it: every row that is touched is one of the R.
+// behind the last are groups of their own, of no expert. Offsets that do not ascend, or leave [0, R], are raised to the
+// largest before them and cut to it: each of the R rows is in one group whatever they hold.
 template <class C, class E>
 struct GroupedWork {
     static constexpr int TM = C::TM;
@@ -51,10 +61,18 @@ struct GroupedWork {
         const int v = p.offsets[g < 1 ? 0 : g - 1 > p.E ? p.E : g - 1];
         return g < 1 ? 0 : g > p.E + 1 ? p.R : v < 0 ? 0 : v > p.R ? p.R : v;
     }
+    int reached;  // the largest bound of the groups ahead of those that are loaded
     __device__ __forceinline__ void load(int g0) {
         const int lane = (int)threadIdx.x & 63;
+        if (g0 == 0) reached = 0;
 #pragma unroll
         for (int j = 0; j < 5; ++j) b[j] = bound(g0 + 4 * lane + j);
+#pragma unroll
+        for (int j = 1; j < 5; ++j) b[j] = max(b[j], b[j - 1]);
+        const int before = max(reached, wave_excl_max(b[4]));
+#pragma unroll
+        for (int j = 0; j < 5; ++j) b[j] = max(b[j], before);
+        reached = __builtin_amdgcn_readlane(b[4], 63);
         sum = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -128,14 +146,14 @@ struct GroupedWork {
         return MmOperands<1>{{w}, p.N - next_n0, x, (uint32_t)(p.rows ? p.x_rows : next_tn) * (uint32_t)p.KB, next_tn};
     }
     __device__ __forceinline__ void take() { expert = next_expert, n0 = next_n0, row0 = next_row0, tn = next_tn; }
-    __device__ __forceinline__ bool store(const typename E::acc (&acc)[C::MR][C::MT], uint8_t* out) const {
+    __device__ __forceinline__ void store(const typename E::acc (&acc)[C::MR][C::MT], uint8_t* out) const {
         MmOut o = p.out;
         if (o.bias) o.bias = static_cast<const uint8_t*>(o.bias) + (int64_t)expert * p.N * (o.bias_dtype == TSA_F32 ? 4 : 2);
         auto scale = [&](int r) {
             const int t = p.rows ? picked(row0 + r) : row0 + r;
             return t >= 0 ? p.xs[t] : 0.0f;
         };
-        return mm_store<C>(acc, o, out, n0, p.N, tn, [&](int r) { return (int64_t)(row0 + r); }, scale, p.ws + (int64_t)expert * p.N);
+        mm_store<C>(acc, o, out, n0, p.N, tn, [&](int r) { return (int64_t)(row0 + r); }, scale, p.ws + (int64_t)expert * p.N);
     }
 };
 

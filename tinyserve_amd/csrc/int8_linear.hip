@@ -27,9 +27,16 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const uint8_t* __res
 template <int XT, bool VEC>
 hipError_t launch_quantize(const void* x, int64_t T, int64_t K, uint8_t* codes, float* scales, hipStream_t st) {
     const uint8_t* xb = static_cast<const uint8_t*>(x);
-    if (T < 1024) hipLaunchKernelGGL((int8_quantize_kernel<XT, VEC, 4>), dim3((unsigned)T), dim3(256), 0, st, xb, T, K, codes, scales);
-    else hipLaunchKernelGGL((int8_quantize_kernel<XT, VEC, 1>), dim3((unsigned)((T + 3) / 4)), dim3(256), 0, st, xb, T, K, codes, scales);
-    return hipGetLastError();
+    constexpr int64_t STEP = (int64_t)1 << 25;  // rows of a launch, which ends at 2^32 threads
+    for (int64_t t = 0; t < T; t += STEP) {
+        const int64_t n = T - t < STEP ? T - t : STEP;
+        const uint8_t* xt = xb + t * K * (XT == TSA_F32 ? 4 : 2);
+        if (n < 1024) hipLaunchKernelGGL((int8_quantize_kernel<XT, VEC, 4>), dim3((unsigned)n), dim3(256), 0, st, xt, n, K, codes + t * K, scales + t);
+        else hipLaunchKernelGGL((int8_quantize_kernel<XT, VEC, 1>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, xt, n, K, codes + t * K, scales + t);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <int XT>
@@ -242,8 +249,8 @@ struct I8Work {
         return MmOperands<1>{{p.w + (int64_t)next_n0 * p.K}, p.N - next_n0, p.x + (int64_t)next_t0 * p.K, (uint32_t)next_tn * (uint32_t)p.K, next_tn};
     }
     __device__ __forceinline__ void take() { n0 = next_n0, t0 = next_t0, tn = next_tn; }
-    __device__ __forceinline__ bool store(const v4i (&acc)[C::MR][C::MT], uint8_t* out) const {
-        return mm_store<C>(acc, p.out, out, n0, p.N, tn, [&](int r) { return (int64_t)(t0 + r); }, [&](int r) { return p.xs[t0 + r]; }, p.ws);
+    __device__ __forceinline__ void store(const v4i (&acc)[C::MR][C::MT], uint8_t* out) const {
+        mm_store<C>(acc, p.out, out, n0, p.N, tn, [&](int r) { return (int64_t)(t0 + r); }, [&](int r) { return p.xs[t0 + r]; }, p.ws);
     }
 };
 
@@ -299,9 +306,10 @@ int gemm_tile(int64_t T, int64_t N, int64_t* time = nullptr) {
 // Whether the row kernel takes a product: up to 32 tokens, and more while its rounds of 16 rows x 32 tokens on every CU take
 // less than the tiles. us of the row kernel / the tiles, weights from memory: 2880 x 2880, 64 / 128 / 192 tokens 8.3 / 16.8, 10.9 /
 // 17.0 and 15.4 / 15.4; 2048 x 4096, 128 / 192 / 256 14.1 / 21.8, 19.3 / 21.8 and 24.4 / 21.9; 5760 x 2880, 64 / 96 / 128 10.9 / 17.0,
-// 15.5 / 15.6 and 17.8 / 15.5; 512 x 2048, 512 tokens 8.3 / 12.9.
+// 15.5 / 15.6 and 17.8 / 15.5; 512 x 2048, 512 tokens 8.3 / 12.9. (Past 2^20 tokens, where one 16-row tile's workgroups would near a launch's
+// limit, the tiles always.)
 bool rows_kernel(int64_t T, int64_t N) {
-    if (T <= 32) return true;
+    if (T <= 32 || T > 1 << 20) return T <= 32;
     const int64_t cus = num_cus() > 0 ? num_cus() : 256, on = ((N + 15) / 16 * ((T + 31) / 32) + cus - 1) / cus;
     int64_t time;
     return gemm_tile(T, N, &time) >= 0 && 3 + 3 * on <= time;

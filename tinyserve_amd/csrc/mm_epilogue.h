@@ -42,8 +42,8 @@ __device__ __forceinline__ uint2 mm_pack4(const v4f& v) {
 }
 
 // 16 tokens' rows of 16 M values, lane 16 q + i holding values 16 m + 4 q .. of token i in v[m]: to(r, c) is where piece c
-// of token r goes, or null. ALL: it never is (and every store is issued).
-template <int M, bool ALL, class To>
+// of token r goes, or null.
+template <int M, class To>
 __device__ __forceinline__ void mm_rows16(const uint2 (&v)[M], uint8_t* out, To to) {
     constexpr int P = 2 * M;  // pieces of a row
     const int lane = threadIdx.x & 63, q = lane >> 4, i = lane & 15;
@@ -57,7 +57,7 @@ __device__ __forceinline__ void mm_rows16(const uint2 (&v)[M], uint8_t* out, To 
         if (P < 4 && r >= 16) continue;
         const u32x4 d = *reinterpret_cast<const u32x4*>(out + 16 * (r * P + (c ^ (r * P / 16))));
         void* dst = to(r, c);
-        if (ALL || dst) *static_cast<u32x4*>(dst) = d;
+        if (dst) *static_cast<u32x4*>(dst) = d;
     }
     asm volatile("" ::: "memory");
 }
@@ -91,9 +91,9 @@ __device__ __forceinline__ v4f mm_bias4(const void* p, int dtype, int n, int N) 
 }
 
 // The tile's rows n0 .. (below N) of its first tn tokens; row(r): y's row of token r. int8 sums are scaled by
-// xs(r) and ws[n]. True where all the last stores are at least MR MT / 2 unconditional ones.
+// xs(r) and ws[n].
 template <class C, class A, class Row, class Scale>
-__device__ __forceinline__ bool mm_store(const A (&acc)[C::MR][C::MT], const MmOut& o, uint8_t* out, int n0, int N, int tn, Row row,
+__device__ __forceinline__ void mm_store(const A (&acc)[C::MR][C::MT], const MmOut& o, uint8_t* out, int n0, int N, int tn, Row row,
                                          Scale xs, const float* ws) {
     constexpr bool INT = std::is_same<A, v4i>::value;
     constexpr int MR = C::MR, MT = C::MT;
@@ -140,7 +140,7 @@ __device__ __forceinline__ bool mm_store(const A (&acc)[C::MR][C::MT], const MmO
                 }
             }
         }
-        return full;
+        return;
     }
     auto rows16 = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
@@ -169,14 +169,12 @@ __device__ __forceinline__ bool mm_store(const A (&acc)[C::MR][C::MT], const MmO
                 if (!full && (tk >= tn || n >= N)) return nullptr;  // N % 8 == 0
                 return static_cast<uint16_t*>(o.y) + row(tk) * o.ldy + n;
             };
-            if (full) mm_rows16<MR, true>(v, out, to);
-            else mm_rows16<MR, false>(v, out, to);
+            mm_rows16<MR>(v, out, to);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (o.y_dtype == TSA_BF16) rows16(std::integral_constant<int, TSA_BF16>{});
     else rows16(std::integral_constant<int, TSA_F16>{});
-    return full;
 }
 
 }  // namespace

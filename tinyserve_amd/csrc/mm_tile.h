@@ -62,7 +62,7 @@ struct MmTile {
     static constexpr int STAGE = (RN + 8 * NW * NXT) * MMB;
     static constexpr int OUT = 16 * MR * 32;  // a wave's place for 16 tokens' results of 16 bits
     static constexpr int LDS = S * STAGE + NW * OUT;
-    static_assert(RN % (8 * NW) == 0 && (S - 1) * PER + MR * MT < 63 && S >= 2 && LDS <= 160 * 1024, "tile");
+    static_assert(RN % (8 * NW) == 0 && (S - 1) * PER < 63 && S >= 2 && LDS <= 160 * 1024, "tile");
 };
 
 // What a tile multiplies. Weight row r of the tile (r < RN) is row r of w[r / (RN / PARTS)] counted
@@ -76,27 +76,17 @@ struct MmOperands {
     int tokens;
 };
 
-// This wave's copies have landed but for the newest N, and its LDS reads are done; then the barrier. `stores`: another
-// STORES of the newest operations are stores that nothing here waits for (reads and writes are counted together, in
-// the order of their issue).
-template <int N, int STORES>
-__device__ __forceinline__ void mm_wait(bool stores) {
-    if (stores) wait_copies_barrier<N + STORES>();
-    else wait_copies_barrier<N>();
-}
-
 // Works through `work`'s tiles. KB: bytes of a row of either operand, a multiple of 16.
 //   bool work.next(): the next tile becomes work's pending one (uniform); false: there is none
 //   MmOperands<PARTS> work.operands(), int work.token(r): of the pending tile; the row of x of its token r (-1: zeros);
 //     GATHER false: token r is row r
 //   void work.take(): the pending tile becomes the current one
-//   bool work.store(acc, out): the current tile's results; `out`: this wave's place in LDS. True: at least MR MT / 2
-//     stores were the last that was done.
+//   void work.store(acc, out): the current tile's results; `out`: this wave's place in LDS
 // acc[m][t]: rows 4 q .. 4 q + 3 of tile m, token 16 t + i, for lane 16 q + i of the wave. Tile m is
 // the wave's m-th: of its MR, the first MR / PARTS belong to part 0.
 template <class C, class E, int PARTS, bool GATHER, class Work>
 __device__ __forceinline__ void mm_run(Work& work, uint32_t KB, uint8_t* smem) {
-    constexpr int MR = C::MR, MT = C::MT, S = C::S, HALF = C::RN / PARTS, MP = MR / PARTS, STORES = MR * MT / 2;
+    constexpr int MR = C::MR, MT = C::MT, S = C::S, HALF = C::RN / PARTS, MP = MR / PARTS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
     const int wr = wave % C::WR, wt = wave / C::WR;
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(smem);
@@ -171,7 +161,6 @@ __device__ __forceinline__ void mm_run(Work& work, uint32_t KB, uint8_t* smem) {
         for (int j = 0; j < C::PER; ++j) issue(j, s, s);
     wait_copies_barrier<(S - 1) * C::PER>();
     int stage = 0;
-    bool stored = false;  // the tile before left its stores behind
     do {
         work.take();
         tokens = pending;
@@ -212,7 +201,7 @@ __device__ __forceinline__ void mm_run(Work& work, uint32_t KB, uint8_t* smem) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // every wave has read this stage, and the next step has landed
-                mm_wait<(S - 2) * C::PER, STORES>(stored && s < S - 1);
+                wait_copies_barrier<(S - 2) * C::PER>();
                 const int next = stage + 1 == S ? 0 : stage + 1;
                 const uint8_t* wn = smem + next * C::STAGE;
 #pragma unroll
@@ -227,7 +216,7 @@ __device__ __forceinline__ void mm_run(Work& work, uint32_t KB, uint8_t* smem) {
             }
         }
         if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may land after the workgroup's end
-        stored = work.store(acc, smem + S * C::STAGE + wave * C::OUT);
+        work.store(acc, smem + S * C::STAGE + wave * C::OUT);
     } while (more);
 }
 

@@ -153,7 +153,8 @@ __device__ const uint32_t dense_zeros[4] = {0, 0, 0, 0};  // what lanes past a m
 
 // One workgroup per token and 4 outputs, over all the token's experts: rows 4 e .. 4 e + 3 of a tile are the outputs' rows
 // of the e-th of four experts, which meet column e (its h); a unit is a step of 128 bytes of such four, and the waves take
-// the units in turn. (Two experts and 8 outputs, half as many workgroups: XX.) int8: the experts' h are quantised in LDS.
+// the units in turn. (Against two experts and 8 outputs, half as many workgroups: 180 us for 189, 8 layers of
+// hidden 2048, 128 experts top-8, bf16, one token.) int8: the experts' h are quantised in LDS.
 template <class E>
 __global__ void __launch_bounds__(64 * DMD_NW, 4) dense_down_kernel(DenseMoe p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -352,7 +353,7 @@ struct DenseUp : DenseWork<C> {
         return MmOperands<2>{{base + L.gate_off + (int64_t)c0 * KB, base + L.up_off + (int64_t)c0 * KB}, (int)L.inter - c0, B::p.xq,
                              (uint32_t)B::p.T * (uint32_t)KB, B::next_tn};
     }
-    __device__ __forceinline__ bool store(const typename E::acc (&acc)[C::MR][MT], uint8_t* out) const {
+    __device__ __forceinline__ void store(const typename E::acc (&acc)[C::MR][MT], uint8_t* out) const {
         const DenseGroup& p = B::p;
         const tsa_expert_layout& L = p.L;
         const int I = (int)L.inter, lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), q = lane >> 4, i = lane & 15;
@@ -393,13 +394,12 @@ struct DenseUp : DenseWork<C> {
                 uint2 v[MP];
 #pragma unroll
                 for (int m = 0; m < MP; ++m) v[m] = mm_pack4<std::is_same<E, MmBf16>::value ? TSA_BF16 : TSA_F16>(h[m]);
-                mm_rows16<MP, false>(v, out, [&](int r, int c) -> void* {
+                mm_rows16<MP>(v, out, [&](int r, int c) -> void* {
                     const int tk = t0 + 16 * t + r, n = cw + 8 * c;
                     return tk < B::tn && n < I ? static_cast<uint16_t*>(p.h) + (int64_t)(B::row0 + tk) * I + n : nullptr;
                 });
             }
         }
-        return false;
     }
 };
 
@@ -414,11 +414,11 @@ struct DenseDown : DenseWork<C> {
         return MmOperands<1>{{B::p.pool + (int64_t)B::next_slot * L.slot_bytes + L.down_off + (int64_t)n0 * KB}, (int)L.hidden - n0,
                              B::p.hq + (int64_t)B::next_row0 * KB, (uint32_t)B::next_tn * (uint32_t)KB, B::next_tn};
     }
-    __device__ __forceinline__ bool store(const typename E::acc (&acc)[C::MR][C::MT], uint8_t* out) const {
+    __device__ __forceinline__ void store(const typename E::acc (&acc)[C::MR][C::MT], uint8_t* out) const {
         const DenseGroup& p = B::p;
         const int H = (int)p.L.hidden;
         const MmOut o = MmOut{p.yk, TSA_F32, H, nullptr, 0, 1};  // H % 32 == 0: rows of whole 16-byte pieces
-        return mm_store<C>(acc, o, out, B::tile * C::RN, H, B::tn, [&](int r) { return (int64_t)p.perm[B::row0 + r]; },
+        mm_store<C>(acc, o, out, B::tile * C::RN, H, B::tn, [&](int r) { return (int64_t)p.perm[B::row0 + r]; },
                            [&](int r) { return p.hs[B::row0 + r]; },
                            reinterpret_cast<const float*>(p.pool + (int64_t)B::slot * p.L.slot_bytes + p.L.down_scales_off));
     }
