@@ -10,8 +10,10 @@
 // stages in LDS by buffer-to-LDS copies; rows and columns past the matrices are offsets past the buffers,
 // which copy zeros. The 16-byte chunk c of row r sits in slot c ^ (r / 2 % 8): the 16 rows that a quarter wave
 // reads at once then fall on distinct banks. The barrier sits between a step's two products: by then the
-// second half's operands are in registers, so the stage is free for the copies of step s + S, which go out
-// among the second half's products, as do the LDS reads of step s + 1.
+// second half's operands are in registers, so the stage is free for the copies of step s + S. They go out among the
+// products of the second half and of the next step's first (with two stages, which are waited for there, of the second
+// half alone; all of them there with three: 2% slower, 4096 x 5760 x 2880 int8 90.5 us for 88.3, 8192 rows of 32
+// experts of 5760 x 2880 bf16 378 for 371). The LDS reads of a half go out among the products of the half before.
 //
 // A workgroup works through tiles one after the other, and their steps are one stream: the last S steps of a tile
 // issue the copies of the next tile's first, and the results go out while those land.
@@ -184,37 +186,55 @@ __device__ __forceinline__ void mm_run(Work& work, uint32_t KB, uint8_t* smem) {
                 for (int t = H0; t < MT; ++t) acc[m][t] = E::mfma(A[h][m], Bv[h][t], acc[m][t]);
             }
         };
+        // row tile m's turn of copies [j0, j1)
+        auto copies = [&](int m, int j0, int j1, int s, int into) {
+#pragma unroll
+            for (int j = j0 + m * (j1 - j0) / MR; j < j0 + (m + 1) * (j1 - j0) / MR; ++j) issue(j, s, into);
+        };
+        auto second = [&](int s, int copied) {  // of step s, and of the copies of step s + S the first `copied`
+            const int next = stage + 1 == S ? 0 : stage + 1;
+            const uint8_t* wn = smem + next * C::STAGE;
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                fetch(wn, m, 0);
+                products(m, 1);
+                copies(m, 0, copied, s, stage);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        constexpr int FIRST = S > 2 ? C::PER / 2 : C::PER;
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            fetch(smem + stage * C::STAGE, m, 1);
+            products(m, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        wait_copies_barrier<(S - 2) * C::PER>();
 #pragma unroll 1
         for (int part = 0; part < 2; ++part) {  // the steps whose copies are this tile's, then those of the next
             if (part) {
                 more = work.next();
                 setup(more);
             }
-            const int s1 = part ? steps : steps - S, ahead = part ? S - steps : S;
+            const int s1 = part ? steps - 1 : steps - S, ahead = part ? S - steps : S;
 #pragma unroll 1
             for (int s = part ? steps - S : 0; s < s1; ++s) {
-                const uint8_t* wl = smem + stage * C::STAGE;
+                second(s + ahead, FIRST);
+                const int free = stage;
+                stage = stage + 1 == S ? 0 : stage + 1;
 #pragma unroll
                 for (int m = 0; m < MR; ++m) {
-                    fetch(wl, m, 1);
+                    fetch(smem + stage * C::STAGE, m, 1);
                     products(m, 0);
+                    copies(m, FIRST, C::PER, s + ahead, free);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // every wave has read this stage, and the next step has landed
                 wait_copies_barrier<(S - 2) * C::PER>();
-                const int next = stage + 1 == S ? 0 : stage + 1;
-                const uint8_t* wn = smem + next * C::STAGE;
-#pragma unroll
-                for (int m = 0; m < MR; ++m) {
-                    fetch(wn, m, 0);
-                    products(m, 1);
-#pragma unroll
-                    for (int j = m * C::PER / MR; j < (m + 1) * C::PER / MR; ++j) issue(j, s + ahead, stage);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                stage = next;
             }
         }
+        second(S - 1, C::PER);
+        stage = stage + 1 == S ? 0 : stage + 1;
         if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may land after the workgroup's end
         work.store(acc, smem + S * C::STAGE + wave * C::OUT);
     } while (more);
