@@ -225,6 +225,38 @@ def test_layouts_of_slots():
         int8_expert_layout(TensorLayout({n: lay.specs[n] for n in names[:3] + [names[4], names[3], names[5]]}))
 
 
+@pytest.mark.parametrize("H,I,act", [(256, 160, nn.GELU()), (256, 160, torch.nn.functional.relu), (250, 160, None), (256, 48, nn.SiLU()),
+                                     (32768, 32, None), (64, 16416, None)])
+def test_16_bit_slots_for_their_template(H, I, act):
+    """16-bit experts that the kernels do not take have no kernel layout: a pipeline runs them through its template."""
+    from tinyserve_amd.expert_forward import forward_from_packed
+    from tinyserve_amd.expert_pipeline import ExpertPipeline
+
+    bf, specs = torch.bfloat16, {"gate_proj": ((I, H), torch.bfloat16), "up_proj": ((I, H), torch.bfloat16), "down_proj": ((H, I), torch.bfloat16)}
+    lay = TensorLayout(specs)
+    assert build_expert_layout(lay, act) is None and _build_dense_inline_forward(lay, act) is None and _build_cpp_layout_args(lay, act) is None
+    assert build_expert_layout(TensorLayout({**specs, "down_proj": ((H, I + 32), bf)})) is None
+
+    class Template(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self._act_fn = act
+            for n, (shape, dt) in specs.items():
+                self.register_parameter(n, nn.Parameter(torch.zeros(shape, dtype=dt), requires_grad=False))
+
+        def forward(self, h):
+            return (self._act_fn or nn.functional.silu)(h @ self.gate_proj.t()) * (h @ self.up_proj.t()) @ self.down_proj.t()
+
+    packed = torch.randn(lay.total_bytes // 2).to(bf).view(torch.uint8)
+    t, h = Template(), torch.randn(2, H).to(bf)
+    store = type("Store", (), dict(layout=lay, num_layers=1, num_experts=1, expert_bytes=lay.total_bytes))()
+    pipe = ExpertPipeline(store, t, torch.device("cpu"), staging_buffer_a=object(), staging_buffer_b=object())
+    assert pipe._inline_fwd is None and pipe._cpp_layout_args is None
+    y = forward_from_packed(t, packed, pipe._param_refs, h)
+    g, u, d = (packed[lay.offsets[n] : lay.offsets[n] + lay.sizes[n]].view(bf).view(specs[n][0]) for n in specs)
+    assert torch.equal(y, (act or nn.functional.silu)(h @ g.t()) * (h @ u.t()) @ d.t())
+
+
 def test_make_int8():
     w, s = synth.make_int8(np.random.default_rng(0), 200, 272)
     assert w.dtype == torch.int8 and s.shape == (200,) and (w.abs().amax(1) == 127).all()

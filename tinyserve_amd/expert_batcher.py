@@ -15,7 +15,7 @@ allocate / get_packed / ``_packed``), ``store`` (copy_to_buffer), ``staging_buff
   (``expert_slot``), every expert of the layer is made resident once and the whole batch
   is one ``tsa_moe_prefill`` call: requests stacked, ids mapped to slots on the device,
   grouped by expert inside the library. No per-expert Python loop, no host sync.
-* generic path, for unquantised (bf16 / f16 / f32) experts: the reference's per-expert
+* generic path, for experts without such a layout (f32, fused 16-bit ones): the reference's per-expert
   loop, hits through ``_inline_fwd`` or ``forward_from_packed``, misses through the staging
   buffer and ``swap_weights_and_forward``, then cached.
 """
@@ -79,7 +79,7 @@ class ExpertBatcher:
         y = ops.moe_prefill(L, p.cache._packed, p.cache.expert_slot(layer_idx), idx, w, h)
         return [y[i : i + 1].to(items[i].hidden_states.dtype) for i in range(len(items))]
 
-    # ---- unquantised experts: the reference's loop over experts
+    # ---- experts without a kernel layout: the reference's loop over experts
     def _batch_execute_loop(self, items: list[BatchItem], layer_idx: int) -> list[torch.Tensor]:
         groups: dict[int, list[tuple[int, float]]] = {}
         for i, it in enumerate(items):

@@ -244,10 +244,24 @@ def dense_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | Non
     return L
 
 
+def _dense_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
+    """dense_expert_layout of a slot of separate matrices, or None where the kernels do not take it (another activation,
+    sizes that are no multiples of 32 or above 16384, matrices that are not one expert's): its template runs it."""
+    if not is_dense_layout(layout) or len(layout.specs["gate_proj"][0]) != 2 or not (act_fn is None or _is_silu(act_fn)):
+        return None
+    try:
+        L = dense_expert_layout(layout, act_fn, slot_bytes)
+    except ValueError:
+        return None
+    sizes_fit = all(n % 32 == 0 and 0 < n <= 16384 for n in (L.hidden, L.inter))
+    places_fit = all(n % 16 == 0 for n in (L.gate_off, L.up_off, L.down_off, L.slot_bytes))
+    return L if sizes_fit and places_fit else None
+
+
 def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | None = None,
                         proj_shapes: dict | None = None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
-    """The kernel-side layout of a packed expert, or None for unquantised layouts of fused matrices
-    (dense_expert_layout takes some of them)."""
+    """The kernel-side layout of a packed expert, or None for unquantised layouts that the kernels do not take, and
+    those of fused matrices (dense_expert_layout takes some of them)."""
     if "gate_up_proj_scales" in layout.specs:
         return mxfp4_expert_layout(layout, act_fn, slot_bytes)
     if is_fp8_layout(layout):
@@ -255,7 +269,7 @@ def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | No
     if is_int8_layout(layout):
         return int8_expert_layout(layout, act_fn, slot_bytes)
     if is_dense_layout(layout):
-        return dense_expert_layout(layout, act_fn, slot_bytes)
+        return _dense_layout_or_none(layout, act_fn, slot_bytes)
     if ggml_types is not None and {"gate", "up", "down"} <= set(layout.specs):
         return gguf_expert_layout(layout, ggml_types, proj_shapes, slot_bytes)
     return None
@@ -465,7 +479,8 @@ def _build_cpp_layout_args(layout: TensorLayout, act_fn):
     if is_int8_layout(layout):
         return {"layout": int8_expert_layout(layout, act_fn)}
     if is_dense_layout(layout):
-        return {"layout": dense_expert_layout(layout, act_fn)}
+        L = _dense_layout_or_none(layout, act_fn)
+        return None if L is None else {"layout": L}
     if "gate_up_proj_scales" not in layout.specs:
         return None
     return {"layout": mxfp4_expert_layout(layout, act_fn)}
@@ -484,10 +499,11 @@ def _build_fp8_inline_forward(layout: TensorLayout, act_fn):
 
 
 def _build_dense_inline_forward(layout: TensorLayout, act_fn):
-    """The same for a 16-bit or int8 slot of gate_proj / up_proj / down_proj."""
+    """The same for an int8 slot, or a 16-bit one of gate_proj / up_proj / down_proj that the kernels take."""
     if is_int8_layout(layout):
         return _layout_forward(int8_expert_layout(layout, act_fn))
-    return _layout_forward(dense_expert_layout(layout, act_fn)) if is_dense_layout(layout) else None
+    L = _dense_layout_or_none(layout, act_fn)
+    return None if L is None else _layout_forward(L)
 
 
 def _layout_forward(L: _lib.ExpertLayout):
