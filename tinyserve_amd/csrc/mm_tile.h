@@ -265,8 +265,8 @@ struct MmRuns {
 // Item `at` of the (entry, row tile) pairs of a grouped product: in bands of 2 row tiles, entry by entry. Each XCD's run is
 // then a few row tiles of every expert: a matrix's rows are read by one XCD, which shares them among its entries in
 // L2, and experts with few tokens (a stream of weights) and with many (products) are spread over all XCDs alike.
-// (8192 rows of 32 uneven experts, 5760 x 2880: 386 us with runs of whole experts in bands of 8, 366 so; bands of 1 and 4
-// measure the same.)
+// (8192 rows of 32 uneven experts, 5760 x 2880, bf16: 386 us with runs of whole experts in bands of 8, 366 so; later, bands
+// of 1 / 2 / 3 / an eighth of the row tiles 384 / 374 / 383 / 379, 24 tokens of 128 experts 46 / 44 / 49 / 49.)
 __device__ __forceinline__ void mm_pair(int at, int entries, int tiles, int& entry, int& tile) {
     constexpr int BAND = 2;
     const int band = at / (BAND * entries), in = at - band * BAND * entries, deep = tiles - BAND * band < BAND ? tiles - BAND * band : BAND;
