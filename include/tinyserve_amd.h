@@ -211,7 +211,7 @@ int tsa_int8_linear(const void* x, int x_dtype, int64_t T, int64_t K, const void
 
 /* y[r, n] = sum_k x[a, k] w[e, n, k] (+ bias[e, n], may be NULL) for the expert e with offsets[e] <= r <
  * offsets[e + 1], r < R: rows sorted by expert, any number of them for each, as tsa_group_by_expert's offsets [E + 1]
- * (ascending in [0, R]) have them. a = r, or rows[r] / top_k where rows [R] is given (tsa_group_by_expert's perm); an a
+ * (ascending in [0, R]; others are raised to the largest before them and cut to it) have them. a = r, or rows[r] / top_k where rows [R] is given (tsa_group_by_expert's perm); an a
  * outside [0, x_rows) reads a row of zeros. Rows of no expert are set to zero, and their entry of `rows` is not used.
  * x [x_rows, K] and w in dtype (BF16 or F16), w + e w_stride bytes [N, K]; float32 sums, one rounding to y_dtype; y [R, N],
  * bias [E, N]. K a multiple of 8 of at most 131056; x and w 16-byte aligned, w_stride a multiple of 16; x

@@ -228,7 +228,7 @@ def test_layouts_of_slots():
 @pytest.mark.parametrize("H,I,act", [(256, 160, nn.GELU()), (256, 160, torch.nn.functional.relu), (250, 160, None), (256, 48, nn.SiLU()),
                                      (32768, 32, None), (64, 16416, None)])
 def test_16_bit_slots_for_their_template(H, I, act):
-    """16-bit experts that the kernels do not take have no kernel layout: a pipeline runs them through its template."""
+    """16-bit experts that the kernels do not take have no kernel layout: a pipeline over them is built as before, and forward_from_packed runs its template."""
     from tinyserve_amd.expert_forward import forward_from_packed
     from tinyserve_amd.expert_pipeline import ExpertPipeline
 

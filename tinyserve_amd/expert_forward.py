@@ -246,7 +246,7 @@ def dense_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | Non
 
 def _dense_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
     """dense_expert_layout of a slot of separate matrices, or None where the kernels do not take it (another activation,
-    sizes that are no multiples of 32 or above 16384, matrices that are not one expert's): its template runs it."""
+    sizes that are no multiples of 32 or above 16384, matrices that are not one expert's): the template forwards run it."""
     if not is_dense_layout(layout) or len(layout.specs["gate_proj"][0]) != 2 or not (act_fn is None or _is_silu(act_fn)):
         return None
     try:

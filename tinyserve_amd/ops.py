@@ -358,7 +358,8 @@ def _grouped_bias(bias: torch.Tensor | None, E: int, N: int):
 def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias: torch.Tensor | None = None,
                    rows: torch.Tensor | None = None, top_k: int = 1, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y [R, N]: y[r] = x[r] @ w[e]^T (+ bias[e]) for offsets[e] <= r < offsets[e + 1], the rows sorted by expert,
-    offsets int32 [E + 1], any number for each; rows of no expert are zeros. x [T, K] and w [E, N, K] in bf16 or fp16 (an expert's matrix
+    offsets int32 [E + 1] (one that does not ascend counts as the largest before it), any number of rows for each; rows of
+    no expert are zeros. x [T, K] and w [E, N, K] in bf16 or fp16 (an expert's matrix
     contiguous, the experts any multiple of 16 bytes apart), bias [E, N]; float32 sums, y in x's dtype unless
     ``out_dtype`` says otherwise. With ``rows`` (int32 [R]), row r takes x[rows[r] // top_k]: group_by_expert's offsets and
     perm with its top_k are the tokens of a routing. K must be a multiple of 8."""
