@@ -1,0 +1,82 @@
+"""Which packed expert slots get a kernel layout, and what runs those that get none: the layout builders, the store, the
+pipeline and the batcher over int8 and 16-bit slots (CPU)."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn as nn
+
+from tinyserve_amd import _lib, synth
+from tinyserve_amd.expert_forward import (Int8ExpertModule, _build_cpp_layout_args, _build_dense_inline_forward, build_expert_layout,
+                                          int8_expert_layout)
+from tinyserve_amd.expert_pipeline import ExpertPipeline
+from tinyserve_amd.expert_store import ExpertStore, TensorLayout, pack_tensors
+
+H, I, E = 64, 32, 3
+INT8 = synth.int8_layout(H, I).specs
+
+
+def store_of(specs: dict, seed: int = 0) -> ExpertStore:
+    """One layer of E experts whose tensors are small random values (scales positive)."""
+    lay, g = TensorLayout(specs, align=16), torch.Generator().manual_seed(seed)
+    data = torch.zeros((1, E, lay.total_bytes), dtype=torch.uint8)
+    for e in range(E):
+        tensors = {}
+        for n, (shape, dt) in specs.items():
+            if dt == torch.int8:
+                tensors[n] = torch.randint(-127, 128, shape, generator=g, dtype=torch.int8)
+            elif "_scale" in n:
+                tensors[n] = (0.0005 + 0.0005 * torch.rand(shape, generator=g)).to(dt)
+            else:
+                tensors[n] = (0.05 * torch.randn(shape, generator=g)).to(dt)
+        pack_tensors(data[0, e], lay, tensors)
+    return ExpertStore(data, lay, 1, E)
+
+
+class Template(nn.Module):
+    """An expert whose parameters are the slot's tensors, computed in float32 by torch: weights times their scales (a scale
+    for each row or for groups of a row), zero points and biases where the slot has them."""
+
+    def __init__(self, specs: dict, act=nn.functional.silu, **named):
+        super().__init__()
+        for n, (shape, dt) in specs.items():
+            self.register_parameter(n, nn.Parameter(torch.zeros(shape, dtype=dt), requires_grad=False))
+        self._computes = [act]
+        for n, v in named.items():
+            setattr(self, n, v)
+
+    def _times(self, x, mat):
+        w = getattr(self, mat).float()
+        if hasattr(self, mat + "_zero_point"):
+            w = w - getattr(self, mat + "_zero_point").float().reshape(-1, 1)
+        if hasattr(self, mat + "_scale"):
+            s = getattr(self, mat + "_scale").float().reshape(w.shape[0], -1)
+            w = (w.unflatten(1, (s.shape[1], -1)) * s.unsqueeze(-1)).flatten(1)
+        y = x @ w.t()
+        return y + getattr(self, mat + "_bias").float() if hasattr(self, mat + "_bias") else y
+
+    def forward(self, h):
+        x = h.float()
+        return self._times(self._computes[0](self._times(x, "gate_proj")) * self._times(x, "up_proj"), "down_proj").to(h.dtype)
+
+
+def no_kernel(lay: TensorLayout, act=None) -> bool:
+    return build_expert_layout(lay, act) is None and _build_dense_inline_forward(lay, act) is None and _build_cpp_layout_args(lay, act) is None
+
+
+# ----------------------------------------------------------------------------- int8 slots that hold more
+@pytest.mark.parametrize("more", [{"down_proj_bias": ((H,), torch.float32)}, {"gate_proj_zero_point": ((I,), torch.int8)},
+                                  {"input_scale": ((1,), torch.float32)}])
+def test_int8_slots_with_further_tensors(more):
+    """The kernels would leave them out: no kernel layout, and no module that drops them."""
+    specs = {**INT8, **more}
+    lay = TensorLayout(specs, align=16)
+    assert no_kernel(lay)
+    for f in (int8_expert_layout, Int8ExpertModule):
+        with pytest.raises(ValueError, match="not an int8"):
+            f(lay)
+    pipe = ExpertPipeline(store_of(specs), Template(specs, _act_fn=nn.SiLU()), "cpu")
+    assert pipe._inline_fwd is None and pipe._cpp_layout_args is None
+    with pytest.raises((ValueError, NotImplementedError)):
+        pipe.kernel_layout(0)
+    assert build_expert_layout(synth.int8_layout(H, I)).format == _lib.EXPERT_INT8

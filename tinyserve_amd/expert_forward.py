@@ -175,8 +175,10 @@ def fp8_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None 
 
 
 def is_int8_layout(layout: TensorLayout) -> bool:
-    """Whether a slot holds an int8 expert: int8 gate_proj / up_proj / down_proj and their scales per row."""
-    return all(m in layout.specs and layout.specs[m][1] == torch.int8 and m + "_scale" in layout.specs for m in _MATS)
+    """Whether a slot holds an int8 expert: int8 gate_proj / up_proj / down_proj and their scales, and nothing else (the
+    kernels would leave a bias or a zero point out)."""
+    return (set(layout.specs) == {*_MATS, *(m + "_scale" for m in _MATS)}
+            and all(layout.specs[m][1] == torch.int8 for m in _MATS))
 
 
 def is_dense_layout(layout: TensorLayout) -> bool:
