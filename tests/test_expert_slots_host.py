@@ -80,3 +80,51 @@ def test_int8_slots_with_further_tensors(more):
     with pytest.raises((ValueError, NotImplementedError)):
         pipe.kernel_layout(0)
     assert build_expert_layout(synth.int8_layout(H, I)).format == _lib.EXPERT_INT8
+
+
+# ----------------------------------------------------------------------------- int8 slots that the kernels do not take
+HALF_SCALES = {n: (shape, torch.float16 if n.endswith("_scale") else dt) for n, (shape, dt) in INT8.items()}
+GROUP_SCALES = {n: ((shape[0], 2), dt) if n.endswith("_scale") else (shape, dt) for n, (shape, dt) in INT8.items()}
+UP_SCALES_FIRST = {n: INT8[n] for n in ("gate_proj", "up_proj", "down_proj", "up_proj_scale", "gate_proj_scale", "down_proj_scale")}
+
+
+@pytest.mark.parametrize("specs,act", [(INT8, nn.GELU()), (INT8, nn.functional.relu), (HALF_SCALES, None), (GROUP_SCALES, nn.SiLU()),
+                                       (UP_SCALES_FIRST, None), (synth.int8_layout(72, 40).specs, None),
+                                       (synth.int8_layout(64, 16416).specs, None), (synth.int8_layout(32768, 32).specs, nn.SiLU())])
+def test_int8_slots_for_their_template(specs, act):
+    """They have no kernel layout: a pipeline over them is built, and their template runs them."""
+    from tinyserve_amd.expert_forward import forward_from_packed
+
+    lay = TensorLayout(specs, align=16)
+    assert no_kernel(lay, act)
+    store, t = store_of(specs), Template(specs, act or nn.functional.silu, _act_fn=act)
+    pipe = ExpertPipeline(store, t, "cpu")
+    assert pipe._inline_fwd is None and pipe._cpp_layout_args is None
+    hidden = specs["gate_proj"][0][1]
+    h = torch.randn((2, hidden), generator=torch.Generator().manual_seed(1))
+    y = forward_from_packed(t, store.get_expert_data(0, 1), pipe._param_refs, h)
+    w = {n: store.get_expert_data(0, 1)[lay.offsets[n] : lay.offsets[n] + lay.sizes[n]].view(dt).view(shape).double()
+         for n, (shape, dt) in specs.items()}
+    deq = {m: w[m] * w[m + "_scale"].reshape(len(w[m]), -1).repeat_interleave(w[m].shape[1] // w[m + "_scale"].reshape(len(w[m]), -1).shape[1], 1)
+           for m in ("gate_proj", "up_proj", "down_proj")}
+    x = h.double()
+    g, u = x @ deq["gate_proj"].t(), x @ deq["up_proj"].t()
+    mid = (act or nn.functional.silu)(g) * u
+    want = mid @ deq["down_proj"].t()
+    # float32: a sum of n terms is off by n 2^-24 of the sum of its terms' magnitudes; the activations' slopes are below 2
+    n1, n2 = hidden + 4, mid.shape[1] + 4
+    eg, eu = (n1 * 2.0**-24 * (x.abs() @ deq[m].abs().t()) for m in ("gate_proj", "up_proj"))
+    emid = 2 * eg * (u.abs() + eu) + (act or nn.functional.silu)(g).abs() * eu + 8 * 2.0**-24 * (mid.abs() + g.abs() * u.abs())
+    err = emid @ deq["down_proj"].abs().t() + n2 * 2.0**-24 * ((mid.abs() + emid) @ deq["down_proj"].abs().t()) + 2.0**-24 * want.abs()
+    assert ((y.double() - want).abs() <= err).all()
+
+
+def test_int8_slots_the_kernels_take():
+    """Scales as vectors or columns, in the builders' order; act None or SiLU."""
+    column = {n: ((shape[0], 1), dt) if n.endswith("_scale") else (shape, dt) for n, (shape, dt) in INT8.items()}
+    for specs in (INT8, column):
+        for act in (None, nn.SiLU(), nn.functional.silu):
+            lay = TensorLayout(specs, align=16)
+            assert build_expert_layout(lay, act).format == _lib.EXPERT_INT8
+            assert _build_dense_inline_forward(lay, act).expert_layout.down_scales_off == lay.offsets["down_proj_scale"]
+            assert _build_cpp_layout_args(lay, act)["layout"].slot_bytes == lay.total_bytes

@@ -246,32 +246,32 @@ def dense_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | Non
     return L
 
 
-def _dense_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
-    """dense_expert_layout of a slot of separate matrices, or None where the kernels do not take it (another activation,
-    sizes that are no multiples of 32 or above 16384, matrices that are not one expert's): the template forwards run it."""
-    if not is_dense_layout(layout) or len(layout.specs["gate_proj"][0]) != 2 or not (act_fn is None or _is_silu(act_fn)):
+def _split_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
+    """The kernel layout of an int8 slot or a 16-bit one of separate matrices, or None where the kernels do not take it
+    (another activation, sizes that are no multiples of 32 or above 16384, matrices that are not one expert's, scales
+    that are not one float32 per row, tensors off 16-byte boundaries): the template forwards run it."""
+    build = int8_expert_layout if is_int8_layout(layout) else dense_expert_layout if is_dense_layout(layout) else None
+    if build is None or len(layout.specs["gate_proj"][0]) != 2 or not (act_fn is None or _is_silu(act_fn)):
         return None
     try:
-        L = dense_expert_layout(layout, act_fn, slot_bytes)
+        L = build(layout, act_fn, slot_bytes)
     except ValueError:
         return None
     sizes_fit = all(n % 32 == 0 and 0 < n <= 16384 for n in (L.hidden, L.inter))
-    places_fit = all(n % 16 == 0 for n in (L.gate_off, L.up_off, L.down_off, L.slot_bytes))
-    return L if sizes_fit and places_fit else None
+    places = [L.gate_off, L.up_off, L.down_off, L.slot_bytes] + [o for o in (L.gate_scales_off, L.down_scales_off) if o >= 0]
+    return L if sizes_fit and all(n % 16 == 0 for n in places) else None
 
 
 def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | None = None,
                         proj_shapes: dict | None = None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
-    """The kernel-side layout of a packed expert, or None for unquantised layouts that the kernels do not take, and
+    """The kernel-side layout of a packed expert, or None for int8 and unquantised layouts that the kernels do not take, and
     those of fused matrices (dense_expert_layout takes some of them)."""
     if "gate_up_proj_scales" in layout.specs:
         return mxfp4_expert_layout(layout, act_fn, slot_bytes)
     if is_fp8_layout(layout):
         return fp8_expert_layout(layout, act_fn, slot_bytes)
-    if is_int8_layout(layout):
-        return int8_expert_layout(layout, act_fn, slot_bytes)
-    if is_dense_layout(layout):
-        return _dense_layout_or_none(layout, act_fn, slot_bytes)
+    if is_int8_layout(layout) or is_dense_layout(layout):
+        return _split_layout_or_none(layout, act_fn, slot_bytes)
     if ggml_types is not None and {"gate", "up", "down"} <= set(layout.specs):
         return gguf_expert_layout(layout, ggml_types, proj_shapes, slot_bytes)
     return None
@@ -475,13 +475,12 @@ def _build_gpu_int4_forward(layout, act_fn):
 def _build_cpp_layout_args(layout: TensorLayout, act_fn):
     """Keyword arguments of fast_expert_forward for slots of this layout: the kernel layout
     of an MXFP4, FP8, int8 or 16-bit slot; None where the TensorLayout alone fixes no kernel layout (GGUF
-    slots need their ggml types, see gguf_expert_layout; fused unquantised slots run on torch)."""
+    slots need their ggml types, see gguf_expert_layout; fused unquantised slots and int8 or 16-bit ones that the
+    kernels do not take run on torch)."""
     if is_fp8_layout(layout):
         return {"layout": fp8_expert_layout(layout, act_fn)}
-    if is_int8_layout(layout):
-        return {"layout": int8_expert_layout(layout, act_fn)}
-    if is_dense_layout(layout):
-        L = _dense_layout_or_none(layout, act_fn)
+    if is_int8_layout(layout) or is_dense_layout(layout):
+        L = _split_layout_or_none(layout, act_fn)
         return None if L is None else {"layout": L}
     if "gate_up_proj_scales" not in layout.specs:
         return None
@@ -501,10 +500,8 @@ def _build_fp8_inline_forward(layout: TensorLayout, act_fn):
 
 
 def _build_dense_inline_forward(layout: TensorLayout, act_fn):
-    """The same for an int8 slot, or a 16-bit one of gate_proj / up_proj / down_proj that the kernels take."""
-    if is_int8_layout(layout):
-        return _layout_forward(int8_expert_layout(layout, act_fn))
-    L = _dense_layout_or_none(layout, act_fn)
+    """The same for an int8 slot, or a 16-bit one of gate_proj / up_proj / down_proj, that the kernels take."""
+    L = _split_layout_or_none(layout, act_fn)
     return None if L is None else _layout_forward(L)
 
 
