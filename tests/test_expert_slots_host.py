@@ -8,7 +8,7 @@ import torch.nn as nn
 
 from tinyserve_amd import _lib, synth
 from tinyserve_amd.expert_forward import (Int8ExpertModule, _build_cpp_layout_args, _build_dense_inline_forward, build_expert_layout,
-                                          int8_expert_layout)
+                                          int8_expert_layout, template_activation)
 from tinyserve_amd.expert_pipeline import ExpertPipeline
 from tinyserve_amd.expert_store import ExpertStore, TensorLayout, pack_tensors
 
@@ -128,3 +128,48 @@ def test_int8_slots_the_kernels_take():
             assert build_expert_layout(lay, act).format == _lib.EXPERT_INT8
             assert _build_dense_inline_forward(lay, act).expert_layout.down_scales_off == lay.offsets["down_proj_scale"]
             assert _build_cpp_layout_args(lay, act)["layout"].slot_bytes == lay.total_bytes
+
+
+# ----------------------------------------------------------------------------- the template's activation
+DENSE = {dt: synth.dense_layout(H, I, dt).specs for dt in (torch.bfloat16, torch.float16)}
+SPLIT = [INT8, DENSE[torch.bfloat16], DENSE[torch.float16]]
+
+
+@pytest.mark.parametrize("specs", SPLIT)
+@pytest.mark.parametrize("named", [{}, {"act_fn": nn.GELU()}, {"_act_fn": None}, {"activation_fn": nn.functional.gelu},
+                                   {"activation": nn.ReLU()}, {"_act_fn": nn.GELU(), "act_fn": nn.SiLU()}, {"_act_fn": None, "act_fn": nn.Tanh()}])
+def test_templates_that_do_not_name_silu(specs, named):
+    """The kernels compute SiLU: a template with another activation, whatever it calls it, is not replaced by them."""
+    pipe = ExpertPipeline(store_of(specs), Template(specs, nn.functional.gelu, **named), "cpu")
+    assert pipe._inline_fwd is None and pipe._cpp_layout_args is None
+    with pytest.raises(NotImplementedError, match="activation"):
+        pipe.kernel_layout(0)
+
+
+@pytest.mark.parametrize("specs", SPLIT)
+@pytest.mark.parametrize("named", [{"_act_fn": nn.SiLU()}, {"act_fn": nn.SiLU()}, {"_act_fn": None, "act_fn": nn.functional.silu},
+                                   {"activation": nn.SiLU()}, None])
+def test_templates_that_name_silu(specs, named):
+    """They are, and so are slots without a template."""
+    pipe = ExpertPipeline(store_of(specs), None if named is None else Template(specs, **named), "cpu")
+    L = pipe.kernel_layout(0)
+    assert L.format in (_lib.EXPERT_INT8, _lib.EXPERT_DENSE) and L.act == _lib.ACT_SILU
+    assert pipe._inline_fwd.expert_layout.format == L.format and pipe._cpp_layout_args["layout"].format == L.format
+
+
+def test_own_template():
+    lay = synth.int8_layout(H, I)
+    t = Int8ExpertModule(lay, device="cpu")
+    pipe = ExpertPipeline(store_of(INT8), t, "cpu")
+    assert pipe.kernel_layout(0).format == _lib.EXPERT_INT8 and pipe._inline_fwd is not None
+    assert set(t.state_dict()) == set(INT8) and not list(t.children())
+
+
+def test_activations_of_other_formats():
+    """MXFP4, FP8 and fused slots take the template's _act_fn alone, as they did."""
+    for lay in (synth.mxfp4_layout(64, 64), synth.fp8_layout(64, 32), TensorLayout({"gate_up_proj": ((64, 64), torch.bfloat16), "down_proj": ((64, 32), torch.bfloat16)})):
+        t = nn.Module()
+        t.act_fn = nn.GELU()
+        assert template_activation(t, lay) is None and template_activation(None, lay) is None
+        t._act_fn = nn.SiLU()
+        assert template_activation(t, lay) is t._act_fn

@@ -262,6 +262,25 @@ def _split_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | N
     return L if sizes_fit and all(n % 16 == 0 for n in places) else None
 
 
+class _Unnamed:
+    """In an activation's place: no SiLU, and no other either."""
+
+    def __repr__(self):
+        return "<none that the template names as its _act_fn or act_fn>"
+
+
+def template_activation(template: nn.Module | None, layout: TensorLayout):
+    """What the layout builders take as ``act_fn`` for slots whose expert a template computes: its ``_act_fn``. Int8 slots and
+    16-bit ones of separate matrices come with any activation, so for them None, which the builders take as SiLU, is
+    left to calls without a template: a template has to name SiLU, as ``_act_fn``, ``act_fn`` (as transformers' modules
+    do), ``activation_fn`` or ``activation``, for the kernels to stand in for it."""
+    act = getattr(template, "_act_fn", None)
+    if template is None or act is not None or not (is_int8_layout(layout) or is_dense_layout(layout)):
+        return act
+    named = (getattr(template, n, None) for n in ("act_fn", "activation_fn", "activation"))
+    return next((a for a in named if a is not None), _Unnamed())
+
+
 def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | None = None,
                         proj_shapes: dict | None = None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
     """The kernel-side layout of a packed expert, or None for int8 and unquantised layouts that the kernels do not take, and
@@ -413,6 +432,7 @@ class Int8ExpertModule(Int8Module):
         for name, (shape, dtype) in layout.specs.items():
             self.register_parameter(name, nn.Parameter(torch.zeros(shape, dtype=dtype, device=device),
                                                        requires_grad=False))
+        self._act_fn = F.silu
 
     def forward(self, h: torch.Tensor) -> torch.Tensor:
         g = ops.int8_linear(h, self.gate_proj, self.gate_proj_scale, out_dtype=torch.float32)

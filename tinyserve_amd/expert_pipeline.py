@@ -34,7 +34,7 @@ from . import ops
 from .expert_cache import ExpertCache
 from .expert_forward import (_build_cpp_layout_args, _build_dense_inline_forward, _build_fp8_inline_forward,
                              _build_gpu_int4_forward, _build_inline_forward, _build_mxfp4_inline_forward,
-                             _precompute_param_refs, mxfp4_expert_layout)
+                             _precompute_param_refs, mxfp4_expert_layout, template_activation)
 
 
 class ExpertPipeline:
@@ -79,12 +79,13 @@ class ExpertPipeline:
         else:
             self._act_fn = getattr(template, "_act_fn", None)
             self._param_refs = _precompute_param_refs(template, store.layout) if template is not None else None
+            self._kernel_act = template_activation(template, self.cache_layout)
             self._inline_fwd = (_build_inline_forward(store.layout, self._act_fn)
                                 or _build_mxfp4_inline_forward(self.cache_layout, self._act_fn)
                                 or _build_fp8_inline_forward(self.cache_layout, self._act_fn)
-                                or _build_dense_inline_forward(self.cache_layout, self._act_fn)
+                                or _build_dense_inline_forward(self.cache_layout, self._kernel_act)
                                 or _build_gpu_int4_forward(store.layout, self._act_fn))
-            self._cpp_layout_args = _build_cpp_layout_args(self.cache_layout, self._act_fn)
+            self._cpp_layout_args = _build_cpp_layout_args(self.cache_layout, self._kernel_act)
         self._kernel_layouts: dict[int, object] = {}
         self._decode_ws: dict[tuple, torch.Tensor] = {}
 
@@ -125,7 +126,7 @@ class ExpertPipeline:
             elif self._tiled_layout is not None:
                 L = mxfp4_expert_layout(self._tiled_layout, self._act_fn, self.cache.expert_bytes, tiled=True)
             else:
-                L = self.store.expert_layout(self._act_fn)
+                L = self.store.expert_layout(self._kernel_act)
             self._kernel_layouts[layer_idx] = L
         return L
 
