@@ -173,3 +173,22 @@ def test_activations_of_other_formats():
         assert template_activation(t, lay) is None and template_activation(None, lay) is None
         t._act_fn = nn.SiLU()
         assert template_activation(t, lay) is t._act_fn
+
+
+@pytest.mark.parametrize("specs", SPLIT)
+@pytest.mark.parametrize("how", ["parameter", "buffer", "module"])
+def test_templates_with_further_tensors(specs, how):
+    """Biases, scales or adapters that the template holds itself, for all experts: the kernels would leave them out."""
+    t = Template(specs, _act_fn=nn.SiLU())
+    if how == "parameter":
+        t.down_proj_bias = nn.Parameter(torch.ones(H))
+    elif how == "buffer":
+        t.register_buffer("smooth", torch.ones(H))
+    else:
+        t.adapter = nn.Linear(H, 4)
+    pipe = ExpertPipeline(store_of(specs), t, "cpu")
+    assert pipe._inline_fwd is None and pipe._cpp_layout_args is None
+    with pytest.raises(NotImplementedError, match="not in the slot"):
+        pipe.kernel_layout(0)
+    t.__delattr__({"parameter": "down_proj_bias", "buffer": "smooth", "module": "adapter"}[how])
+    assert ExpertPipeline(store_of(specs), t, "cpu").kernel_layout(0).act == _lib.ACT_SILU

@@ -262,23 +262,30 @@ def _split_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | N
     return L if sizes_fit and all(n % 16 == 0 for n in places) else None
 
 
-class _Unnamed:
-    """In an activation's place: no SiLU, and no other either."""
+class _NotSilu:
+    """In an activation's place: why the kernels cannot stand in for a template."""
+
+    def __init__(self, why: str):
+        self._why = why
 
     def __repr__(self):
-        return "<none that the template names as its _act_fn or act_fn>"
+        return f"<{self._why}>"
 
 
 def template_activation(template: nn.Module | None, layout: TensorLayout):
     """What the layout builders take as ``act_fn`` for slots whose expert a template computes: its ``_act_fn``. Int8 slots and
     16-bit ones of separate matrices come with any activation, so for them None, which the builders take as SiLU, is
     left to calls without a template: a template has to name SiLU, as ``_act_fn``, ``act_fn`` (as transformers' modules
-    do), ``activation_fn`` or ``activation``, for the kernels to stand in for it."""
+    do), ``activation_fn`` or ``activation``, for the kernels to stand in for it, and have no parameters or buffers
+    besides the slot's tensors (biases, adapters), which they would leave out."""
     act = getattr(template, "_act_fn", None)
-    if template is None or act is not None or not (is_int8_layout(layout) or is_dense_layout(layout)):
+    if template is None or not (is_int8_layout(layout) or is_dense_layout(layout)):
         return act
-    named = (getattr(template, n, None) for n in ("act_fn", "activation_fn", "activation"))
-    return next((a for a in named if a is not None), _Unnamed())
+    further = sorted({n for n, _ in (*template.named_parameters(), *template.named_buffers())} - set(layout.specs))
+    if further:
+        return _NotSilu(f"in a template with tensors that are not in the slot: {', '.join(further[:4])}")
+    named = (getattr(template, n, None) for n in ("_act_fn", "act_fn", "activation_fn", "activation"))
+    return next((a for a in named if a is not None), _NotSilu("none that the template names as its _act_fn or act_fn"))
 
 
 def build_expert_layout(layout: TensorLayout, act_fn=None, ggml_types: dict | None = None,
