@@ -7,6 +7,7 @@ import torch
 import torch.nn as nn
 
 from tinyserve_amd import _lib, synth
+from tinyserve_amd.expert_batcher import BatchItem, ExpertBatcher
 from tinyserve_amd.expert_forward import (Int8ExpertModule, _build_cpp_layout_args, _build_dense_inline_forward, build_expert_layout,
                                           int8_expert_layout, template_activation)
 from tinyserve_amd.expert_pipeline import ExpertPipeline
@@ -60,6 +61,25 @@ class Template(nn.Module):
         return self._times(self._computes[0](self._times(x, "gate_proj")) * self._times(x, "up_proj"), "down_proj").to(h.dtype)
 
 
+def expert64(store: ExpertStore, e: int, h: torch.Tensor, act=None):
+    """(expert e of h in 64 bits, how far float32 may be off): a sum of n terms is off by n 2^-24 of the sum of its terms'
+    magnitudes, and the activations' slopes are below 2."""
+    lay, act = store.layout, act or nn.functional.silu
+    w = {n: store.get_expert_data(0, e)[lay.offsets[n] : lay.offsets[n] + lay.sizes[n]].view(dt).view(shape).double()
+         for n, (shape, dt) in lay.specs.items()}
+    for m in ("gate_proj", "up_proj", "down_proj"):
+        if m + "_scale" in w:
+            s = w[m + "_scale"].reshape(len(w[m]), -1)
+            w[m] = w[m] * s.repeat_interleave(w[m].shape[1] // s.shape[1], 1)
+    x = h.double()
+    g, u = x @ w["gate_proj"].t(), x @ w["up_proj"].t()
+    mid, down = act(g) * u, w["down_proj"].t()
+    want, n1, n2 = mid @ down, x.shape[1] + 4, mid.shape[1] + 4
+    eg, eu = (n1 * 2.0**-24 * (x.abs() @ w[m].abs().t()) for m in ("gate_proj", "up_proj"))
+    emid = 2 * eg * (u.abs() + eu) + act(g).abs() * eu + 8 * 2.0**-24 * (mid.abs() + g.abs() * u.abs())
+    return want, emid @ down.abs() + n2 * 2.0**-24 * ((mid.abs() + emid) @ down.abs()) + 2.0**-24 * want.abs()
+
+
 def no_kernel(lay: TensorLayout, act=None) -> bool:
     return build_expert_layout(lay, act) is None and _build_dense_inline_forward(lay, act) is None and _build_cpp_layout_args(lay, act) is None
 
@@ -103,19 +123,7 @@ def test_int8_slots_for_their_template(specs, act):
     hidden = specs["gate_proj"][0][1]
     h = torch.randn((2, hidden), generator=torch.Generator().manual_seed(1))
     y = forward_from_packed(t, store.get_expert_data(0, 1), pipe._param_refs, h)
-    w = {n: store.get_expert_data(0, 1)[lay.offsets[n] : lay.offsets[n] + lay.sizes[n]].view(dt).view(shape).double()
-         for n, (shape, dt) in specs.items()}
-    deq = {m: w[m] * w[m + "_scale"].reshape(len(w[m]), -1).repeat_interleave(w[m].shape[1] // w[m + "_scale"].reshape(len(w[m]), -1).shape[1], 1)
-           for m in ("gate_proj", "up_proj", "down_proj")}
-    x = h.double()
-    g, u = x @ deq["gate_proj"].t(), x @ deq["up_proj"].t()
-    mid = (act or nn.functional.silu)(g) * u
-    want = mid @ deq["down_proj"].t()
-    # float32: a sum of n terms is off by n 2^-24 of the sum of its terms' magnitudes; the activations' slopes are below 2
-    n1, n2 = hidden + 4, mid.shape[1] + 4
-    eg, eu = (n1 * 2.0**-24 * (x.abs() @ deq[m].abs().t()) for m in ("gate_proj", "up_proj"))
-    emid = 2 * eg * (u.abs() + eu) + (act or nn.functional.silu)(g).abs() * eu + 8 * 2.0**-24 * (mid.abs() + g.abs() * u.abs())
-    err = emid @ deq["down_proj"].abs().t() + n2 * 2.0**-24 * ((mid.abs() + emid) @ deq["down_proj"].abs().t()) + 2.0**-24 * want.abs()
+    want, err = expert64(store, 1, h, act)
     assert ((y.double() - want).abs() <= err).all()
 
 
@@ -192,3 +200,43 @@ def test_templates_with_further_tensors(specs, how):
         pipe.kernel_layout(0)
     t.__delattr__({"parameter": "down_proj_bias", "buffer": "smooth", "module": "adapter"}[how])
     assert ExpertPipeline(store_of(specs), t, "cpu").kernel_layout(0).act == _lib.ACT_SILU
+
+
+# ----------------------------------------------------------------------------- the store's layout, and the batcher
+UNTAKEN = [(DENSE[torch.bfloat16], nn.GELU(), {"_act_fn": nn.GELU()}), (DENSE[torch.float16], nn.functional.relu, {"act_fn": nn.functional.relu}),
+           (synth.dense_layout(72, 40).specs, None, {"_act_fn": nn.SiLU()}), (synth.int8_layout(72, 40).specs, None, {"act_fn": nn.SiLU()}),
+           (INT8, nn.functional.gelu, {}), (GROUP_SCALES, None, {"_act_fn": nn.SiLU()}),
+           ({n: (shape, torch.float32) for n, (shape, _) in DENSE[torch.bfloat16].items()}, None, {"_act_fn": nn.SiLU()})]
+
+
+@pytest.mark.parametrize("specs,act,named", UNTAKEN)
+def test_batches_over_slots_the_kernels_do_not_take(specs, act, named):
+    """The batcher over the framework's own pipeline runs the loop over experts and their template: experts that are not
+    cached yet, then cached ones."""
+    store = store_of(specs)
+    pipe = ExpertPipeline(store, Template(specs, act or nn.functional.silu, **named), "cpu")
+    g = torch.Generator().manual_seed(3)
+    chosen = [torch.tensor(c) for c in ([0, 2], [2, 1], [1, 1], [2, 0])]
+    items = [BatchItem(torch.randn((1, specs["gate_proj"][0][1]), generator=g), c, torch.rand(2, generator=g), i) for i, c in enumerate(chosen)]
+    for _ in range(2):
+        for it, y in zip(items, pipe.execute_batched_experts(items, 0)):
+            want, err = torch.zeros(()), torch.zeros(())
+            for e, w in zip(it.expert_indices.tolist(), it.routing_weights.double()):
+                v, d = expert64(store, e, it.hidden_states, act)
+                want, err = want + w * v, err + w * (d + 3 * 2.0**-24 * (v.abs() + d))
+            assert ((y.double() - want).abs() <= err).all()
+    assert pipe.cache.hits == 3 and pipe.cache.misses == 3
+
+
+@pytest.mark.parametrize("specs,act", [(s, a) for s, a, _ in UNTAKEN])
+def test_store_and_builders_agree(specs, act):
+    """Where build_expert_layout has none, the store's layout is refused, and a batch without a template too."""
+    store = store_of(specs)
+    assert build_expert_layout(store.layout, act) is None
+    with pytest.raises((ValueError, NotImplementedError)):
+        store.expert_layout(act)
+    if act is None:
+        pipe = ExpertPipeline(store, None, "cpu")
+        item = BatchItem(torch.zeros((1, specs["gate_proj"][0][1])), torch.tensor([0]), torch.ones(1), 0)
+        with pytest.raises((ValueError, NotImplementedError)):
+            ExpertBatcher(pipe).batch_execute([item], 0)

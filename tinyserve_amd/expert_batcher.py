@@ -15,9 +15,10 @@ allocate / get_packed / ``_packed``), ``store`` (copy_to_buffer), ``staging_buff
   (``expert_slot``), every expert of the layer is made resident once and the whole batch
   is one ``tsa_moe_prefill`` call: requests stacked, ids mapped to slots on the device,
   grouped by expert inside the library. No per-expert Python loop, no host sync.
-* generic path, for experts without such a layout (f32, fused 16-bit ones): the reference's per-expert
-  loop, hits through ``_inline_fwd`` or ``forward_from_packed``, misses through the staging
-  buffer and ``swap_weights_and_forward``, then cached.
+* generic path, for experts without such a layout (f32, fused 16-bit ones, int8 and 16-bit ones of
+  activations or sizes that the kernels do not take): the reference's per-expert loop, hits through
+  ``_inline_fwd`` or ``forward_from_packed``, misses through the staging buffer and
+  ``swap_weights_and_forward``, then cached.
 """
 from __future__ import annotations
 
@@ -46,7 +47,13 @@ class ExpertBatcher:
         if not hasattr(getattr(p, "cache", None), "expert_slot"):
             return None
         if hasattr(p, "kernel_layout"):
-            return p.kernel_layout(layer_idx)
+            try:
+                return p.kernel_layout(layer_idx)
+            except (NotImplementedError, ValueError):
+                # slots that the kernels do not take: the loop, which needs a template
+                if getattr(p, "template", None) is None or getattr(p, "_param_refs", None) is None:
+                    raise
+                return None
         return getattr(getattr(p, "_inline_fwd", None), "expert_layout", None)
 
     def _make_resident(self, layer_idx: int) -> None:

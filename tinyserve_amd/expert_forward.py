@@ -190,6 +190,8 @@ def _plain_layout(fmt: int, layout: TensorLayout, act_fn, slot_bytes: int | None
     """The fields that 16-bit and int8 slots of gate_proj / up_proj / down_proj share, checked."""
     if act_fn is not None and not _is_silu(act_fn):
         raise NotImplementedError(f"unsupported activation {act_fn!r}")
+    if len(layout.specs["gate_proj"][0]) != 2:
+        raise ValueError(f"inconsistent {what} expert shapes: gate_proj {layout.specs['gate_proj']} is no matrix")
     (I, H), off = layout.specs["gate_proj"][0], layout.offsets
     for m, shape in (("gate_proj", (I, H)), ("up_proj", (I, H)), ("down_proj", (H, I))):
         if tuple(layout.specs[m][0]) != shape or layout.specs[m][1] != layout.specs["gate_proj"][1]:
@@ -203,6 +205,16 @@ def _plain_layout(fmt: int, layout: TensorLayout, act_fn, slot_bytes: int | None
     L.gate_bias_off = L.down_bias_off = -1
     L.bias_dtype = _lib.BF16
     L.swiglu_limit, L.swiglu_alpha = _SWIGLU_LIMIT, _QUICK_GELU_COEFF
+    return L
+
+
+def _taken(L: _lib.ExpertLayout, what: str) -> _lib.ExpertLayout:
+    """L, if its sizes and places are ones that the kernels of 16-bit and int8 experts take."""
+    if any(n % 32 or not 0 < n <= 16384 for n in (L.hidden, L.inter)):
+        raise ValueError(f"{what} experts: hidden ({L.hidden}) and inter ({L.inter}) must be multiples of 32, at most 16384")
+    places = [L.gate_off, L.up_off, L.down_off, L.slot_bytes] + [o for o in (L.gate_scales_off, L.down_scales_off) if o >= 0]
+    if any(n % 16 for n in places):
+        raise ValueError(f"{what} experts: tensors and slots must start on multiples of 16 bytes, got {places}")
     return L
 
 
@@ -221,7 +233,7 @@ def int8_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None
     if off["up_proj_scale"] != off["gate_proj_scale"] + layout.sizes["gate_proj_scale"]:
         raise ValueError("up_proj_scale must follow gate_proj_scale in the slot")
     L.gate_scales_off, L.down_scales_off = off["gate_proj_scale"], off["down_proj_scale"]
-    return L
+    return _taken(L, "int8")
 
 
 def dense_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout:
@@ -243,7 +255,7 @@ def dense_expert_layout(layout: TensorLayout, act_fn=None, slot_bytes: int | Non
     else:
         raise ValueError(f"not a 16-bit expert slot: {specs}")
     L.gate_type = L.up_type = L.down_type = _lib.tsa_dtype(dt)
-    return L
+    return _taken(L, "16-bit")
 
 
 def _split_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | None = None) -> _lib.ExpertLayout | None:
@@ -251,15 +263,10 @@ def _split_layout_or_none(layout: TensorLayout, act_fn=None, slot_bytes: int | N
     (another activation, sizes that are no multiples of 32 or above 16384, matrices that are not one expert's, scales
     that are not one float32 per row, tensors off 16-byte boundaries): the template forwards run it."""
     build = int8_expert_layout if is_int8_layout(layout) else dense_expert_layout if is_dense_layout(layout) else None
-    if build is None or len(layout.specs["gate_proj"][0]) != 2 or not (act_fn is None or _is_silu(act_fn)):
-        return None
     try:
-        L = build(layout, act_fn, slot_bytes)
-    except ValueError:
+        return build(layout, act_fn, slot_bytes) if build else None
+    except (NotImplementedError, ValueError):
         return None
-    sizes_fit = all(n % 32 == 0 and 0 < n <= 16384 for n in (L.hidden, L.inter))
-    places = [L.gate_off, L.up_off, L.down_off, L.slot_bytes] + [o for o in (L.gate_scales_off, L.down_scales_off) if o >= 0]
-    return L if sizes_fit and all(n % 16 == 0 for n in places) else None
 
 
 class _NotSilu:

@@ -247,7 +247,8 @@ class ExpertStore:
         return self._data[layer_idx].to(device)
 
     def expert_layout(self, act_fn=None):
-        """The kernels' tsa_expert_layout of these slots."""
+        """The kernels' tsa_expert_layout of these slots; ValueError or NotImplementedError where the kernels do not take
+        them."""
         from .expert_forward import (dense_expert_layout, fp8_expert_layout, int8_expert_layout, is_fp8_layout, is_int8_layout,
                                      mxfp4_expert_layout)
 
