@@ -280,7 +280,8 @@ using TileD = MmTile<4, 1, 2, 4, 3>;  // 128 x 64
 
 // The tile (A .. D as 0 .. 3) with the least time, where a CU that works on 1 .. `per` tiles at once takes cost[0 .. per - 1]
 // for them, and on more in rounds; -1 if every tile gives 2^30 of them or more. (us of a product of K 2880 to 4096. Over the shapes of N 512
-// to 8192 and 33 to 8192 tokens that were measured: within 6% of the best tile but for a few of fewer than 100 tokens.)
+// to 8192 and 33 to 8192 tokens that were measured: within 6% of the best tile but for a few of fewer than 100 tokens. K scales
+// all four alike but for what a tile costs apart from its steps; other K were not measured.)
 struct GemmTile { int rows, tok, per, cost[2]; };
 constexpr GemmTile gemm_tiles[4] = {{TileA::RN, TileA::TM, 1, {43}},
                                     {TileB::RN, TileB::TM, 1, {25}},
@@ -412,7 +413,8 @@ extern "C" int tsa_int8_matmul(const void* codes, const float* scales, int64_t T
 // itself 3.3 us of host time (9.7 to 10 us, whatever the sizes), while every group of 8 tokens here adds a load latency and
 // its arithmetic to every workgroup. us of one launch / two: calls one by one, 2880 x 2880, 2048 x 4096 and 5760 x 2880, 8 tokens
 // 6.3, 7.2 and 8.0 / 9.7, 12 tokens 7.0, 8.0 and 9.6 / 9.7, 16 tokens 8.0, 9.3 and 10.9 / 9.8; inside a graph, 8 tokens 7.0, 8.0 and
-// 8.8 / 7.1, 8.7 and 8.9, 12 tokens 7.8, 8.9 and 10.5 / 7.3, 9.1 and 9.1.
+// 8.8 / 7.1, 8.7 and 8.9, 12 tokens 7.8, 8.9 and 10.5 / 7.3, 9.1 and 9.1. The rule goes by calls made one by one: inside a graph it costs
+// up to 1.4 us at 12 tokens.
 static bool linear_in_one(int64_t T, int64_t K) { return T <= 12 && i8r_lds(0, 1, K, (int)T) <= 128 * 1024; }
 static int64_t linear_ws(int64_t T, int64_t K) { return linear_in_one(T, K) ? 0 : (T * K + 255) / 256 * 256 + T * 4; }
 

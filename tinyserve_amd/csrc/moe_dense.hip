@@ -512,7 +512,8 @@ bool dense_format(const tsa_expert_layout& L) { return L.format == TSA_EXPERT_DE
 // routing: hidden 2048, 128 experts top-8, 2 / 3 / 4 / 8 tokens, bf16 (9.4 MB an expert) 39 / 43 / 47 / 56 and 34 / 46 / 58 / 105, int8 33 /
 // 35 / 38 / 44 and 24 / 32 / 40 / 72; hidden 2880, 32 experts top-4, 2 / 3 / 4 tokens, bf16 (50 MB) 82 / 87 / 91 and 74 / 102 / 130, int8 62 /
 // 62 / 65 and 57 / 76 / 96; hidden 1440, 20 experts top-3, int8 (3.2 MB), 6 / 8 tokens 28 / 28 and 27 / 33; hidden 1024, 16 experts top-2, bf16
-// (3.1 MB), 12 / 16 tokens 26 / 26 and 27 / 34; hidden 256, 64 experts top-4 (0.25 MB), 16 / 24 tokens 18 / 18 and 12 / 15.
+// (3.1 MB), 12 / 16 tokens 26 / 26 and 27 / 34; hidden 256, 64 experts top-4 (0.25 MB), 16 / 24 tokens 18 / 18 and 12 / 15. (T k stops at
+// 64 all the same, where experts as small as the last would gain 3 us more.)
 int64_t dense_pair_tokens(const tsa_expert_layout& L, int k) {
     const int64_t expert = 3 * L.hidden * L.inter * (L.format == TSA_EXPERT_INT8 ? 1 : 2), bytes = ((int64_t)72 << 20) / (k * expert), few = 64 / k;
     const int64_t most = bytes < few ? bytes : few;
