@@ -240,3 +240,14 @@ def test_store_and_builders_agree(specs, act):
         item = BatchItem(torch.zeros((1, specs["gate_proj"][0][1])), torch.tensor([0]), torch.ones(1), 0)
         with pytest.raises((ValueError, NotImplementedError)):
             ExpertBatcher(pipe).batch_execute([item], 0)
+
+
+@pytest.mark.parametrize("specs", SPLIT)
+def test_templates_that_are_no_modules(specs):
+    """Any callable with the slot's tensors as attributes serves as a template."""
+    from types import SimpleNamespace
+
+    params = {n: nn.Parameter(torch.zeros(shape, dtype=dt), requires_grad=False) for n, (shape, dt) in specs.items()}
+    pipe = ExpertPipeline(store_of(specs), SimpleNamespace(**params), "cpu")
+    assert pipe._inline_fwd is None and len(pipe._param_refs) == len(specs)
+    assert ExpertPipeline(store_of(specs), SimpleNamespace(**params, _act_fn=nn.SiLU()), "cpu").kernel_layout(0).act == _lib.ACT_SILU

@@ -279,7 +279,7 @@ class _NotSilu:
         return f"<{self._why}>"
 
 
-def template_activation(template: nn.Module | None, layout: TensorLayout):
+def template_activation(template, layout: TensorLayout):
     """What the layout builders take as ``act_fn`` for slots whose expert a template computes: its ``_act_fn``. Int8 slots and
     16-bit ones of separate matrices come with any activation, so for them None, which the builders take as SiLU, is
     left to calls without a template: a template has to name SiLU, as ``_act_fn``, ``act_fn`` (as transformers' modules
@@ -288,7 +288,8 @@ def template_activation(template: nn.Module | None, layout: TensorLayout):
     act = getattr(template, "_act_fn", None)
     if template is None or not (is_int8_layout(layout) or is_dense_layout(layout)):
         return act
-    further = sorted({n for n, _ in (*template.named_parameters(), *template.named_buffers())} - set(layout.specs))
+    held = (*template.named_parameters(), *template.named_buffers()) if isinstance(template, nn.Module) else ()
+    further = sorted({n for n, _ in held} - set(layout.specs))
     if further:
         return _NotSilu(f"in a template with tensors that are not in the slot: {', '.join(further[:4])}")
     named = (getattr(template, n, None) for n in ("_act_fn", "act_fn", "activation_fn", "activation"))
